@@ -1,0 +1,395 @@
+"""The 4-bit operators and the few-token expert layer, as measurable cases.
+
+``fp4``      quantise rows to microscaled 4-bit floats and read them back
+``linear``   a dense projection in w4a4: quantise the rows, multiply with 4-bit weights
+``experts``  a mixture-of-experts layer in w4a4, a prompt's worth of tokens
+``decode``   a whole mixture-of-experts layer for a few decoding tokens
+
+Layer shapes are those of this repository's benchmark.
+"""
+import math
+
+import torch
+
+own = False
+
+FP8 = torch.float8_e4m3fn
+
+# E experts, K routes per token, H hidden size, I intermediate size
+SMALL = dict(E=8, K=2, H=1024, I=512)
+MIXTRAL = dict(E=8, K=2, H=4096, I=14336)
+DEEPSEEK = dict(E=256, K=8, H=7168, I=2048)
+QWEN_30B = dict(E=128, K=8, H=2048, I=768)
+QWEN_235B = dict(E=128, K=8, H=4096, I=1536)
+
+
+def listed():
+    return [
+        # one token's row on its way into a 4-bit projection: latency alone
+        dict(op="fp4", name="fp4_one_row", fmt="nvfp4", dtype="bf16", M=1, H=7168, scaled=True),
+        # a prefill batch, read once and written at a quarter of its size
+        dict(op="fp4", name="fp4_rows", fmt="mxfp4", dtype="bf16", M=8192, H=7168, scaled=False),
+        # projections of one and of a few sequences: the weights' bytes are the time
+        dict(op="linear", name="linear_one", fmt="nvfp4", dtype="bf16", M=1, N=4096, H=7168),
+        dict(op="linear", name="linear_few", fmt="mxfp4", dtype="f16", M=23, N=7168, H=2048),
+        # a ragged prefill batch, and a full one that the tensor cores bound
+        dict(op="linear", name="linear_ragged", fmt="mxfp4", dtype="bf16", M=777, N=4096, H=7168),
+        dict(op="linear", name="linear_full", fmt="nvfp4", dtype="bf16", M=8192, N=7168, H=4096),
+        # expert layers of a prompt: a quarter of 256 experts on this GPU; many small experts
+        dict(DEEPSEEK, op="experts", name="experts_prefill", fmt="nvfp4", E=64, M=1500),
+        dict(QWEN_235B, op="experts", name="experts_chunk", fmt="mxfp4", M=333),
+        # a test-sized layer, two sequences: nothing but launches and latency
+        dict(SMALL, op="decode", name="decode_small", kind="bf16", M=2, router=True),
+        # 8-bit block-scaled experts, one sequence (batch-1 latency), routed inside
+        dict(DEEPSEEK, op="decode", name="decode_one", kind="fp8_block", M=1, router=True),
+        # 8-bit integer experts with per-channel scales, some sequences, many small experts
+        dict(QWEN_30B, op="decode", name="decode_int8", kind="int8_channel", M=5, router=False),
+        # 4-bit experts, eight sequences that touch a quarter of 256 experts
+        dict(DEEPSEEK, op="decode", name="decode_fp4", kind="nvfp4", M=8, router=False),
+    ]
+
+
+def _between(rng, low, high):
+    """A whole number spread evenly over the logarithm of [low, high]."""
+    return max(low, min(high, int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))))
+
+
+def draw(rng):
+    """One more case: an operator, then sizes anywhere in its range."""
+    op = rng.choice(("fp4", "linear", "experts", "decode", "decode"))
+    fmt = rng.choice(("nvfp4", "mxfp4"))
+    if op == "fp4":
+        step = 16 if fmt == "nvfp4" else 32
+        h = step * _between(rng, 1, 8192 // step)
+        return dict(op=op, fmt=fmt, dtype=rng.choice(("bf16", "f16", "f32")), H=h,
+                    M=_between(rng, 1, 8192), scaled=fmt == "nvfp4" and rng.random() < 0.5)
+    if op == "linear":
+        step = 64 if fmt == "nvfp4" else 128
+        return dict(op=op, fmt=fmt, dtype=rng.choice(("bf16", "f16")), M=_between(rng, 1, 8192),
+                    N=_between(rng, 1, 7168), H=step * _between(rng, 1, 7168 // step))
+    if op == "experts":
+        model = rng.choice((SMALL, QWEN_30B, QWEN_235B, dict(DEEPSEEK, E=32)))
+        return dict(model, op=op, fmt=fmt, M=_between(rng, 1, 1024))
+    model = rng.choice((SMALL, MIXTRAL, DEEPSEEK, QWEN_30B, QWEN_235B))
+    kind = rng.choice(("bf16", "f16", "fp8_block", "int8_channel", "nvfp4", "mxfp4"))
+    if model is DEEPSEEK and kind in ("bf16", "f16"):
+        model = dict(DEEPSEEK, E=64)
+    most = {7168: 8, 4096: 16}.get(model["H"], 32)
+    return dict(model, op=op, kind=kind, M=_between(rng, 1, most), router=rng.random() < 0.5)
+
+
+# ---------------------------------------------------------------------------
+# inputs
+# ---------------------------------------------------------------------------
+def _dtype(name):
+    return {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}[name]
+
+
+def _block(fmt):
+    return 16 if fmt == "nvfp4" else 32
+
+
+def _pack(fmt, w):
+    """[..., K] -> two codes a byte (the first in the low bits) and the scales as they are stored."""
+    v = w.float().unflatten(-1, (-1, _block(fmt)))
+    amax = v.abs().amax(-1)
+    if fmt == "nvfp4":
+        scale = (amax / 6.0).clamp(max=448.0).to(FP8)
+        y = v / scale.float().clamp_min(2.0 ** -9)[..., None]
+    else:
+        part, exponent = torch.frexp(amax)
+        exponent = exponent - torch.where(part <= 0.75, 3, 2)
+        scale = (exponent + 127).clamp(0, 254).to(torch.uint8)
+        y = torch.ldexp(v, -exponent[..., None])
+    a, code = y.abs(), torch.zeros(v.shape, dtype=torch.uint8, device=w.device)
+    for border, even in ((0.25, 0), (0.75, 1), (1.25, 0), (1.75, 1), (2.5, 0), (3.5, 1), (5.0, 0)):
+        code += (a >= border) if even else (a > border)
+    code = (code + (y < 0).to(torch.uint8) * 8).flatten(-2)
+    return code[..., 0::2] + code[..., 1::2] * 16, scale
+
+
+def _store(kind, part):
+    """Weights as `kind` stores them: (codes, scale, one scale for the whole matrix), or fewer."""
+    if kind == "fp8_block":
+        v = part.unflatten(-1, (-1, 128)).unflatten(-3, (-1, 128))
+        s = v.abs().amax((-1, -3)).float().clamp_min(1e-10) / 448.0
+        return (v.float() / s[..., :, None, :, None]).to(FP8).view(part.shape), s, None
+    if kind == "int8_channel":
+        s = part.abs().amax(-1).float().clamp_min(1e-10) / 127.0
+        return (part.float() / s[..., None]).round_().clamp_(-127, 127).to(torch.int8), s, None
+    if kind == "nvfp4":
+        g = part.abs().amax((-1, -2)).float() / (448.0 * 6.0)
+        return *_pack(kind, part.float() / g[..., None, None]), g
+    if kind == "mxfp4":
+        return *_pack(kind, part), None
+    return part, None, None
+
+
+def _weights(kind, experts, n, k, gen):
+    """Expert weights ~N(0, 0.02^2) in the storage of `kind`."""
+    dtype = torch.float16 if kind == "f16" else torch.bfloat16
+    step = max(1, min(experts, (1 << 27) // (n * k)))
+    out = None
+    for e in range(0, experts, step):
+        c = min(step, experts - e)
+        got = _store(kind, torch.randn(c, n, k, generator=gen, device="cuda", dtype=dtype).mul_(0.02))
+        if out is None:
+            out = [None if t is None else torch.empty(experts, *t.shape[1:], dtype=t.dtype, device="cuda")
+                   for t in got]
+        for to, t in zip(out, got):
+            if to is not None:
+                to[e:e + c] = t
+    return out
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    op, m, h = case["op"], case["M"], case["H"]
+    kind = case.get("kind", case.get("fmt"))
+    dtype = _dtype(case["dtype"]) if "dtype" in case else torch.float16 if kind == "f16" else torch.bfloat16
+    x = torch.randn(m, h, generator=gen, device="cuda", dtype=dtype)
+    state = dict(case=case, x=x)
+    # scales of whole tensors, as a calibration leaves them: the largest value seen maps to the
+    # largest that a code and its block's scale can stand for
+    largest = lambda v: torch.full((1,), v / (448.0 * 6.0), device="cuda")  # noqa: E731
+    if op == "fp4":
+        return dict(state, g=largest(5.5) if case["scaled"] else None)
+    if op == "linear":
+        w, ws, g = _weights(kind, 1, case["N"], h, gen)
+        xg = largest(5.5) if kind == "nvfp4" else None
+        return dict(state, w=w[0], ws=ws[0], xg=xg, alpha=xg * g if kind == "nvfp4" else None)
+    experts, inter = case["E"], case["I"]
+    for name, n, k in (("1", 2 * inter, h), ("2", h, inter)):
+        state["w" + name], state["s" + name], state["g" + name] = _weights(kind, experts, n, k, gen)
+    state["a1"] = largest(5.5) if kind == "nvfp4" else None
+    state["a2"] = largest(12.0 * (0.02 ** 2 * h) ** 0.5 * 2) if kind == "nvfp4" else None
+    logits = torch.randn(m, experts, generator=gen, device="cuda")
+    if case.get("router"):
+        return dict(state, logits=logits)
+    weights, ids = torch.softmax(logits, -1).topk(case["K"], -1)
+    return dict(state, ids=ids.to(torch.int32), weights=weights / weights.sum(-1, keepdim=True))
+
+
+# ---------------------------------------------------------------------------
+# one pass: the framework's calls, and the plain form in 32 bits
+# ---------------------------------------------------------------------------
+def run(state):
+    return _own(state) if own else _plain(state)
+
+
+def _own(state):
+    from boltops_b200.fp4 import fp4_dequant, fp4_quant
+    from boltops_b200.fused_moe import fused_experts_decode, fused_experts_fp4, fused_moe_decode
+    from boltops_b200.gemm import gemm_a4w4
+    case, x = state["case"], state["x"]
+    if case["op"] == "fp4":
+        codes, scales = fp4_quant(x, case["fmt"], state["g"])
+        return fp4_dequant(codes, scales, state["g"], dtype=x.dtype)
+    if case["op"] == "linear":
+        codes, scales = fp4_quant(x, case["fmt"], state["xg"])
+        return gemm_a4w4(codes, state["w"], scales, state["ws"], alpha=state["alpha"], dtype=x.dtype)
+    fp4 = dict(w1_scale=state["s1"], w2_scale=state["s2"], w1_global_scale=state["g1"],
+               w2_global_scale=state["g2"], a1_global_scale=state["a1"], a2_global_scale=state["a2"])
+    if case["op"] == "experts":
+        return fused_experts_fp4(x, state["w1"], state["w2"], state["weights"], state["ids"], **fp4)
+    kw = {"fp8_block": dict(use_fp8_w8a8=True, block_shape=[128, 128]),
+          "int8_channel": dict(use_int8_w8a8=True, per_channel_quant=True),
+          "nvfp4": dict(use_fp4_w4a4=True), "mxfp4": dict(use_fp4_w4a4=True)}.get(case["kind"], {})
+    if kw:
+        kw.update(fp4 if "use_fp4_w4a4" in kw else dict(w1_scale=state["s1"], w2_scale=state["s2"]))
+    if case["router"]:
+        return fused_moe_decode(x, state["logits"], state["w1"], state["w2"], case["K"], True, **kw)
+    return fused_experts_decode(x, state["w1"], state["w2"], state["weights"], state["ids"], **kw)
+
+
+def _fp4_values(fmt, x, g):
+    """The values that the 4-bit codes of x stand for (a code is rounded to the nearest, ties to even)."""
+    v = x.float()
+    if g is not None:
+        v = v * (1.0 / g)
+    v = v.unflatten(-1, (-1, _block(fmt)))
+    amax = v.abs().amax(-1, keepdim=True)
+    if fmt == "nvfp4":
+        scale = (amax / 6.0).clamp(max=448.0).to(FP8).float()
+    else:
+        part, exponent = torch.frexp(amax)
+        scale = torch.ldexp(torch.ones_like(amax), exponent - torch.where(part <= 0.75, 3, 2))
+    y = torch.where(scale > 0, v / scale, 0.0)
+    a = y.abs()
+    a = torch.where(a < 2, (2 * a).round() / 2, torch.where(a < 4, a.round(), 2 * (a / 2).round()))
+    v = (torch.copysign(a.clamp(max=6.0), y) * scale).flatten(-2)
+    return v if g is None else v * g
+
+
+def _fp4_read(fmt, codes, scales, g):
+    """Packed codes and stored scales as values."""
+    table = torch.tensor((0, .5, 1, 1.5, 2, 3, 4, 6, -0., -.5, -1, -1.5, -2, -3, -4, -6), device=codes.device)
+    v = table[torch.stack((codes & 15, codes >> 4), -1).flatten(-2).int()]
+    s = scales.float() if fmt == "nvfp4" else torch.exp2(scales.float() - 127.0)
+    if g is not None:
+        s = s * g.view(-1, *[1] * (s.dim() - 1))
+    return (v.unflatten(-1, (-1, _block(fmt))) * s[..., None]).flatten(-2)
+
+
+def _weight_values(kind, w, s, g):
+    if kind in ("nvfp4", "mxfp4"):
+        return _fp4_read(kind, w, s, g)
+    if kind == "fp8_block":
+        v = w.float().unflatten(-1, (-1, 128)).unflatten(-3, (-1, 128))
+        return (v * s[..., :, None, :, None]).view(w.shape)
+    return w.float() if s is None else w.float() * s[..., None]
+
+
+def _row_values(kind, x, g):
+    """Activations after the quantiser of the recipe, which is part of what a layer computes."""
+    if kind in ("nvfp4", "mxfp4"):
+        return _fp4_values(kind, x, g)
+    if kind in ("bf16", "f16"):
+        return x.float()
+    v = x.float().unflatten(-1, (-1, 128 if kind == "fp8_block" else x.shape[-1]))
+    amax = v.abs().amax(-1, keepdim=True).clamp_min(1e-10)
+    if kind == "fp8_block":
+        s = amax / 448.0
+        return ((v * (1.0 / s)).clamp(-448.0, 448.0).to(FP8).float() * s).flatten(-2)
+    s = amax / 127.0
+    return ((v * (1.0 / s)).round().clamp(-128, 127) * s).flatten(-2)
+
+
+def _plain(state):
+    case, x = state["case"], state["x"]
+    if case["op"] == "fp4":
+        return _fp4_values(case["fmt"], x, state["g"]).to(x.dtype)
+    if case["op"] == "linear":
+        fmt, g = case["fmt"], state["xg"]
+        w = _fp4_read(fmt, state["w"], state["ws"], None)
+        y = _fp4_values(fmt, x, g) @ w.t()
+        return (y if g is None else y * (state["alpha"] / g)).to(x.dtype)
+    kind = case.get("kind", case.get("fmt"))
+    if case.get("router"):
+        weights, ids = torch.softmax(state["logits"], -1).topk(case["K"], -1)
+        weights = weights / weights.sum(-1, keepdim=True)
+    else:
+        weights, ids = state["weights"], state["ids"].long()
+    m, k = ids.shape
+    rows = _row_values(kind, x, state["a1"])
+    w1, w2, s1, s2, g1, g2 = (state[n] for n in ("w1", "w2", "s1", "s2", "g1", "g2"))
+    if m * k <= case["E"]:      # the routes' experts, one row each; else every row through every expert
+        pick = lambda t: None if t is None else t[ids.flatten()]  # noqa: E731
+        w1, w2, s1, s2, g1, g2 = (pick(t) for t in (w1, w2, s1, s2, g1, g2))
+        rows = rows.repeat_interleave(k, 0)[:, None]
+    else:
+        rows = rows.expand(case["E"], -1, -1)
+    gate, up = torch.bmm(rows, _weight_values(kind, w1, s1, g1).transpose(1, 2)).chunk(2, -1)
+    act = _row_values(kind, gate * torch.sigmoid(gate) * up, state["a2"])
+    del gate, up
+    y = torch.bmm(act, _weight_values(kind, w2, s2, g2).transpose(1, 2))
+    if m * k <= case["E"]:
+        out = (y.view(m, k, -1) * weights[..., None]).sum(1)
+    else:
+        share = torch.zeros(m, case["E"], device=x.device).scatter_add_(1, ids, weights)
+        out = torch.einsum("emh,me->mh", y, share)
+    return out.to(x.dtype)
+
+
+# ---------------------------------------------------------------------------
+# what a pass cannot do without
+# ---------------------------------------------------------------------------
+def work(case):
+    m, h = case["M"], case["H"]
+    kind = case.get("kind", case.get("fmt"))
+    fp4 = 0.5 + 1.0 / _block(kind)
+    if case["op"] == "fp4":     # values in, codes and scales out, these in again, values out
+        size = _dtype(case["dtype"]).itemsize
+        return dict(bytes=m * h * (2.0 * size + 2 * fp4), flops=2.0 * m * h)
+    if case["op"] == "linear":  # rows in, weights in, result out
+        n = case["N"]
+        return dict(bytes=2.0 * m * h + n * h * fp4 + 2.0 * m * n, flops=2.0 * m * n * h)
+    experts, k, inter = case["E"], case["K"], case["I"]
+    touched = experts * (1 - (1 - k / experts) ** m)     # expected number of experts
+    per_weight = {"fp8_block": 1 + 4 / 16384, "int8_channel": 1.0, "nvfp4": fp4, "mxfp4": fp4}.get(kind, 2.0)
+    routing = m * (4.0 * experts if case.get("router") else 8.0 * k)
+    return dict(bytes=touched * 3 * inter * h * per_weight + 4.0 * m * h + routing,
+                flops=6.0 * m * k * inter * h)
+
+
+# ---------------------------------------------------------------------------
+# the same answers in 64 bits
+# ---------------------------------------------------------------------------
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def _exact_fp4(fmt, x, g):
+    """Rows as their 4-bit codes say them: of the eight magnitudes the nearest, of two as near the even."""
+    y = x.double() / (1.0 if g is None else g.double())
+    y = y.reshape(y.shape[0], -1, _block(fmt))
+    top = y.abs().max(-1, keepdim=True).values
+    if fmt == "nvfp4":
+        s = (top / 6).clamp(max=448).to(torch.float32).to(FP8).double()
+    else:
+        s = torch.exp2(torch.ceil(torch.log2((top / 6).clamp_min(2.0 ** -127))))
+        s = torch.where(top <= 3 * s, s / 2, s)     # (a logarithm rounded up past a power of two)
+    t = y.abs() / s.clamp_min(2.0 ** -140)
+    code = torch.zeros_like(t)
+    for i in range(7):
+        middle = (_E2M1[i] + _E2M1[i + 1]) / 2
+        code += (t >= middle) if i % 2 else (t > middle)
+    v = torch.tensor(_E2M1, dtype=torch.float64, device=x.device)[code.long()]
+    v = torch.where(y < 0, -v, v) * s * (1.0 if g is None else g.double())
+    return v.reshape(x.shape)
+
+
+def _exact_weight(kind, w, s, g):
+    """One matrix [N, K] as the values its codes and scales stand for."""
+    if kind in ("nvfp4", "mxfp4"):
+        low, high = w % 16, w // 16
+        code = torch.stack((low, high), -1).reshape(w.shape[0], -1).long()
+        v = torch.tensor(_E2M1, dtype=torch.float64, device=w.device)[code % 8]
+        v = torch.where(code >= 8, -v, v)
+        s = s.double() if kind == "nvfp4" else 2.0 ** (s.double() - 127)
+        return v * s.repeat_interleave(_block(kind), 1) * (1.0 if g is None else g.double())
+    if kind == "fp8_block":
+        return w.double() * s.double().repeat_interleave(128, 0).repeat_interleave(128, 1)
+    return w.double() if s is None else w.double() * s.double()[:, None]
+
+
+def _exact_rows(kind, v, g):
+    if kind in ("nvfp4", "mxfp4"):
+        return _exact_fp4(kind, v, g)
+    if kind in ("bf16", "f16"):
+        return v.double()
+    # the 8-bit recipe scales in 32 bits, by the reciprocal of the scale: with 16-bit rows many a
+    # value lies on the border of two codes, and these roundings, which decide it, belong to the recipe
+    largest = 448 if kind == "fp8_block" else 127
+    y = v.float().reshape(v.shape[0], -1, 128 if kind == "fp8_block" else v.shape[1])
+    s = y.abs().max(-1, keepdim=True).values.clamp_min(1e-10) / largest
+    q = y * s.reciprocal()
+    q = q.clamp(-448, 448).to(FP8).double() if kind == "fp8_block" else q.round().double()
+    return (q * s.double()).reshape(v.shape)
+
+
+def exact(case, seed):
+    state = prepare(case, seed)
+    x = state["x"]
+    if case["op"] == "fp4":
+        return _exact_fp4(case["fmt"], x, state["g"])
+    if case["op"] == "linear":
+        kind, g = case["fmt"], state["xg"]
+        scale = 1.0 if g is None else state["alpha"].double() / g.double()
+        return _exact_fp4(kind, x, g) @ _exact_weight(kind, state["w"], state["ws"], None).t() * scale
+    kind = case.get("kind", case.get("fmt"))
+    if case.get("router"):
+        weights, ids = torch.softmax(state["logits"].double(), -1).topk(case["K"], -1)
+        weights = weights / weights.sum(-1, keepdim=True)
+    else:
+        weights, ids = state["weights"].double(), state["ids"].long()
+    rows = _exact_rows(kind, x, state["a1"])
+    out = torch.zeros(rows.shape, dtype=torch.float64, device=x.device)
+    one = lambda n, e: None if state[n] is None else state[n][e]  # noqa: E731
+    for e in ids.unique().tolist():
+        token, slot = (ids == e).nonzero(as_tuple=True)
+        both = rows[token] @ _exact_weight(kind, state["w1"][e], one("s1", e), one("g1", e)).t()
+        gate, up = both.chunk(2, -1)
+        act = _exact_rows(kind, gate / (1 + torch.exp(-gate)) * up, state["a2"])
+        y = act @ _exact_weight(kind, state["w2"][e], one("s2", e), one("g2", e)).t()
+        out.index_add_(0, token, y * weights[token, slot][:, None])
+    return out
