@@ -178,28 +178,26 @@ def run(state):
 
 
 def _own(state):
-    from boltops_b200.fp4 import fp4_dequant, fp4_quant
-    from boltops_b200.fused_moe import fused_experts_decode, fused_experts_fp4, fused_moe_decode
-    from boltops_b200.gemm import gemm_a4w4
+    from boltops_b200 import fp4, fused_moe, gemm
     case, x = state["case"], state["x"]
     if case["op"] == "fp4":
-        codes, scales = fp4_quant(x, case["fmt"], state["g"])
-        return fp4_dequant(codes, scales, state["g"], dtype=x.dtype)
+        codes, scales = fp4.fp4_quant(x, case["fmt"], state["g"])
+        return fp4.fp4_dequant(codes, scales, state["g"], dtype=x.dtype)
     if case["op"] == "linear":
-        codes, scales = fp4_quant(x, case["fmt"], state["xg"])
-        return gemm_a4w4(codes, state["w"], scales, state["ws"], alpha=state["alpha"], dtype=x.dtype)
-    fp4 = dict(w1_scale=state["s1"], w2_scale=state["s2"], w1_global_scale=state["g1"],
-               w2_global_scale=state["g2"], a1_global_scale=state["a1"], a2_global_scale=state["a2"])
+        codes, scales = fp4.fp4_quant(x, case["fmt"], state["xg"])
+        return gemm.gemm_a4w4(codes, state["w"], scales, state["ws"], alpha=state["alpha"], dtype=x.dtype)
+    w4a4 = dict(w1_scale=state["s1"], w2_scale=state["s2"], w1_global_scale=state["g1"],
+                w2_global_scale=state["g2"], a1_global_scale=state["a1"], a2_global_scale=state["a2"])
     if case["op"] == "experts":
-        return fused_experts_fp4(x, state["w1"], state["w2"], state["weights"], state["ids"], **fp4)
+        return fused_moe.fused_experts_fp4(x, state["w1"], state["w2"], state["weights"], state["ids"], **w4a4)
     kw = {"fp8_block": dict(use_fp8_w8a8=True, block_shape=[128, 128]),
           "int8_channel": dict(use_int8_w8a8=True, per_channel_quant=True),
           "nvfp4": dict(use_fp4_w4a4=True), "mxfp4": dict(use_fp4_w4a4=True)}.get(case["kind"], {})
     if kw:
-        kw.update(fp4 if "use_fp4_w4a4" in kw else dict(w1_scale=state["s1"], w2_scale=state["s2"]))
+        kw.update(w4a4 if "use_fp4_w4a4" in kw else dict(w1_scale=state["s1"], w2_scale=state["s2"]))
     if case["router"]:
-        return fused_moe_decode(x, state["logits"], state["w1"], state["w2"], case["K"], True, **kw)
-    return fused_experts_decode(x, state["w1"], state["w2"], state["weights"], state["ids"], **kw)
+        return fused_moe.fused_moe_decode(x, state["logits"], state["w1"], state["w2"], case["K"], True, **kw)
+    return fused_moe.fused_experts_decode(x, state["w1"], state["w2"], state["weights"], state["ids"], **kw)
 
 
 def _fp4_values(fmt, x, g):
