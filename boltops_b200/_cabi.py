@@ -25,6 +25,11 @@ GEMM_BF16, GEMM_F16, GEMM_FP8_BLOCK, GEMM_INT8_CHANNEL, GEMM_FP8_CHANNEL, GEMM_I
     GEMM_MXFP8, GEMM_MXFP4 = range(8)
 # enum bolt_gemm_epilogue
 EPI_STORE, EPI_SILU_MUL, EPI_SILU_MUL_QUANT = range(3)
+# enum bolt_decode_kind
+DECODE_BF16, DECODE_F16, DECODE_FP8_BLOCK, DECODE_INT8_CHANNEL, DECODE_FP8_CHANNEL, \
+    DECODE_INT8_BLOCK, DECODE_NVFP4, DECODE_MXFP4 = range(8)
+# enum bolt_fp4_format
+FP4_NV, FP4_MX = range(2)
 # BOLT_ABI_VERSION of the header these structures were written against
 ABI_VERSION = 4
 # enum bolt_gemm_schedule, BOLT_PAIR_SEGMENT_ROWS
@@ -82,6 +87,27 @@ class LayerArgs(C.Structure):
         ("routed_scaling_factor", C.c_float),
         ("out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
         ("status", C.c_void_p), ("schedule", C.c_int),
+    ]
+
+
+class DecodeArgs(C.Structure):
+    """struct bolt_decode_args"""
+    _fields_ = [
+        ("kind", C.c_int), ("x_dtype", C.c_int), ("out_dtype", C.c_int),
+        ("num_tokens", C.c_int), ("topk", C.c_int),
+        ("hidden", C.c_int), ("inter", C.c_int), ("model_dim", C.c_int),
+        ("num_experts", C.c_int), ("global_num_experts", C.c_int),
+        ("hidden_states", C.c_void_p), ("w1", C.c_void_p), ("w2", C.c_void_p),
+        ("w1_scale", C.c_void_p), ("w2_scale", C.c_void_p),
+        ("w1_global_scale", C.c_void_p), ("w2_global_scale", C.c_void_p),
+        ("a1_global_scale", C.c_void_p), ("a2_global_scale", C.c_void_p),
+        ("topk_weights", C.c_void_p), ("topk_ids", C.c_void_p),
+        ("gating", C.c_void_p), ("gating_dtype", C.c_int), ("renormalize", C.c_int),
+        ("is_softmax", C.c_int), ("expert_map", C.c_void_p),
+        ("activation", C.c_int), ("act_alpha", C.c_float), ("act_limit", C.c_float),
+        ("routed_scaling_factor", C.c_float),
+        ("out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("status", C.c_void_p), ("sm_count", C.c_int),
     ]
 
 
@@ -167,6 +193,12 @@ _SIGNATURES = {
     "bolt_moe_layer_workspace_bytes": (C.c_size_t, [C.POINTER(LayerArgs)]),
     "bolt_moe_layer_kernel_count": (C.c_int, [C.POINTER(LayerArgs)]),
     "bolt_moe_layer": (C.c_int, [C.POINTER(LayerArgs), C.c_void_p]),
+    "bolt_fp4_quant": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int, C.c_void_p,
+                                 C.c_void_p, C.c_void_p, C.c_void_p]),
+    "bolt_fp4_dequant": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_void_p,
+                                   C.c_void_p, C.c_int, C.c_void_p]),
+    "bolt_moe_decode_workspace_bytes": (C.c_size_t, [C.POINTER(DecodeArgs)]),
+    "bolt_moe_decode": (C.c_int, [C.POINTER(DecodeArgs), C.c_void_p]),
 }
 
 EXPORTS = tuple(_SIGNATURES)

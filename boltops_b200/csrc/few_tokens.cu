@@ -1,0 +1,1005 @@
+// A whole mixture-of-experts layer for 1 to 32 tokens in two kernels.
+//
+//   out[m] = s * sum_k w[m, k] * W2[e] . Q2(act(W1[e] . Q1(x[m]))),  e = ids[m, k]
+//
+// k_few_up: routing (and, from logits, the router's top-k), Q1, the gate and up projections and the
+// activation; k_few_down: routing again, Q2, the down projection and the weighted sum over a token's
+// experts.  Nothing is sorted or copied: with so few tokens the routing is a bit mask of tokens per
+// expert, which every block builds for itself in shared memory in about a microsecond.
+//
+// What bounds it: the weights of the touched experts, read once each from HBM.  Split: k_few_up's unit
+// is 16 (MX: 32) intermediate columns of one expert, gate and up rows together over the whole hidden
+// size, so that activation and (4-bit experts) the block quantiser run on finished sums; k_few_down's
+// unit is 16 output columns over ALL touched experts, so that the sum over a token's experts stays in
+// registers.  Units go to the blocks in contiguous runs, the 128-byte boxes of a unit to the warps
+// (token_mma.cuh).  The second kernel is launched with programmatic serialisation: its blocks start
+// as soon as there is room, build the routing and fill their rings with weights while the first
+// kernel finishes, and wait for it before they read its activations.  No block waits for another,
+// nothing is counted in memory, and results do not depend on timing.
+//
+// Rounding: 16-bit experts round the activation to the weights' type (the tensor cores' operand);
+// quantised experts keep fp32 up to their quantiser.  All sums are fp32, rounded once at the end.
+#include <cuda.h>
+
+#include <atomic>
+
+#include "act_pair.cuh"
+#include "routing_row.cuh"
+#include "token_mma.cuh"
+
+namespace bolt {
+namespace few {
+namespace {
+
+struct Params {
+  const void* x;            // [tokens, hidden], 16-bit
+  int x_dtype, out_dtype;
+  int tokens, topk, hidden, inter, model_dim, experts, global_experts;
+  const void* s1;           // 8-bit: fp32; 4-bit: scale bytes [experts, 2 inter, hidden / block]
+  const void* s2;
+  const float *g1, *g2, *a1, *a2;   // scales of whole tensors (4-bit), null: 1
+  const float* wts;         // [tokens, topk]
+  const int32_t* ids;
+  const void* gating;       // router logits [tokens, global_experts]: ids and wts are made here
+  int gating_dtype, renormalize, softmax;
+  const int32_t* emap;
+  ActParams act;
+  float out_scale;
+  void* out;
+  // workspace: activations of every (expert, token) slot
+  uint8_t* act_rows;        // 16-bit values, fp32 values (8-bit kinds) or codes (4-bit kinds)
+  uint8_t* act_sf;          // scale bytes (4-bit kinds)
+  float* act_amax;          // [slots][units of an expert] (per-channel kinds)
+  int32_t* status;
+  int slots_per_warp;
+};
+
+// ---------------------------------------------------------------------------
+// routing
+// ---------------------------------------------------------------------------
+struct Routes {
+  uint32_t* mask;   // [experts] tokens of an expert
+  int* off;         // [experts] slot of its first token: slots go by (expert, token)
+  int* list;        // touched experts, ascending
+  float* coef;      // [slots] router weight (of all routes of a token to the expert)
+  int* token;       // [slots]
+  int* ids;         // [routes] local expert or -1
+  float* wts;       // [routes]
+  int touched;
+};
+__host__ __device__ inline int route_bytes(int experts, int routes) {
+  return 4 * (3 * experts + 4 * routes) + 128;
+}
+
+template <int NPL>
+__device__ __noinline__ void route_token(const void* row, int dt, int experts, int topk, int renormalize,
+                                         int softmax, int lane, float& w, int& id) {
+  float v[NPL];
+#pragma unroll
+  for (int j = 0; j < NPL; ++j) {
+    const int e = lane + 32 * j;
+    v[j] = 0.f;
+    if (e < experts)
+      v[j] = dt == BOLT_F32    ? static_cast<const float*>(row)[e]
+             : dt == BOLT_BF16 ? to_f32(static_cast<const __nv_bfloat16*>(row)[e])
+                               : to_f32(static_cast<const __half*>(row)[e]);
+  }
+  topk_of_row<NPL>(v, experts, topk, renormalize, softmax, lane, w, id);
+}
+
+__device__ __forceinline__ int local_expert(const Params& p, int id) {
+  if (id < 0 || id >= p.global_experts) return -1;
+  const int e = p.emap != nullptr ? p.emap[id] : id;
+  return e >= 0 && e < p.experts ? e : -1;
+}
+
+__device__ void build_routes(const Params& p, Routes& r, uint8_t* mem) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int routes = p.tokens * p.topk, experts = p.experts;
+  r.mask = reinterpret_cast<uint32_t*>(mem);
+  r.off = reinterpret_cast<int*>(r.mask + experts);
+  r.list = r.off + experts;
+  r.coef = reinterpret_cast<float*>(r.list + experts);
+  r.token = reinterpret_cast<int*>(r.coef + routes);
+  r.ids = r.token + routes;
+  r.wts = reinterpret_cast<float*>(r.ids + routes);
+  int* totals = reinterpret_cast<int*>(r.wts + routes);   // [8] per warp
+  for (int e = tid; e < experts; e += kThreads) r.mask[e] = 0;
+  if (p.gating != nullptr) {
+    const int size = p.gating_dtype == BOLT_F32 ? 4 : 2;
+    const int npl = (p.global_experts + 31) / 32;
+    for (int m = warp; m < p.tokens; m += kWarps) {
+      const void* row = static_cast<const uint8_t*>(p.gating) + (int64_t)m * p.global_experts * size;
+      float w;
+      int id;
+      if (npl <= 1) route_token<1>(row, p.gating_dtype, p.global_experts, p.topk, p.renormalize, p.softmax, lane, w, id);
+      else if (npl <= 4) route_token<4>(row, p.gating_dtype, p.global_experts, p.topk, p.renormalize, p.softmax, lane, w, id);
+      else if (npl <= 8) route_token<8>(row, p.gating_dtype, p.global_experts, p.topk, p.renormalize, p.softmax, lane, w, id);
+      else route_token<32>(row, p.gating_dtype, p.global_experts, p.topk, p.renormalize, p.softmax, lane, w, id);
+      if (lane < p.topk) {
+        r.ids[m * p.topk + lane] = local_expert(p, id);
+        r.wts[m * p.topk + lane] = w;
+      }
+    }
+  } else {
+    for (int i = tid; i < routes; i += kThreads) {
+      r.ids[i] = local_expert(p, p.ids[i]);
+      r.wts[i] = p.wts[i];
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < routes; i += kThreads)
+    if (r.ids[i] >= 0) atomicOr(&r.mask[r.ids[i]], 1u << (i / p.topk));
+  __syncthreads();
+  // exclusive sums over the experts: tokens (low half), touched experts (high half)
+  int base = 0;
+  for (int e0 = 0; e0 < experts; e0 += kThreads) {
+    const int e = e0 + tid;
+    const int c = e < experts ? __popc(r.mask[e]) : 0;
+    const int mine = c | (c > 0 ? 0x10000 : 0);
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    if (lane == 31) totals[warp] = sum;
+    __syncthreads();
+    int before = base, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += totals[w];
+      all += totals[w];
+    }
+    before += sum - mine;
+    if (e < experts) {
+      r.off[e] = before & 0xFFFF;
+      if (c > 0) r.list[before >> 16] = e;
+    }
+    base += all;
+    __syncthreads();
+  }
+  r.touched = base >> 16;
+  for (int i = tid; i < routes; i += kThreads) {
+    const int e = r.ids[i];
+    if (e < 0) continue;
+    const int m = i / p.topk, first = m * p.topk, last = first + p.topk;
+    bool again = false;
+    for (int j = first; j < i; ++j) again |= r.ids[j] == e;
+    if (again) continue;       // the same expert twice for a token: one slot, the weights' sum
+    float w = 0.f;
+    for (int j = i; j < last; ++j)
+      if (r.ids[j] == e) w += r.wts[j];
+    const int slot = r.off[e] + __popc(r.mask[e] & ((1u << m) - 1u));
+    r.coef[slot] = w;
+    r.token[slot] = m;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ int slot_of(uint32_t mask, int off, int token) {
+  return (mask >> token) & 1u ? off + __popc(mask & ((1u << token) - 1u)) : -1;
+}
+
+// ---------------------------------------------------------------------------
+// a warp's ring of weight boxes
+// ---------------------------------------------------------------------------
+struct Ring {
+  uint32_t base, bars;
+  int slots, bytes;
+  int s_in = 0, s_out = 0;
+  uint32_t ph = 0;
+  __device__ void init(uint32_t smem, uint32_t bar, int n, int box_bytes) {
+    base = smem;
+    bars = bar;
+    slots = n;
+    bytes = box_bytes;
+  }
+  // lane 0 only: the barrier and the address of the next box to bring
+  __device__ __forceinline__ uint32_t next_in(uint32_t& dst) {
+    const uint32_t bar = bars + 8 * s_in;
+    dst = base + s_in * bytes;
+    mbar_expect_tx(bar, bytes);
+    if (++s_in == slots) s_in = 0;
+    return bar;
+  }
+  __device__ __forceinline__ uint32_t wait(volatile int* abort_flag, int32_t* status) {
+    mbar_wait(bars + 8 * s_out, ph, abort_flag, status, 30);
+    return base + s_out * bytes;
+  }
+  __device__ __forceinline__ void release() {
+    __syncwarp();
+    if (++s_out == slots) {
+      s_out = 0;
+      ph ^= 1;
+    }
+  }
+};
+
+constexpr int kCtrlBytes = 1024;   // barriers and the abort flag
+constexpr int kMaxSlots = 14;      // 8 warps x 14 barriers x 8 bytes < 1024
+
+__device__ __forceinline__ uint8_t* carve(uint8_t* raw) {
+  return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+}
+
+// What both kernels begin with: barriers, the ring.
+__device__ __forceinline__ volatile int* start(Ring& ring, uint8_t* smem, int slots, int box_bytes) {
+  const int warp = threadIdx.x >> 5;
+  uint8_t* ctrl = smem + kWarps * slots * box_bytes;
+  const uint32_t bars = smem_u32(ctrl);
+  if (threadIdx.x < kWarps * slots) mbar_init(bars + 8 * threadIdx.x, 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + kCtrlBytes - 8);
+  if (threadIdx.x == 0) *abort_flag = 0;
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __syncthreads();
+  ring.init(smem_u32(smem) + warp * slots * box_bytes, bars + 8 * warp * slots, slots, box_bytes);
+  return abort_flag;
+}
+// A wait that ran out leaves copies in flight: give them time to land before the block's memory
+// goes to another.
+__device__ __forceinline__ void finish(volatile int* abort_flag) {
+  __syncthreads();
+  if (*abort_flag)
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+}
+
+template <int MT, int NT>
+__device__ __forceinline__ void put_sums(float* red, const float (&acc)[MT][NT][4], int warp, int lane,
+                                         unsigned live) {
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if (!((live >> nt) & 1u)) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) red[(((warp * MT + mt) * NT + nt) * 4 + i) * 32 + lane] = acc[mt][nt][i];
+    }
+}
+// Sum over the warps of element (row half r, row g of tile mt, token n).
+template <int MT, int NT>
+__device__ __forceinline__ float get_sum(const float* red, int mt, int r, int g, int n) {
+  const int at = ((mt * NT + (n >> 3)) * 4 + 2 * r + (n & 1)) * 32 + 4 * g + ((n & 7) >> 1);
+  float v = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) v += red[w * MT * NT * 128 + at];
+  return v;
+}
+
+constexpr int unit_cols(int k) { return k == K_MX4 ? 32 : 16; }
+constexpr int up_box_bytes(int k) { return 2 * unit_cols(k) * 128; }
+constexpr int kDownRows = 16;
+constexpr int kDownBoxBytes = kDownRows * 128;
+// (above: registers would be spilled)
+constexpr int blocks_per_sm(int k, int nt) { return nt == 1 || (nt == 2 && k != K_MX4) ? 2 : 1; }
+constexpr int red_bytes(int mt, int nt) { return kWarps * mt * nt * 128 * 4; }
+
+// ---------------------------------------------------------------------------
+// gate and up projections, activation
+// ---------------------------------------------------------------------------
+template <int K, int NT>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(K, NT))
+k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
+  constexpr int UC = unit_cols(K), MT = UC / 8, kBox = up_box_bytes(K);
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = carve(raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  Ring ring;
+  volatile int* abort_flag = start(ring, smem, p.slots_per_warp, kBox);
+  uint8_t* rest = smem + kWarps * p.slots_per_warp * kBox + kCtrlBytes;
+  float* red = reinterpret_cast<float*>(rest);
+  rest += red_bytes(MT, NT);
+  let_next_start();
+
+  Routes r;
+  build_routes(p, r, rest);
+  rest += (route_bytes(p.experts, p.tokens * p.topk) + 15) & ~15;
+
+  const int per_expert = (p.inter + UC - 1) / UC;
+  const int64_t units = (int64_t)r.touched * per_expert;
+  const int u0 = (int)(units * blockIdx.x / gridDim.x), u1 = (int)(units * (blockIdx.x + 1) / gridDim.x);
+  const int nb = (int)((row_bytes(K, p.hidden) + 127) / 128);
+  const int64_t boxes = (int64_t)(u1 - u0) * nb;
+  const int n_it = boxes > warp ? (int)((boxes - warp + kWarps - 1) / kWarps) : 0;
+
+  // boxes of this block's units in order, every eighth this warp's
+  int in_u = u0, in_kb = warp, in_it = 0;
+  auto bring = [&]() {
+    while (in_kb >= nb) {
+      in_kb -= nb;
+      ++in_u;
+    }
+    if (lane == 0) {
+      uint32_t dst;
+      const uint32_t bar = ring.next_in(dst);
+      tma_load_4d(dst, &map, bar, in_kb * 128, (in_u % per_expert) * UC, 0, r.list[in_u / per_expert]);
+    }
+    in_kb += kWarps;
+    ++in_it;
+  };
+  for (int i = 0; i < p.slots_per_warp && in_it < n_it; ++i) bring();
+
+  // ---- Q1 that needs whole rows, once per block while the first boxes travel ----
+  float* row_scale = reinterpret_cast<float*>(rest);       // [tokens][2]: scale, reciprocal
+  uint8_t* x_codes = rest;                                 // [tokens][hidden / 2], scales behind them
+  uint8_t* x_sf = x_codes + (int64_t)p.tokens * (p.hidden / 2);
+  constexpr int kBlk = K == K_NV4 ? 16 : 32;
+  const int sf_row = p.hidden / kBlk;
+  if constexpr (is_channel(K)) {
+    for (int m = warp; m < p.tokens; m += kWarps) {
+      const uint16_t* row = static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden;
+      float amax = 0.f;
+      for (int c = lane * 8; c < p.hidden; c += 256) {
+        const uint4 u = *reinterpret_cast<const uint4*>(row + c);
+        const uint32_t q[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (p.x_dtype == BOLT_BF16) {
+            amax = fmaxf(amax, fabsf(__uint_as_float(q[j] << 16)));
+            amax = fmaxf(amax, fabsf(__uint_as_float(q[j] & 0xFFFF0000u)));
+          } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q[j]));
+            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+      }
+      for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (lane == 0) scale8<K>(amax, row_scale[2 * m], row_scale[2 * m + 1]);
+    }
+    __syncthreads();
+  } else if constexpr (is4(K)) {
+    const bool nv = K == K_NV4;
+    const float inv_g = p.a1 != nullptr ? __frcp_rn(*p.a1) : 1.f;
+    const int per_row = p.hidden / 32;
+    for (int i = tid; i < p.tokens * per_row; i += kThreads) {
+      const int m = i / per_row, c = (i - m * per_row) * 32;
+      float v[32];
+      load_values32(v, static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden, p.x_dtype, p.hidden, c);
+      if (nv && p.a1 != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] *= inv_g;
+      }
+      uint32_t w[4];
+#pragma unroll
+      for (int b = 0; b < 32 / kBlk; ++b) {
+        float amax = 0.f;
+#pragma unroll
+        for (int j = 0; j < kBlk; ++j) amax = fp4::amax_nan(amax, v[b * kBlk + j]);
+        const uint32_t byte = fp4::scale_byte<K == K_NV4>(amax);
+        const fp4::Scaler sc = fp4::scaler_of<K == K_NV4>(byte);
+#pragma unroll
+        for (int j = 0; j < kBlk / 8; ++j)
+          w[b * (kBlk / 8) + j] = fp4::codes8<K == K_NV4>(v + b * kBlk + 8 * j, sc);
+        x_sf[(int64_t)m * sf_row + c / kBlk + b] = (uint8_t)byte;
+      }
+      *reinterpret_cast<uint4*>(x_codes + (int64_t)m * (p.hidden / 2) + c / 2) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __syncthreads();
+  }
+
+  int it = 0, kb = warp, ku = u0;   // the box this warp computes next
+  while (kb >= nb) {
+    kb -= nb;
+    ++ku;
+  }
+  const int64_t sf1_row = p.hidden / kBlk;
+  auto row_scales = [&](RowScales<K>(&ws)[MT], int u, int box) {
+    if constexpr (is4(K)) {
+      const int64_t e = r.list[u / per_expert];
+      const int c0 = (u % per_expert) * UC;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          load_block_scales<K>(ws[mt].sf[h],
+                               static_cast<const uint8_t*>(p.s1) +
+                                   ((e * 2 + h) * p.inter + c0 + 8 * mt + g) * sf1_row,
+                               (int)sf1_row, box, t);
+    }
+  };
+  RowScales<K> ws[MT], ws_next[MT];
+  if (it < n_it) row_scales(ws_next, ku, kb);
+
+  for (int u = u0; u < u1; ++u) {
+    const int e = r.list[u / per_expert], c0 = (u % per_expert) * UC;
+    const uint32_t mask = r.mask[e];
+    const int off = r.off[e], cnt = __popc(mask);
+    const unsigned live = (1u << ((cnt + 7) / 8)) - 1u;
+    float acc[MT][NT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[mt][nt][i] = 0.f;
+    int tok[NT];     // token of column g of every tile
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) tok[nt] = 8 * nt + g < cnt ? r.token[off + 8 * nt + g] : -1;
+
+    while (it < n_it && ku == u) {
+      // next box's scales travel while this one is computed
+      int nkb = kb + kWarps, nu = ku;
+      while (nkb >= nb) {
+        nkb -= nb;
+        ++nu;
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) ws[mt] = ws_next[mt];
+      if (it + 1 < n_it) row_scales(ws_next, nu, nkb);
+
+      TokenBox<K> x[NT];
+      float xs[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (!((live >> nt) & 1u)) continue;
+        const int m = tok[nt];
+        if constexpr (is16(K)) {
+          load_token<K>(x[nt], m < 0 ? nullptr : static_cast<const uint8_t*>(p.x) + (int64_t)m * p.hidden * 2,
+                        p.hidden * 2, kb, t);
+        } else if constexpr (is8(K)) {
+          float v[32];
+          load_values32(v, m < 0 ? nullptr : static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden,
+                        p.x_dtype, p.hidden, kb * 128 + 32 * t);
+          float inv;
+          if constexpr (is_block(K)) {
+            float amax = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) amax = fmaxf(amax, fabsf(v[j]));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            scale8<K>(amax, xs[nt], inv);
+          } else {
+            inv = m < 0 ? 0.f : row_scale[2 * m + 1];
+          }
+          codes32<K>(v, inv, x[nt].w);
+        } else {
+          load_token<K>(x[nt], m < 0 ? nullptr : x_codes + (int64_t)m * (p.hidden / 2), p.hidden / 2, kb, t);
+          if constexpr (K == K_NV4) {
+            load_block_scales<K>(x[nt].sf, m < 0 ? nullptr : x_sf + (int64_t)m * sf_row, sf_row, kb, t);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int col = 8 * nt + 2 * t + i;
+              load_block_scales<K>(x[nt].sf + 2 * i,
+                                   col < cnt ? x_sf + (int64_t)r.token[off + col] * sf_row : nullptr,
+                                   sf_row, kb, t);
+            }
+          }
+        }
+      }
+      const uint32_t box = ring.wait(abort_flag, p.status);
+      if constexpr (is_block(K)) {
+        const float* s1 = static_cast<const float*>(p.s1);
+        const int blocks_n = 2 * p.inter / 128, blocks_k = p.hidden / 128;
+        const float sg = s1[((int64_t)e * blocks_n + c0 / 128) * blocks_k + kb];
+        const float su = s1[((int64_t)e * blocks_n + (p.inter + c0) / 128) * blocks_k + kb];
+        float part[MT][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[mt][nt][i] = 0.f;
+        box_mma<K, MT, NT, true>(box, lane, x, ws, live, part);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (!((live >> nt) & 1u)) continue;
+          const float x0 = __shfl_sync(0xffffffffu, xs[nt], 8 * t);
+          const float x1 = __shfl_sync(0xffffffffu, xs[nt], 8 * t + 4);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            acc[mt][nt][0] = fmaf(part[mt][nt][0], x0 * sg, acc[mt][nt][0]);
+            acc[mt][nt][1] = fmaf(part[mt][nt][1], x1 * sg, acc[mt][nt][1]);
+            acc[mt][nt][2] = fmaf(part[mt][nt][2], x0 * su, acc[mt][nt][2]);
+            acc[mt][nt][3] = fmaf(part[mt][nt][3], x1 * su, acc[mt][nt][3]);
+          }
+        }
+      } else {
+        box_mma<K, MT, NT, true>(box, lane, x, ws, live, acc);
+      }
+      ring.release();
+      if (in_it < n_it) bring();
+      kb = nkb;
+      ku = nu;
+      ++it;
+    }
+
+    // ---- sums over the warps, activation, Q2 of the 4-bit kinds ----
+    put_sums<MT, NT>(red, acc, warp, lane, live);
+    __syncthreads();
+    const int all = ((cnt * UC + 31) / 32) * 32;      // whole warps take part in the exchanges
+    for (int i = tid; i < all; i += kThreads) {
+      const int n = i / UC, c = i % UC, col = c0 + c;
+      const bool have = n < cnt && col < p.inter;
+      const int slot = off + n;
+      float a = 0.f;
+      if (have) {
+        float gate = get_sum<MT, NT>(red, c >> 3, 0, c & 7, n);
+        float up = get_sum<MT, NT>(red, c >> 3, 1, c & 7, n);
+        if constexpr (is_channel(K)) {
+          const float* s1 = static_cast<const float*>(p.s1) + (int64_t)e * 2 * p.inter;
+          const float xsc = row_scale[2 * r.token[slot]];
+          gate *= xsc * s1[col];
+          up *= xsc * s1[p.inter + col];
+        } else if constexpr (is4(K)) {
+          const float f = (p.g1 != nullptr ? p.g1[e] : 1.f) * (p.a1 != nullptr ? *p.a1 : 1.f);
+          gate *= f;
+          up *= f;
+        }
+        a = act_pair(p.act, gate, up);
+      }
+      if constexpr (is16(K)) {
+        if (have) {
+          const int64_t at = (int64_t)slot * p.inter + col;
+          if (K == K_BF16) reinterpret_cast<__nv_bfloat16*>(p.act_rows)[at] = __float2bfloat16_rn(a);
+          else reinterpret_cast<__half*>(p.act_rows)[at] = __float2half_rn(a);
+        }
+      } else if constexpr (is8(K)) {
+        if (have) reinterpret_cast<float*>(p.act_rows)[(int64_t)slot * p.inter + col] = a;
+        if constexpr (is_channel(K)) {
+          float amax = fabsf(a);
+#pragma unroll
+          for (int o = UC / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+          if (c == 0 && n < cnt) p.act_amax[(int64_t)slot * per_expert + u % per_expert] = amax;
+        }
+      } else {
+        // UC columns of one slot are one block
+        if (K == K_NV4 && p.a2 != nullptr) a *= __frcp_rn(*p.a2);
+        float amax = fabsf(a);
+#pragma unroll
+        for (int o = UC / 2; o > 0; o >>= 1) amax = fp4::amax_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const uint32_t byte = fp4::scale_byte<K == K_NV4>(amax);
+        const fp4::Scaler sc = fp4::scaler_of<K == K_NV4>(byte);
+        const float q = sc.r == 0.f ? 0.f : fp4::quotient<K == K_NV4>(a, sc);
+        const float other = __shfl_down_sync(0xffffffffu, q, 1);
+        if (have && (c & 1) == 0)
+          p.act_rows[(int64_t)slot * (p.inter / 2) + col / 2] = (uint8_t)fp4::pack2(q, other);
+        if (have && c == 0) p.act_sf[(int64_t)slot * (p.inter / kBlk) + col / kBlk] = (uint8_t)byte;
+      }
+    }
+    __syncthreads();
+  }
+  finish(abort_flag);
+}
+
+// ---------------------------------------------------------------------------
+// down projection, sum over a token's experts
+// ---------------------------------------------------------------------------
+template <int K, int NT>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(K, NT))
+k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
+  constexpr int kBox = kDownBoxBytes;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = carve(raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  Ring ring;
+  volatile int* abort_flag = start(ring, smem, p.slots_per_warp, kBox);
+  uint8_t* rest = smem + kWarps * p.slots_per_warp * kBox + kCtrlBytes;
+  float* red = reinterpret_cast<float*>(rest);
+  rest += red_bytes(1, NT);
+
+  Routes r;
+  build_routes(p, r, rest);
+  rest += (route_bytes(p.experts, p.tokens * p.topk) + 15) & ~15;
+
+  const int units = (p.model_dim + kDownRows - 1) / kDownRows;
+  const int u0 = (int)((int64_t)units * blockIdx.x / gridDim.x);
+  const int u1 = (int)((int64_t)units * (blockIdx.x + 1) / gridDim.x);
+  const int nb = (int)((row_bytes(K, p.inter) + 127) / 128);
+  const int64_t boxes = (int64_t)(u1 - u0) * r.touched * nb;
+  const int n_it = boxes > warp ? (int)((boxes - warp + kWarps - 1) / kWarps) : 0;
+
+  // boxes in the order (unit, expert, place in the reduction), every eighth this warp's
+  struct Place {
+    int u, a, kb;
+  };
+  auto settle = [&](Place& q) {
+    while (q.kb >= nb) {
+      q.kb -= nb;
+      if (++q.a == r.touched) {
+        q.a = 0;
+        ++q.u;
+      }
+    }
+  };
+  Place in = {u0, 0, warp};
+  int in_it = 0;
+  auto bring = [&]() {
+    settle(in);
+    if (lane == 0) {
+      uint32_t dst;
+      const uint32_t bar = ring.next_in(dst);
+      tma_load_3d(dst, &map, bar, in.kb * 128, in.u * kDownRows, r.list[in.a]);
+    }
+    in.kb += kWarps;
+    ++in_it;
+  };
+  for (int i = 0; i < p.slots_per_warp && in_it < n_it; ++i) bring();
+
+  constexpr int kBlk = K == K_NV4 ? 16 : 32;
+  const int sf_row = p.inter / kBlk;
+  Place cur = {u0, 0, warp};
+  if (n_it > 0) settle(cur);
+  auto row_scales = [&](RowScales<K>& ws, const Place& q) {
+    if constexpr (is4(K)) {
+      const int64_t e = r.list[q.a];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = q.u * kDownRows + 8 * h + g;
+        load_block_scales<K>(ws.sf[h],
+                             row < p.model_dim
+                                 ? static_cast<const uint8_t*>(p.s2) + (e * p.model_dim + row) * sf_row
+                                 : nullptr,
+                             sf_row, q.kb, t);
+      }
+    }
+  };
+  RowScales<K> ws[1], ws_next;
+  int it = 0;
+  if (n_it > 0) row_scales(ws_next, cur);
+
+  wait_for_previous();     // the activations
+  float* row_scale = reinterpret_cast<float*>(rest);       // [slots][2]
+  if constexpr (is_channel(K)) {
+    const int per_expert = (p.inter + unit_cols(K) - 1) / unit_cols(K);
+    int slots = 0;
+    if (r.touched > 0) {
+      const int last = r.list[r.touched - 1];
+      slots = r.off[last] + __popc(r.mask[last]);
+    }
+    for (int s = warp; s < slots; s += kWarps) {
+      float amax = 0.f;
+      for (int i = lane; i < per_expert; i += 32) amax = fmaxf(amax, p.act_amax[(int64_t)s * per_expert + i]);
+      for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (lane == 0) scale8<K>(amax, row_scale[2 * s], row_scale[2 * s + 1]);
+    }
+    __syncthreads();
+  }
+
+  for (int u = u0; u < u1; ++u) {
+    float acc[1][NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[0][nt][i] = 0.f;
+
+    while (it < n_it && cur.u == u) {
+      Place nxt = cur;
+      nxt.kb += kWarps;
+      settle(nxt);
+      ws[0] = ws_next;
+      if (it + 1 < n_it) row_scales(ws_next, nxt);
+
+      const int e = r.list[cur.a], kb = cur.kb;
+      const uint32_t mask = r.mask[e];
+      const int off = r.off[e];
+      unsigned live = 0;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) live |= ((mask >> (8 * nt)) & 0xFFu) != 0u ? 1u << nt : 0u;
+
+      TokenBox<K> x[NT];
+      float xs[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (!((live >> nt) & 1u)) continue;
+        const int slot = slot_of(mask, off, 8 * nt + g);
+        if constexpr (is16(K)) {
+          load_token<K>(x[nt], slot < 0 ? nullptr : p.act_rows + (int64_t)slot * p.inter * 2, p.inter * 2, kb, t);
+        } else if constexpr (is8(K)) {
+          float v[32];
+          load_values32(v, slot < 0 ? nullptr : reinterpret_cast<const float*>(p.act_rows) + (int64_t)slot * p.inter,
+                        BOLT_F32, p.inter, kb * 128 + 32 * t);
+          float inv;
+          if constexpr (is_block(K)) {
+            float amax = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) amax = fmaxf(amax, fabsf(v[j]));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            scale8<K>(amax, xs[nt], inv);
+          } else {
+            inv = slot < 0 ? 0.f : row_scale[2 * slot + 1];
+          }
+          codes32<K>(v, inv, x[nt].w);
+        } else {
+          load_token<K>(x[nt], slot < 0 ? nullptr : p.act_rows + (int64_t)slot * (p.inter / 2), p.inter / 2, kb, t);
+          if constexpr (K == K_NV4) {
+            load_block_scales<K>(x[nt].sf, slot < 0 ? nullptr : p.act_sf + (int64_t)slot * sf_row, sf_row, kb, t);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int s = slot_of(mask, off, 8 * nt + 2 * t + i);
+              load_block_scales<K>(x[nt].sf + 2 * i, s < 0 ? nullptr : p.act_sf + (int64_t)s * sf_row, sf_row, kb, t);
+            }
+          }
+        }
+      }
+      float wr0 = 1.f, wr1 = 1.f;     // scale of weight rows g and g + 8
+      if constexpr (is_block(K)) {
+        wr0 = wr1 = static_cast<const float*>(p.s2)[((int64_t)e * (p.model_dim / 128) + u * kDownRows / 128) *
+                                                        (p.inter / 128) + kb];
+      } else if constexpr (is_channel(K)) {
+        const float* s2 = static_cast<const float*>(p.s2) + (int64_t)e * p.model_dim;
+        const int row = u * kDownRows + g;
+        wr0 = row < p.model_dim ? s2[row] : 0.f;
+        wr1 = row + 8 < p.model_dim ? s2[row + 8] : 0.f;
+      } else if constexpr (is4(K)) {
+        wr0 = wr1 = (p.g2 != nullptr ? p.g2[e] : 1.f) * (p.a2 != nullptr ? *p.a2 : 1.f);
+      }
+      const uint32_t box = ring.wait(abort_flag, p.status);
+      float part[1][NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[0][nt][i] = 0.f;
+      box_mma<K, 1, NT, false>(box, lane, x, ws, live, part);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (!((live >> nt) & 1u)) continue;
+        float s01[2] = {1.f, 1.f};
+        if constexpr (is_block(K)) {
+          s01[0] = __shfl_sync(0xffffffffu, xs[nt], 8 * t);
+          s01[1] = __shfl_sync(0xffffffffu, xs[nt], 8 * t + 4);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          // tokens that did not choose the expert get nothing (not even a NaN of its weights)
+          const int slot = slot_of(mask, off, 8 * nt + 2 * t + i);
+          if (slot < 0) continue;
+          float f = r.coef[slot] * s01[i];
+          if constexpr (is_channel(K)) f *= row_scale[2 * slot];
+          acc[0][nt][i] = fmaf(part[0][nt][i], f * wr0, acc[0][nt][i]);
+          acc[0][nt][2 + i] = fmaf(part[0][nt][2 + i], f * wr1, acc[0][nt][2 + i]);
+        }
+      }
+      ring.release();
+      if (in_it < n_it) bring();
+      cur = nxt;
+      ++it;
+    }
+
+    put_sums<1, NT>(red, acc, warp, lane, ~0u);
+    __syncthreads();
+    for (int i = tid; i < p.tokens * kDownRows; i += kThreads) {
+      const int n = i / kDownRows, c = i % kDownRows, col = u * kDownRows + c;
+      if (col >= p.model_dim) continue;
+      const float v = get_sum<1, NT>(red, 0, c >> 3, c & 7, n) * p.out_scale;
+      const int64_t at = (int64_t)n * p.model_dim + col;
+      if (p.out_dtype == BOLT_BF16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+      else if (p.out_dtype == BOLT_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
+      else static_cast<float*>(p.out)[at] = v;
+    }
+    __syncthreads();
+  }
+  finish(abort_flag);
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static const EncodeTiledFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
+        qres == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<EncodeTiledFn>(ptr);
+    return EncodeTiledFn(nullptr);
+  }();
+  return fn;
+}
+
+int encode(CUtensorMap* map, const void* base, int dims, const cuuint64_t* size, const cuuint64_t* strides,
+           const cuuint32_t* box) {
+  const EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) {
+    set_error("moe_decode: cuTensorMapEncodeTiled is not available");
+    return BOLT_ERR_CUDA;
+  }
+  const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+  const CUresult rc = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, dims, const_cast<void*>(base), size, strides, box,
+                         one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) {
+    set_error("moe_decode: cuTensorMapEncodeTiled failed (%d)", (int)rc);
+    return BOLT_ERR_CUDA;
+  }
+  return BOLT_OK;
+}
+
+inline size_t a256(size_t n) { return (n + 255) & ~size_t(255); }
+inline int a16(int n) { return (n + 15) & ~15; }
+
+// bytes of the three parts of the workspace
+void workspace_parts(const bolt_decode_args* a, size_t (&part)[3]) {
+  const size_t slots = (size_t)a->num_tokens * a->topk;
+  const int k = a->kind;
+  part[0] = a256(slots * (is8(k) ? 4 * (size_t)a->inter : (size_t)row_bytes(k, a->inter)));
+  part[1] = is4(k) ? a256(slots * (a->inter / (k == K_NV4 ? 16 : 32))) : 0;
+  part[2] = is_channel(k) ? a256(slots * ((a->inter + 15) / 16) * 4) : 0;
+}
+
+// Shared memory left over by the fixed parts goes to the rings.  Two blocks of 113 KB share an SM, so
+// that the second kernel's can come in beside the first's; where a ring would then hold less than
+// three boxes a warp (long 4-bit rows of many tokens, the sums of more than 16), one block takes all.
+constexpr int kHalfSm = 113 * 1024, kWholeSm = 226 * 1024;
+int ring_slots(int fixed, int box_bytes, int* total) {
+  int slots = (kHalfSm - fixed) / (kWarps * box_bytes);
+  if (slots < 3) slots = (kWholeSm - fixed) / (kWarps * box_bytes);
+  if (slots > kMaxSlots) slots = kMaxSlots;
+  *total = fixed + slots * kWarps * box_bytes;
+  return slots;
+}
+
+template <int K, int NT>
+int launch(const bolt_decode_args* a, const CUtensorMap& m1, const CUtensorMap& m2, Params p, cudaStream_t st) {
+  static std::atomic<bool> ready[2][kMaxDevices];
+  int rc = configure_kernel(k_few_up<K, NT>, kWholeSm, ready[0], 0, 0, 0, 0);
+  if (rc == BOLT_OK) rc = configure_kernel(k_few_down<K, NT>, kWholeSm, ready[1], 0, 0, 0, 0);
+  if (rc != BOLT_OK) return rc;
+  const int routes = a16(route_bytes(p.experts, p.tokens * p.topk));
+  int up = 1024 + kCtrlBytes + red_bytes(unit_cols(K) / 8, NT) + routes;
+  int down = 1024 + kCtrlBytes + red_bytes(1, NT) + routes;
+  if (is_channel(K)) {
+    up += 8 * p.tokens;
+    down += 8 * p.tokens * p.topk;
+  }
+  if (is4(K)) up += p.tokens * (p.hidden / 2 + p.hidden / (K == K_NV4 ? 16 : 32));
+  int up_bytes, down_bytes;
+  const int up_slots = ring_slots(up, up_box_bytes(K), &up_bytes);
+  const int down_slots = ring_slots(down, kDownBoxBytes, &down_bytes);
+  if (up_slots < 2 || down_slots < 2) {
+    set_error("moe_decode: %d tokens x hidden size %d do not fit in shared memory", p.tokens, p.hidden);
+    return BOLT_ERR_UNSUPPORTED;
+  }
+  const int sms = a->sm_count > 0 ? a->sm_count : sm_count_of_current_device();
+  p.slots_per_warp = up_slots;
+  k_few_up<K, NT><<<sms, kThreads, up_bytes, st>>>(m1, p);
+  BOLT_LAUNCH_CHECK();
+  p.slots_per_warp = down_slots;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(sms);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = down_bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  BOLT_CUDA(cudaLaunchKernelEx(&cfg, k_few_down<K, NT>, m2, p));
+  return BOLT_OK;
+}
+
+template <int K>
+int launch_kind(const bolt_decode_args* a, const CUtensorMap& m1, const CUtensorMap& m2, const Params& p,
+                cudaStream_t st) {
+  if (p.tokens <= 8) return launch<K, 1>(a, m1, m2, p, st);
+  if (p.tokens <= 16) return launch<K, 2>(a, m1, m2, p, st);
+  return launch<K, 4>(a, m1, m2, p, st);
+}
+
+int check_args(const bolt_decode_args* a) {
+  BOLT_REQUIRE(a != nullptr, "moe_decode: null args");
+  BOLT_REQUIRE(a->kind >= K_BF16 && a->kind <= K_MX4, "moe_decode: unknown kind %d", a->kind);
+  BOLT_REQUIRE(a->num_tokens >= 0 && a->num_tokens <= kMaxTokens, "moe_decode: %d tokens, at most %d",
+               a->num_tokens, kMaxTokens);
+  BOLT_REQUIRE(a->topk > 0 && a->topk <= 32, "moe_decode: topk %d out of range", a->topk);
+  BOLT_REQUIRE(a->num_experts > 0 && a->num_experts <= 1024 && a->global_num_experts > 0,
+               "moe_decode: at most 1024 local experts");
+  BOLT_REQUIRE(a->hidden > 0 && a->inter > 0 && a->model_dim > 0, "moe_decode: bad shape");
+  const int k = a->kind;
+  const int step = k == K_NV4 ? 64 : (k == K_MX4 || is_block(k)) ? 128 : is8(k) ? 16 : 8;
+  BOLT_REQUIRE(a->hidden % step == 0 && a->inter % step == 0,
+               "moe_decode: hidden size %d and intermediate size %d must be multiples of %d", a->hidden,
+               a->inter, step);
+  BOLT_REQUIRE(!is_block(k) || a->model_dim % 128 == 0, "moe_decode: output size %d must be a multiple of 128",
+               a->model_dim);
+  return BOLT_OK;
+}
+
+}  // namespace
+}  // namespace few
+}  // namespace bolt
+
+extern "C" size_t bolt_moe_decode_workspace_bytes(const bolt_decode_args* a) {
+  using namespace bolt::few;
+  if (check_args(a) != BOLT_OK) return 0;
+  size_t part[3];
+  workspace_parts(a, part);
+  return part[0] + part[1] + part[2] + 256;
+}
+
+extern "C" int bolt_moe_decode(const bolt_decode_args* a, void* stream) {
+  using namespace bolt;
+  using namespace bolt::few;
+  int rc = check_args(a);
+  if (rc != BOLT_OK) return rc;
+  if (a->num_tokens == 0) return BOLT_OK;
+  const int k = a->kind;
+  BOLT_REQUIRE(a->hidden_states && a->w1 && a->w2 && a->out && a->workspace, "moe_decode: null pointer");
+  BOLT_REQUIRE(is16(k) || (a->w1_scale && a->w2_scale), "moe_decode: scales required");
+  BOLT_REQUIRE(a->gating != nullptr || (a->topk_weights && a->topk_ids), "moe_decode: no routing");
+  BOLT_REQUIRE(a->gating == nullptr || (a->global_num_experts <= 32 * kMaxPerLane && a->topk <= a->global_num_experts),
+               "moe_decode: top-%d of %d experts", a->topk, a->global_num_experts);
+  BOLT_REQUIRE(a->gating == nullptr || a->gating_dtype == BOLT_F32 || a->gating_dtype == BOLT_BF16 ||
+                   a->gating_dtype == BOLT_F16,
+               "moe_decode: bad gating dtype %d", a->gating_dtype);
+  BOLT_REQUIRE(a->x_dtype == BOLT_BF16 || a->x_dtype == BOLT_F16, "moe_decode: rows must be 16-bit");
+  BOLT_REQUIRE(!is16(k) || a->x_dtype == (k == K_BF16 ? BOLT_BF16 : BOLT_F16),
+               "moe_decode: rows and weights of different types");
+  BOLT_REQUIRE(a->out_dtype == BOLT_BF16 || a->out_dtype == BOLT_F16 || a->out_dtype == BOLT_F32,
+               "moe_decode: bad output dtype %d", a->out_dtype);
+  BOLT_REQUIRE(((reinterpret_cast<uintptr_t>(a->hidden_states) | reinterpret_cast<uintptr_t>(a->w1) |
+                 reinterpret_cast<uintptr_t>(a->w2) | reinterpret_cast<uintptr_t>(a->workspace)) & 15) == 0,
+               "moe_decode: operands must be 16-byte aligned");
+  BOLT_REQUIRE(!is4(k) || ((reinterpret_cast<uintptr_t>(a->w1_scale) | reinterpret_cast<uintptr_t>(a->w2_scale)) & 3) == 0,
+               "moe_decode: scale bytes must be 4-byte aligned");
+  size_t part[3];
+  workspace_parts(a, part);
+  BOLT_REQUIRE(a->workspace_bytes >= part[0] + part[1] + part[2], "moe_decode: workspace too small");
+
+  Params p = {};
+  p.x = a->hidden_states;
+  p.x_dtype = a->x_dtype;
+  p.out_dtype = a->out_dtype;
+  p.tokens = a->num_tokens;
+  p.topk = a->topk;
+  p.hidden = a->hidden;
+  p.inter = a->inter;
+  p.model_dim = a->model_dim;
+  p.experts = a->num_experts;
+  p.global_experts = a->global_num_experts;
+  p.s1 = a->w1_scale;
+  p.s2 = a->w2_scale;
+  p.g1 = a->w1_global_scale;
+  p.g2 = a->w2_global_scale;
+  p.a1 = a->a1_global_scale;
+  p.a2 = a->a2_global_scale;
+  p.wts = a->topk_weights;
+  p.ids = a->topk_ids;
+  p.gating = a->gating;
+  p.gating_dtype = a->gating_dtype;
+  p.renormalize = a->renormalize;
+  p.softmax = a->is_softmax;
+  p.emap = a->expert_map;
+  p.act = {a->activation, 1, a->act_alpha, a->act_limit};
+  p.out_scale = a->routed_scaling_factor;
+  p.out = a->out;
+  p.act_rows = static_cast<uint8_t*>(a->workspace);
+  p.act_sf = p.act_rows + part[0];
+  p.act_amax = reinterpret_cast<float*>(p.act_sf + part[1]);
+  p.status = a->status;
+
+  CUtensorMap m1, m2;
+  {
+    const cuuint64_t kb = (cuuint64_t)row_bytes(k, a->hidden), i = a->inter;
+    const cuuint64_t size[4] = {kb, i, 2, (cuuint64_t)a->num_experts};
+    const cuuint64_t strides[3] = {kb, kb * i, 2 * kb * i};
+    const cuuint32_t box[4] = {128, (cuuint32_t)unit_cols(k), 2, 1};
+    if ((rc = encode(&m1, a->w1, 4, size, strides, box)) != BOLT_OK) return rc;
+  }
+  {
+    const cuuint64_t kb = (cuuint64_t)row_bytes(k, a->inter), n = a->model_dim;
+    const cuuint64_t size[3] = {kb, n, (cuuint64_t)a->num_experts};
+    const cuuint64_t strides[2] = {kb, kb * n};
+    const cuuint32_t box[3] = {128, kDownRows, 1};
+    if ((rc = encode(&m2, a->w2, 3, size, strides, box)) != BOLT_OK) return rc;
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (k) {
+    case K_BF16: return launch_kind<K_BF16>(a, m1, m2, p, st);
+    case K_F16: return launch_kind<K_F16>(a, m1, m2, p, st);
+    case K_F8_BLOCK: return launch_kind<K_F8_BLOCK>(a, m1, m2, p, st);
+    case K_I8_CHANNEL: return launch_kind<K_I8_CHANNEL>(a, m1, m2, p, st);
+    case K_F8_CHANNEL: return launch_kind<K_F8_CHANNEL>(a, m1, m2, p, st);
+    case K_I8_BLOCK: return launch_kind<K_I8_BLOCK>(a, m1, m2, p, st);
+    case K_NV4: return launch_kind<K_NV4>(a, m1, m2, p, st);
+    default: return launch_kind<K_MX4>(a, m1, m2, p, st);
+  }
+}

@@ -9,11 +9,10 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "routing_row.cuh"
 
 namespace bolt {
 namespace {
-
-constexpr int kMaxPerLane = 32;  // experts per lane -> up to 1024 experts
 
 template <typename T, int NPL>
 __global__ void __launch_bounds__(256) k_fused_topk(const T* __restrict__ logits, int64_t tokens,
@@ -27,71 +26,16 @@ __global__ void __launch_bounds__(256) k_fused_topk(const T* __restrict__ logits
   for (int64_t m = warp0; m < tokens; m += nwarps) {
     const T* row = logits + m * experts;
     float v[NPL];
-    float mx = -FLT_MAX;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
       const int e = lane + 32 * j;
       v[j] = (j < per_lane && e < experts) ? to_f32(row[e]) : -FLT_MAX;
-      mx = fmaxf(mx, v[j]);
     }
-    if (softmax) {
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < NPL; ++j) {
-        const int e = lane + 32 * j;
-        if (j < per_lane && e < experts) {
-          v[j] = expf(v[j] - mx);
-          sum += v[j];
-        } else {
-          v[j] = -3.f;  // never offered
-        }
-      }
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float inv = 1.0f / sum;
-#pragma unroll
-      for (int j = 0; j < NPL; ++j)
-        if (v[j] >= 0.f) v[j] *= inv;
-    } else {
-#pragma unroll
-      for (int j = 0; j < NPL; ++j) {
-        const int e = lane + 32 * j;
-        v[j] = (j < per_lane && e < experts) ? 1.0f / (1.0f + expf(-v[j])) : -3.f;
-      }
-    }
-    // top-k by repeated warp arg-max (ties: lowest expert index)
-    float my_w = 0.f;
-    int my_id = 0;
-    int past_end = 0;
-    float total = 0.f;
-    for (int k = 0; k < topk; ++k) {
-      float best = -2.f;
-      int best_e = 0x7fffffff;
-#pragma unroll
-      for (int j = 0; j < NPL; ++j) {
-        const int e = lane + 32 * j;
-        if (v[j] > best) { best = v[j]; best_e = e; }
-      }
-      // (scores are not negative, and a lane that holds none offers -2: their bit patterns order
-      // like the values as signed integers)
-      const int top = __reduce_max_sync(0xffffffffu, __float_as_int(best));
-      best_e = __reduce_min_sync(0xffffffffu, __float_as_int(best) == top ? best_e : 0x7fffffff);
-      best = __int_as_float(top);
-      if (top < 0) {   // all that is left is NaN: ids past the last expert, which the sort drops
-        best_e = experts + past_end++;
-        if (best_e < 32 * kMaxPerLane) best = -1.f;
-        else best_e = 0x7fffffff;
-      }
-      if ((best_e & 31) == lane) {
-#pragma unroll
-        for (int j = 0; j < NPL; ++j)
-          if (lane + 32 * j == best_e) v[j] = -3.f;  // taken
-      }
-      if (lane == k) { my_w = best; my_id = best_e; }
-      total += best;
-    }
+    float my_w;
+    int my_id;
+    topk_of_row<NPL>(v, experts, topk, renormalize, softmax, lane, my_w, my_id);
     if (lane < topk) {
-      weights[m * topk + lane] = renormalize ? my_w / total : my_w;
+      weights[m * topk + lane] = my_w;
       ids[m * topk + lane] = my_id;
     }
   }

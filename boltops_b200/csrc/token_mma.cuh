@@ -1,0 +1,369 @@
+// Products of streamed weights with a few rows of activations (1 to 32 tokens), shared by the
+// few-token layer and the few-row 4-bit projection.
+//
+// At these sizes a product reads every weight once for a handful of multiply-adds, so it is bound by
+// HBM, and what matters is that every SM always has enough bytes in flight and spends few
+// instructions per byte:
+//
+// * Each of a block's eight warps owns a ring of shared-memory slots and fills it itself with bulk
+//   tensor copies of (rows x 128 bytes) boxes; no warp waits for another inside a reduction.  The
+//   warps share out the boxes of a unit (a few weight rows over the whole reduction) and add up
+//   their accumulators through shared memory once per unit.
+// * The weights are the A operand (16 rows) of mma.sync.m16n8k16, the tokens its eight columns.
+//   tcgen05 wants 128 rows on the A side and its operands in shared memory in their final format;
+//   here the 8- and 4-bit codes are widened to halves in registers on the way (exact: e4m3, int8
+//   and e2m1 x e4m3 all fit a half), and the instruction rate is far from what bounds the kernel.
+// * The K order inside a box is free as long as both operands agree.  A lane takes 32 contiguous
+//   bytes of its row (two 16-byte chunks, which the 128-byte swizzle places without bank
+//   conflicts), and the same 32 bytes' worth of its token.  MX codes go by 4-byte words instead, so
+//   that one instruction pair covers exactly one 32-value block, whose scales multiply the fp32
+//   partial sum: two E8M0 scales span more than a half's exponent.
+#pragma once
+
+#include "fp4.cuh"
+#include "tc_ptx.cuh"
+
+namespace bolt {
+namespace few {
+using namespace tc;
+
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kMaxTokens = 32;
+
+// values of enum bolt_decode_kind
+enum Kind { K_BF16, K_F16, K_F8_BLOCK, K_I8_CHANNEL, K_F8_CHANNEL, K_I8_BLOCK, K_NV4, K_MX4 };
+constexpr bool is16(int k) { return k == K_BF16 || k == K_F16; }
+constexpr bool is4(int k) { return k == K_NV4 || k == K_MX4; }
+constexpr bool is8(int k) { return !is16(k) && !is4(k); }
+constexpr bool is_i8(int k) { return k == K_I8_CHANNEL || k == K_I8_BLOCK; }
+constexpr bool is_block(int k) { return k == K_F8_BLOCK || k == K_I8_BLOCK; }
+constexpr bool is_channel(int k) { return k == K_F8_CHANNEL || k == K_I8_CHANNEL; }
+constexpr int box_elems(int k) { return is16(k) ? 64 : is4(k) ? 256 : 128; }   // in 128 bytes
+// bytes of a row of n values
+__host__ __device__ constexpr int64_t row_bytes(int k, int64_t n) {
+  return is16(k) ? 2 * n : is4(k) ? n / 2 : n;
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0,
+                                            int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
+      "{%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+// The next kernel of the stream may start (it still waits for this one before it reads its results).
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;"); }
+// All earlier kernels of the stream are done and their writes can be read.
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+template <bool BF>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (BF)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// four 8-bit codes -> two packed pairs of halves, exact
+template <bool INT>
+__device__ __forceinline__ void halves4(uint32_t w, uint32_t& p0, uint32_t& p1) {
+  if (INT) {
+    // 0x6400 + u is the half 1024 + u; u = code + 128
+    const uint32_t u = w ^ 0x80808080u;
+    const uint32_t lo = __byte_perm(u, 0x64646464u, 0x4140), hi = __byte_perm(u, 0x64646464u, 0x4342);
+    const uint32_t off = 0x64806480u;      // 1024 + 128
+    const __half2 o = *reinterpret_cast<const __half2*>(&off);
+    const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), o);
+    const __half2 b = __hsub2(*reinterpret_cast<const __half2*>(&hi), o);
+    p0 = *reinterpret_cast<const uint32_t*>(&a);
+    p1 = *reinterpret_cast<const uint32_t*>(&b);
+  } else {
+    asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %2;\ncvt.rn.f16x2.e4m3x2 %0, lo;\n"
+        "cvt.rn.f16x2.e4m3x2 %1, hi;\n}\n"
+        : "=r"(p0), "=r"(p1)
+        : "r"(w));
+  }
+}
+// E4M3 scale byte i of a word, in both halves of a pair
+__device__ __forceinline__ uint32_t scale_pair(uint32_t w, int i) {
+  uint32_t lo, hi;
+  halves4<false>(w, lo, hi);
+  return __byte_perm(i < 2 ? lo : hi, 0u, (i & 1) ? 0x3232 : 0x1010);
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// 32 bytes of one token, as the lane (column lane / 4, position lane % 4) multiplies them, with the
+// scales of 4-bit codes: NV the lane's own four E4M3 bytes, MX the eight E8M0 bytes of the columns
+// 2 (lane % 4) and 2 (lane % 4) + 1.
+template <int K>
+struct TokenBox {
+  uint32_t w[8];
+  uint32_t sf[is4(K) ? (K == K_MX4 ? 4 : 1) : 1];
+};
+// Scales of 4-bit weight rows g and g + 8 of a tile (NV: of the lane's 64 values; MX: of the box).
+template <int K>
+struct RowScales {
+  uint32_t sf[2][is4(K) ? (K == K_MX4 ? 2 : 1) : 1];
+};
+
+// d[tile][token tile] += (box of weights) . (tokens).  The box: rows of 128 bytes, swizzled.  Tile
+// mt holds the box's rows 8 mt + g and 8 MT + 8 mt + g (UP: a gate row with its up row) or
+// 16 mt + g and 16 mt + 8 + g.  Only the token tiles of `live` are computed.
+template <int K, int MT, int NT, bool UP>
+__device__ __forceinline__ void box_mma(uint32_t box, int lane, const TokenBox<K> (&x)[NT],
+                                        const RowScales<K> (&ws)[MT], unsigned live,
+                                        float (&d)[MT][NT][4]) {
+  const int g = lane >> 2, t = lane & 3;
+  uint32_t row[MT][2];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    row[mt][0] = box + (uint32_t)((UP ? 8 * mt : 16 * mt) + g) * 128u;
+    row[mt][1] = box + (uint32_t)((UP ? 8 * MT + 8 * mt : 16 * mt + 8) + g) * 128u;
+  }
+  if constexpr (K == K_MX4) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const uint32_t at = (uint32_t)((c ^ g) << 4) + 4u * t;
+      uint32_t a[MT][2][4];
+      float sw[MT][2];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          fp4::halves8(lds32(row[mt][r] + at), a[mt][r]);
+          sw[mt][r] = fp4::e8m0_to_f32((ws[mt].sf[r][c >> 2] >> (8 * (c & 3))) & 0xFFu);
+        }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (!((live >> nt) & 1u)) continue;
+        uint32_t b[4];
+        fp4::halves8(x[nt].w[c], b);
+        const float s0 = fp4::e8m0_to_f32((x[nt].sf[c >> 2] >> (8 * (c & 3))) & 0xFFu);
+        const float s1 = fp4::e8m0_to_f32((x[nt].sf[2 + (c >> 2)] >> (8 * (c & 3))) & 0xFFu);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          float part[4] = {0.f, 0.f, 0.f, 0.f};
+          mma16816<false>(part, a[mt][0][0], a[mt][1][0], a[mt][0][1], a[mt][1][1], b[0], b[1]);
+          mma16816<false>(part, a[mt][0][2], a[mt][1][2], a[mt][0][3], a[mt][1][3], b[2], b[3]);
+          d[mt][nt][0] = fmaf(part[0], sw[mt][0] * s0, d[mt][nt][0]);
+          d[mt][nt][1] = fmaf(part[1], sw[mt][0] * s1, d[mt][nt][1]);
+          d[mt][nt][2] = fmaf(part[2], sw[mt][1] * s0, d[mt][nt][2]);
+          d[mt][nt][3] = fmaf(part[3], sw[mt][1] * s1, d[mt][nt][3]);
+        }
+      }
+    }
+    return;
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t at = (uint32_t)(((2 * t + h) ^ g) << 4);
+      uint32_t a[MT][2][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint4 v = lds128(row[mt][r] + at);
+          a[mt][r][0] = v.x;
+          a[mt][r][1] = v.y;
+          a[mt][r][2] = v.z;
+          a[mt][r][3] = v.w;
+        }
+      if constexpr (is16(K)) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            if (!((live >> nt) & 1u)) continue;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+              mma16816<K == K_BF16>(d[mt][nt], a[mt][0][2 * s], a[mt][1][2 * s], a[mt][0][2 * s + 1],
+                                    a[mt][1][2 * s + 1], x[nt].w[4 * h + 2 * s],
+                                    x[nt].w[4 * h + 2 * s + 1]);
+          }
+      } else if constexpr (is8(K)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t p[MT][2][2];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) halves4<is_i8(K)>(a[mt][r][j], p[mt][r][0], p[mt][r][1]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            if (!((live >> nt) & 1u)) continue;
+            uint32_t b0, b1;
+            halves4<is_i8(K)>(x[nt].w[4 * h + j], b0, b1);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+              mma16816<false>(d[mt][nt], p[mt][0][0], p[mt][1][0], p[mt][0][1], p[mt][1][1], b0, b1);
+          }
+        }
+      } else {   // NV: codes times their block's scale, exact in a half
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int blk = 2 * h + (j >> 1);
+          uint32_t p[MT][2][4];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              fp4::halves8(a[mt][r][j], p[mt][r]);
+              const uint32_t s = scale_pair(ws[mt].sf[r][0], blk);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) p[mt][r][i] = hmul2(p[mt][r][i], s);
+            }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            if (!((live >> nt) & 1u)) continue;
+            uint32_t b[4];
+            fp4::halves8(x[nt].w[4 * h + j], b);
+            const uint32_t s = scale_pair(x[nt].sf[0], blk);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] = hmul2(b[i], s);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              mma16816<false>(d[mt][nt], p[mt][0][0], p[mt][1][0], p[mt][0][1], p[mt][1][1], b[0], b[1]);
+              mma16816<false>(d[mt][nt], p[mt][0][2], p[mt][1][2], p[mt][0][3], p[mt][1][3], b[2], b[3]);
+            }
+          }
+        }
+      }
+    }
+  }
+}
+
+// One token's 32 bytes of box kb out of rows that are stored in the operand's format (16-bit values,
+// 4-bit codes): `row` is the token's row or null (zeros), `bytes` its length.
+template <int K>
+__device__ __forceinline__ void load_token(TokenBox<K>& x, const uint8_t* row, int bytes, int kb, int t) {
+  if constexpr (K == K_MX4) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const int off = kb * 128 + 16 * c;
+      x.w[c] = row != nullptr && off < bytes ? *reinterpret_cast<const uint32_t*>(row + off + 4 * t) : 0u;
+    }
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int off = kb * 128 + 32 * t + 16 * h;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (row != nullptr && off < bytes) v = *reinterpret_cast<const uint4*>(row + off);
+      x.w[4 * h] = v.x;
+      x.w[4 * h + 1] = v.y;
+      x.w[4 * h + 2] = v.z;
+      x.w[4 * h + 3] = v.w;
+    }
+  }
+}
+// Block scales of box kb out of a row of `bytes` scale bytes (a multiple of four): NV the word of
+// the lane's own 64 values, MX both words of the box.
+template <int K>
+__device__ __forceinline__ void load_block_scales(uint32_t* sf, const uint8_t* row, int bytes, int kb,
+                                                  int t) {
+  if constexpr (K == K_NV4) {
+    const int off = kb * 16 + 4 * t;
+    sf[0] = row != nullptr && off < bytes ? *reinterpret_cast<const uint32_t*>(row + off) : 0u;
+  } else if constexpr (K == K_MX4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int off = kb * 8 + 4 * i;
+      sf[i] = row != nullptr && off < bytes ? *reinterpret_cast<const uint32_t*>(row + off) : 0u;
+    }
+  }
+}
+
+// 32 values -> 32 8-bit codes, the arithmetic of the row quantisers (quant.cu).
+template <int K>
+__device__ __forceinline__ void codes32(const float (&v)[32], float inv, uint32_t (&w)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float* q = v + 4 * j;
+    if (is_i8(K)) {
+      w[j] = ((uint32_t)(uint8_t)f32_to_i8(q[0] * inv)) | ((uint32_t)(uint8_t)f32_to_i8(q[1] * inv) << 8) |
+             ((uint32_t)(uint8_t)f32_to_i8(q[2] * inv) << 16) |
+             ((uint32_t)(uint8_t)f32_to_i8(q[3] * inv) << 24);
+    } else {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(q[0] * inv, q[1] * inv), __NV_SATFINITE,
+                                                   __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(q[2] * inv, q[3] * inv), __NV_SATFINITE,
+                                                   __NV_E4M3);
+      w[j] = lo | (hi << 16);
+    }
+  }
+}
+template <int K>
+__device__ __forceinline__ void scale8(float amax, float& scale, float& inv) {
+  scale = __fdiv_rn(fmaxf(amax, 1.0e-10f), is_i8(K) ? 127.0f : 448.0f);
+  inv = __frcp_rn(scale);
+}
+
+// 32 consecutive values of a row as floats; dt BOLT_BF16 / BOLT_F16 / BOLT_F32.  Chunks of 16 that
+// begin at or after `cols` are zeros.
+__device__ __forceinline__ void load_values32(float (&v)[32], const void* row, int dt, int cols, int at) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int c = at + 16 * h;
+    const bool ok = row != nullptr && c < cols;
+    if (dt == BOLT_F32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (ok) f = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + c + 4 * i);
+        v[16 * h + 4 * i] = f.x;
+        v[16 * h + 4 * i + 1] = f.y;
+        v[16 * h + 4 * i + 2] = f.z;
+        v[16 * h + 4 * i + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint4 u = make_uint4(0u, 0u, 0u, 0u);
+        if (ok) u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + c + 8 * i);
+        const uint32_t q[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float2 f;
+          if (dt == BOLT_BF16) {
+            f.x = __uint_as_float(q[j] << 16);
+            f.y = __uint_as_float(q[j] & 0xFFFF0000u);
+          } else {
+            f = __half22float2(*reinterpret_cast<const __half2*>(&q[j]));
+          }
+          v[16 * h + 8 * i + 2 * j] = f.x;
+          v[16 * h + 8 * i + 2 * j + 1] = f.y;
+        }
+      }
+    }
+  }
+}
+
+}  // namespace few
+}  // namespace bolt

@@ -1,0 +1,109 @@
+"""Microscaled 4-bit floating point: rows to e2m1 codes with a scale per block, and back.
+
+Two formats.  ``"nvfp4"``: blocks of 16 values, an E4M3 scale each, optionally one fp32 scale for the
+whole tensor.  ``"mxfp4"``: blocks of 32, an E8M0 scale (a power of two) each.  Codes are packed two to
+a byte along the last dimension, the first value in the low bits; a tensor's format is the dtype of
+its scales, ``torch.float8_e4m3fn`` or ``torch.uint8``, wherever the framework takes one.  The products
+that read them: ``gemm.gemm_a4w4``, ``fused_moe.fused_experts_fp4`` and ``fused_moe.fused_experts_decode``.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _cabi
+from ._cabi import check, dtype_code, ptr, stream_of
+
+FORMATS = {"nvfp4": (_cabi.FP4_NV, 16, torch.float8_e4m3fn), "mxfp4": (_cabi.FP4_MX, 32, torch.uint8)}
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def format_of(scales: torch.Tensor) -> str:
+    """The format that scales of this dtype belong to."""
+    for name, (_, _, dtype) in FORMATS.items():
+        if scales.dtype == dtype:
+            return name
+    raise TypeError(f"4-bit scales are float8_e4m3fn (nvfp4) or uint8 (mxfp4), not {scales.dtype}")
+
+
+def check_global_scale(name: str, scale: Optional[torch.Tensor], fmt: str, numel: int,
+                       device: torch.device) -> Optional[torch.Tensor]:
+    """A whole-tensor scale as the kernels read it: ``numel`` fp32 values on ``device``, or None."""
+    if scale is None:
+        return None
+    if fmt != "nvfp4":
+        raise ValueError(f"{name}: mxfp4 has no scale of the whole tensor")
+    if scale.numel() != numel or scale.dtype != torch.float32:
+        raise ValueError(f"{name} must hold {numel} float32 value(s)")
+    if scale.device != device:
+        raise ValueError(f"{name} is on {scale.device}, the rows on {device}")
+    return scale.contiguous()
+
+
+def fp4_quant(x: torch.Tensor, format: str = "nvfp4", global_scale: Optional[torch.Tensor] = None
+              ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(codes [..., K/2] uint8, scales [..., K/block])`` of ``x`` [..., K] (bf16, fp16 or fp32).
+
+    nvfp4: ``y = x * (1 / global_scale)``, ``scale = e4m3(min(amax(y) / 6, 448))``; mxfp4: the smallest
+    power of two that is at least ``amax / 6`` (byte 0 for a block of zeros).  A code is the nearest of
+    ``value / scale``, ties to even.  A block that holds a NaN or an infinity gets the NaN scale and
+    reads back as NaNs."""
+    if format not in FORMATS:
+        raise ValueError(f"unknown 4-bit format {format!r}: nvfp4 or mxfp4")
+    code, block, scale_dtype = FORMATS[format]
+    if not x.is_cuda:
+        raise ValueError("boltops_b200 kernels need CUDA tensors (there is no CPU path)")
+    if x.dtype not in _FLOATS:
+        raise TypeError(f"fp4_quant takes bf16, fp16 or fp32, not {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] % block:
+        raise ValueError(f"the last dimension must be whole blocks of {block} values ({format})")
+    g = check_global_scale("global_scale", global_scale, format, 1, x.device)
+    x = x.contiguous()
+    if x.data_ptr() % 16:
+        x = x.clone()
+    cols = x.shape[-1]
+    codes = torch.empty((*x.shape[:-1], cols // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((*x.shape[:-1], cols // block), dtype=scale_dtype, device=x.device)
+    if x.numel() == 0:
+        return codes, scales
+    with _cabi.on_device(x.device):
+        check(_cabi.load().bolt_fp4_quant(ptr(x), dtype_code(x.dtype), x.numel() // cols, cols, code,
+                                          ptr(g), ptr(codes), ptr(scales), stream_of(x)))
+    from .fused_moe import ops
+    ops._count()
+    return codes, scales
+
+
+def fp4_dequant(codes: torch.Tensor, scales: torch.Tensor, global_scale: Optional[torch.Tensor] = None,
+                dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values ``code * scale * global_scale`` [..., K] of packed codes [..., K/2]."""
+    format = format_of(scales)
+    code, block, _ = FORMATS[format]
+    if not codes.is_cuda:
+        raise ValueError("boltops_b200 kernels need CUDA tensors (there is no CPU path)")
+    if codes.dtype != torch.uint8 or dtype not in _FLOATS:
+        raise TypeError("fp4_dequant takes uint8 codes and gives bf16, fp16 or fp32")
+    if codes.dim() < 1 or (2 * codes.shape[-1]) % block or \
+            tuple(scales.shape) != (*codes.shape[:-1], 2 * codes.shape[-1] // block):
+        raise ValueError(f"scales {tuple(scales.shape)} do not belong to codes {tuple(codes.shape)} "
+                         f"in blocks of {block}")
+    if scales.device != codes.device:
+        raise ValueError(f"scales are on {scales.device}, codes on {codes.device}")
+    g = check_global_scale("global_scale", global_scale, format, 1, codes.device)
+    codes, scales = codes.contiguous(), scales.contiguous()
+    if codes.data_ptr() % 4:
+        codes = codes.clone()
+    cols = 2 * codes.shape[-1]
+    out = torch.empty((*codes.shape[:-1], cols), dtype=dtype, device=codes.device)
+    if out.numel() == 0:
+        return out
+    with _cabi.on_device(codes.device):
+        check(_cabi.load().bolt_fp4_dequant(ptr(codes), ptr(scales), out.numel() // cols, cols, code,
+                                            ptr(g), ptr(out), dtype_code(dtype), stream_of(codes)))
+    from .fused_moe import ops
+    ops._count()
+    return out
+
+
+__all__ = ["fp4_quant", "fp4_dequant"]

@@ -108,8 +108,12 @@ def moe_activation(
          activation_situ_linear_beta=activation_situ_linear_beta)
 
 
+from .decode import fused_experts_decode, fused_moe_decode  # noqa: E402
+
 __all__ = [
     "fused_experts",
+    "fused_experts_decode",
+    "fused_moe_decode",
     "normalize_moe_activation",
     "moe_activation_output_size",
     "moe_activation",

@@ -1,0 +1,326 @@
+"""A whole expert layer for a few decoding tokens, in two kernels.
+
+``fused_experts`` is built for any number of tokens: it sorts the routes, places rows, multiplies and
+combines in five to seven launches.  With one or a few tokens these launches and the half-empty tiles are
+a large part of the time.  The forms here take 1 to 32 tokens and leave out everything but
+the weights: routing is a bit mask per expert that every block of the kernel builds for itself, the
+first kernel does gate, up and activation, the second the down projection and the sum over a token's
+experts, and it fills its weight rings while the first one finishes.
+
+Same recipes as ``fused_experts`` (16-bit, fp8 and int8 w8a8 block-scaled and per-channel) and
+``fused_experts_fp4`` (w4a4), with fewer roundings: GEMM 1 and the routes' results stay in fp32, quantised
+experts quantise the fp32 activation, 16-bit experts round it to the weights' type.
+"""
+from __future__ import annotations
+
+from typing import List, Optional
+
+import torch
+
+from .. import _cabi
+from ..fp4 import FORMATS, check_global_scale, format_of
+from . import ops
+from .activation import normalize_moe_activation, resolve_kernel
+
+MAX_TOKENS = 32
+_FLOAT_OUT = (torch.float16, torch.bfloat16, torch.float32)
+_16BIT = (torch.bfloat16, torch.float16)
+
+
+def _kind(w1, w1_scale, use_fp8_w8a8, use_int8_w8a8, use_fp4_w4a4, per_channel_quant, block_shape) -> int:
+    if use_fp8_w8a8 + use_int8_w8a8 + use_fp4_w4a4 > 1:
+        raise ValueError("the quantisation flags exclude each other")
+    if use_fp4_w4a4:
+        if per_channel_quant:
+            raise ValueError("w4a4 experts have block scales, per_channel_quant does not apply")
+        fmt = format_of(w1_scale)
+        if block_shape is not None and list(block_shape) != [1, FORMATS[fmt][1]]:
+            raise ValueError(f"{fmt} block_shape must be [1, {FORMATS[fmt][1]}]")
+        return _cabi.DECODE_NVFP4 if fmt == "nvfp4" else _cabi.DECODE_MXFP4
+    if use_fp8_w8a8 or use_int8_w8a8:
+        if not per_channel_quant:
+            if block_shape is None:
+                raise NotImplementedError("per-tensor quantised experts are not built in boltops_b200")
+            if list(block_shape) != [128, 128]:
+                raise NotImplementedError("only block_shape [128, 128] is built in boltops_b200")
+            return _cabi.DECODE_FP8_BLOCK if use_fp8_w8a8 else _cabi.DECODE_INT8_BLOCK
+        return _cabi.DECODE_FP8_CHANNEL if use_fp8_w8a8 else _cabi.DECODE_INT8_CHANNEL
+    if w1.dtype == torch.bfloat16:
+        return _cabi.DECODE_BF16
+    if w1.dtype == torch.float16:
+        return _cabi.DECODE_F16
+    raise NotImplementedError(f"unquantised experts in {w1.dtype} are not built in boltops_b200")
+
+
+def check_weights(kind_name, w1, w2, w1_scale, w2_scale, hidden, w_dtype, scale_dtype, pack, scale1, scale2,
+                  dev):
+    """Shapes, types and devices of the weights and their scales; returns (experts, inter, model_dim)."""
+    if w1.dim() != 3 or w2.dim() != 3:
+        raise ValueError("w1 and w2 are [experts, rows, columns]")
+    e, n1, k1 = w1.shape
+    model_dim, inter = w2.shape[1], n1 // 2
+    if n1 % 2 or k1 * pack != hidden:
+        raise ValueError(f"w1 {tuple(w1.shape)} does not fit {hidden} hidden columns ({kind_name})")
+    if w2.shape[0] != e or w2.shape[2] * pack != inter:
+        raise ValueError(f"w2 {tuple(w2.shape)} does not fit w1 {tuple(w1.shape)} ({kind_name})")
+    if w1.dtype != w_dtype or w2.dtype != w_dtype:
+        raise TypeError(f"{kind_name} weights are {w_dtype}")
+    for name, t in (("w1", w1), ("w2", w2), ("w1_scale", w1_scale), ("w2_scale", w2_scale)):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, hidden_states on {dev}")
+    if scale_dtype is not None:
+        for name, s, shape in (("w1_scale", w1_scale, scale1(e, n1, hidden)),
+                               ("w2_scale", w2_scale, scale2(e, model_dim, inter))):
+            if s is None:
+                raise ValueError(f"{name} is required ({kind_name})")
+            if s.numel() != _numel(shape):
+                raise ValueError(f"{name} {tuple(s.shape)}: expected {shape} ({kind_name})")
+            if scale_dtype != torch.float32 and s.dtype != scale_dtype:
+                raise TypeError(f"{name} must be {scale_dtype} ({kind_name})")
+    return e, inter, model_dim
+
+
+def _numel(shape):
+    n = 1
+    for s in shape:
+        n *= s
+    return n
+
+
+def _aligned(t: torch.Tensor, to: int = 16) -> torch.Tensor:
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % to else t
+
+
+def _decode(hidden_states, w1, w2, topk_weights, topk_ids, gating, topk, renormalize, is_softmax, *,
+            use_fp8_w8a8, use_int8_w8a8, use_fp4_w4a4, per_channel_quant, block_shape, w1_scale, w2_scale,
+            w1_global_scale, w2_global_scale, a1_global_scale, a2_global_scale, activation, gemm1_alpha,
+            gemm1_limit, activation_situ_beta, activation_situ_linear_beta, global_num_experts, expert_map,
+            routed_scaling_factor, output_dtype, out):
+    if not hidden_states.is_cuda:
+        raise ValueError("boltops_b200 kernels need CUDA tensors (there is no CPU path)")
+    if hidden_states.dim() != 2 or hidden_states.dtype not in _16BIT:
+        raise ValueError("hidden_states must be [tokens, hidden] in bf16 or fp16")
+    m, hidden = hidden_states.shape
+    if m > MAX_TOKENS:
+        raise NotImplementedError(f"{m} tokens: this form takes at most {MAX_TOKENS}, fused_experts any number")
+    if (use_fp4_w4a4 or use_fp8_w8a8 or use_int8_w8a8) and (w1_scale is None or w2_scale is None):
+        raise ValueError("quantised experts need w1_scale and w2_scale")
+    kind = _kind(w1, w1_scale, use_fp8_w8a8, use_int8_w8a8, use_fp4_w4a4, per_channel_quant, block_shape)
+    dev = hidden_states.device
+    fp4 = kind in (_cabi.DECODE_NVFP4, _cabi.DECODE_MXFP4)
+    if fp4:
+        fmt = format_of(w1_scale)
+        block = FORMATS[fmt][1]
+        e, inter, model_dim = check_weights(
+            fmt, w1, w2, w1_scale, w2_scale, hidden, torch.uint8, FORMATS[fmt][2], 2,
+            *[lambda e, n, k: (e, n, k // block)] * 2, dev)
+    else:
+        fmt = None
+        if any(t is not None for t in (w1_global_scale, w2_global_scale, a1_global_scale, a2_global_scale)):
+            raise ValueError("scales of whole tensors belong to use_fp4_w4a4")
+        if use_fp8_w8a8 or use_int8_w8a8:
+            w_dtype = torch.float8_e4m3fn if use_fp8_w8a8 else torch.int8
+            shape = (lambda e, n, k: (e, n)) if per_channel_quant else \
+                (lambda e, n, k: (e, n // 128, k // 128))
+            if not per_channel_quant and (hidden % 128 or w1.shape[1] % 256 or w2.shape[1] % 128):
+                raise NotImplementedError("block-scaled experts need sizes in multiples of 128")
+            for name, s in (("w1_scale", w1_scale), ("w2_scale", w2_scale)):
+                if s.dtype not in _FLOAT_OUT:
+                    raise ValueError(f"{name} must be a decoded floating-point multiplier")
+            e, inter, model_dim = check_weights("w8a8", w1, w2, w1_scale, w2_scale, hidden, w_dtype,
+                                                torch.float32, 1, shape, shape, dev)
+            w1_scale, w2_scale = w1_scale.float(), w2_scale.float()
+        else:
+            if w1_scale is not None or w2_scale is not None:
+                raise ValueError("unquantised experts take no scales")
+            e, inter, model_dim = check_weights("16-bit", w1, w2, None, None, hidden, hidden_states.dtype,
+                                                None, 1, None, None, dev)
+    step = {_cabi.DECODE_NVFP4: 64, _cabi.DECODE_MXFP4: 128}.get(kind, 128 if not per_channel_quant else 16) \
+        if (fp4 or use_fp8_w8a8 or use_int8_w8a8) else 8
+    if hidden % step or inter % step:
+        raise NotImplementedError(f"hidden size {hidden} and intermediate size {inter} must be multiples "
+                                  f"of {step} here")
+    if e == 0 or e > 1024:
+        raise NotImplementedError("1 to 1024 local experts")
+    if expert_map is not None:
+        if expert_map.dim() != 1 or expert_map.device != dev:
+            raise ValueError(f"expert_map must be one row of entries on {dev}")
+        if global_num_experts == -1:
+            global_num_experts = expert_map.numel()
+        if expert_map.numel() < global_num_experts:
+            raise ValueError("expert_map has fewer entries than there are experts")
+        expert_map = expert_map.to(torch.int32).contiguous()
+    elif global_num_experts == -1:
+        global_num_experts = e
+    activation, is_gated = normalize_moe_activation("silu" if activation is None else activation)
+    if not is_gated or activation == "swigluoai":
+        raise NotImplementedError("gated activations on [gate | up] rows only")
+    act, alpha, limit = resolve_kernel(activation, True, gemm1_alpha, gemm1_limit, activation_situ_beta,
+                                       activation_situ_linear_beta)
+    out_dtype = hidden_states.dtype if output_dtype is None else output_dtype
+    if out_dtype not in _FLOAT_OUT:
+        raise ValueError("output_dtype must be bf16, fp16 or fp32")
+    if out is None:
+        out = torch.empty((m, model_dim), dtype=out_dtype, device=dev)
+    elif tuple(out.shape) != (m, model_dim) or out.dtype != out_dtype or out.device != dev \
+            or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {out_dtype} [{m}, {model_dim}] on {dev}")
+
+    args = _cabi.DecodeArgs()
+    keep = []
+    if gating is not None:
+        if gating.dim() != 2 or tuple(gating.shape) != (m, global_num_experts) or gating.device != dev:
+            raise ValueError(f"gating_output must be [{m}, {global_num_experts}] on {dev}")
+        if gating.dtype not in _FLOAT_OUT:
+            raise ValueError("gating_output must be bf16, fp16 or fp32")
+        if global_num_experts > 1024:
+            raise NotImplementedError("the router takes at most 1024 experts")
+        if not 1 <= topk <= min(32, global_num_experts):
+            raise ValueError(f"topk {topk} out of range")
+        gating = gating.contiguous()
+        args.gating, args.gating_dtype = gating.data_ptr(), _cabi.dtype_code(gating.dtype)
+        args.renormalize, args.is_softmax = int(renormalize), int(is_softmax)
+    else:
+        if topk_ids.dim() != 2 or topk_weights.shape != topk_ids.shape or topk_ids.shape[0] != m:
+            raise ValueError("topk_weights and topk_ids must both be [tokens, topk]")
+        for name, t in (("topk_weights", topk_weights), ("topk_ids", topk_ids)):
+            if t.device != dev:
+                raise ValueError(f"{name} is on {t.device}, hidden_states on {dev}")
+        topk = topk_ids.shape[1]
+        if not 1 <= topk <= 32:
+            raise ValueError(f"topk {topk} out of range")
+        ids = topk_ids.to(torch.int32).contiguous()
+        wts = topk_weights.to(torch.float32).contiguous()
+        keep += [ids, wts]
+        args.topk_ids, args.topk_weights = ids.data_ptr(), wts.data_ptr()
+    if m == 0:
+        return out
+
+    x = _aligned(hidden_states)
+    w1, w2 = _aligned(w1), _aligned(w2)
+    args.kind, args.x_dtype, args.out_dtype = kind, _cabi.dtype_code(x.dtype), _cabi.dtype_code(out_dtype)
+    args.num_tokens, args.topk = m, topk
+    args.hidden, args.inter, args.model_dim = hidden, inter, model_dim
+    args.num_experts, args.global_num_experts = e, global_num_experts
+    args.hidden_states, args.w1, args.w2 = x.data_ptr(), w1.data_ptr(), w2.data_ptr()
+    if w1_scale is not None:
+        w1_scale, w2_scale = _aligned(w1_scale), _aligned(w2_scale)
+        args.w1_scale, args.w2_scale = w1_scale.data_ptr(), w2_scale.data_ptr()
+    if fp4:
+        for name, t, n in (("w1_global_scale", w1_global_scale, e), ("w2_global_scale", w2_global_scale, e),
+                           ("a1_global_scale", a1_global_scale, 1), ("a2_global_scale", a2_global_scale, 1)):
+            t = check_global_scale(name, t, fmt, n, dev)
+            keep.append(t)
+            setattr(args, name, _cabi.ptr(t))
+    args.expert_map = _cabi.ptr(expert_map)
+    args.activation, args.act_alpha, args.act_limit = act, alpha, limit
+    args.routed_scaling_factor = 1.0 if routed_scaling_factor is None else float(routed_scaling_factor)
+    args.out = out.data_ptr()
+    args.status = ops.device_status(dev).data_ptr()
+    lib = _cabi.load()
+    need = lib.bolt_moe_decode_workspace_bytes(args)
+    if need == 0:
+        _cabi.check(1)
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    args.workspace, args.workspace_bytes = workspace.data_ptr(), need
+    with _cabi.on_device(dev):
+        _cabi.check(lib.bolt_moe_decode(args, _cabi.stream_of(x)))
+    ops._count(2)
+    return out
+
+
+def fused_experts_decode(
+    hidden_states: torch.Tensor,
+    w1: torch.Tensor,
+    w2: torch.Tensor,
+    topk_weights: torch.Tensor,
+    topk_ids: torch.Tensor,
+    *,
+    activation: Optional[str] = None,
+    use_fp8_w8a8: bool = False,
+    use_int8_w8a8: bool = False,
+    use_fp4_w4a4: bool = False,
+    per_channel_quant: bool = False,
+    block_shape: Optional[List[int]] = None,
+    w1_scale: Optional[torch.Tensor] = None,
+    w2_scale: Optional[torch.Tensor] = None,
+    w1_global_scale: Optional[torch.Tensor] = None,
+    w2_global_scale: Optional[torch.Tensor] = None,
+    a1_global_scale: Optional[torch.Tensor] = None,
+    a2_global_scale: Optional[torch.Tensor] = None,
+    global_num_experts: int = -1,
+    expert_map: Optional[torch.Tensor] = None,
+    routed_scaling_factor: Optional[float] = 1.0,
+    gemm1_alpha: Optional[float] = None,
+    gemm1_limit: Optional[float] = None,
+    activation_situ_beta: Optional[float] = None,
+    activation_situ_linear_beta: Optional[float] = None,
+    output_dtype: Optional[torch.dtype] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``fused_experts`` for 1 to 32 tokens in two kernels; arguments as there.
+
+    ``use_fp4_w4a4``: weights and scales as ``fused_experts_fp4`` takes them.  Routes whose id is out of
+    range or not local under ``expert_map`` add nothing; a token with none gives zeros; an expert
+    that a token names twice counts with the sum of its weights.  ``out``: a contiguous buffer for
+    the result.  Raises ``NotImplementedError`` above 32 tokens and for sizes that are not multiples of
+    8 (16-bit), 16 (per-channel), 64 (nvfp4) or 128 (block-scaled, mxfp4)."""
+    return _decode(hidden_states, w1, w2, topk_weights, topk_ids, None, 0, False, True,
+                   use_fp8_w8a8=use_fp8_w8a8, use_int8_w8a8=use_int8_w8a8, use_fp4_w4a4=use_fp4_w4a4,
+                   per_channel_quant=per_channel_quant, block_shape=block_shape, w1_scale=w1_scale,
+                   w2_scale=w2_scale, w1_global_scale=w1_global_scale, w2_global_scale=w2_global_scale,
+                   a1_global_scale=a1_global_scale, a2_global_scale=a2_global_scale,
+                   activation=activation, gemm1_alpha=gemm1_alpha, gemm1_limit=gemm1_limit,
+                   activation_situ_beta=activation_situ_beta,
+                   activation_situ_linear_beta=activation_situ_linear_beta,
+                   global_num_experts=global_num_experts, expert_map=expert_map,
+                   routed_scaling_factor=routed_scaling_factor, output_dtype=output_dtype, out=out)
+
+
+def fused_moe_decode(
+    hidden_states: torch.Tensor,
+    gating_output: torch.Tensor,
+    w1: torch.Tensor,
+    w2: torch.Tensor,
+    topk: int,
+    renormalize: bool,
+    is_softmax: bool = True,
+    *,
+    activation: Optional[str] = None,
+    use_fp8_w8a8: bool = False,
+    use_int8_w8a8: bool = False,
+    use_fp4_w4a4: bool = False,
+    per_channel_quant: bool = False,
+    block_shape: Optional[List[int]] = None,
+    w1_scale: Optional[torch.Tensor] = None,
+    w2_scale: Optional[torch.Tensor] = None,
+    w1_global_scale: Optional[torch.Tensor] = None,
+    w2_global_scale: Optional[torch.Tensor] = None,
+    a1_global_scale: Optional[torch.Tensor] = None,
+    a2_global_scale: Optional[torch.Tensor] = None,
+    global_num_experts: int = -1,
+    expert_map: Optional[torch.Tensor] = None,
+    routed_scaling_factor: Optional[float] = 1.0,
+    gemm1_alpha: Optional[float] = None,
+    gemm1_limit: Optional[float] = None,
+    activation_situ_beta: Optional[float] = None,
+    activation_situ_linear_beta: Optional[float] = None,
+    output_dtype: Optional[torch.dtype] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``fused_experts_decode`` from the router's logits [tokens, experts]: the top-k choice of
+    ``routing.fused_topk`` (the same one, to the last bit) is made inside the layer's kernels."""
+    return _decode(hidden_states, w1, w2, None, None, gating_output, topk, renormalize, is_softmax,
+                   use_fp8_w8a8=use_fp8_w8a8, use_int8_w8a8=use_int8_w8a8, use_fp4_w4a4=use_fp4_w4a4,
+                   per_channel_quant=per_channel_quant, block_shape=block_shape, w1_scale=w1_scale,
+                   w2_scale=w2_scale, w1_global_scale=w1_global_scale, w2_global_scale=w2_global_scale,
+                   a1_global_scale=a1_global_scale, a2_global_scale=a2_global_scale,
+                   activation=activation, gemm1_alpha=gemm1_alpha, gemm1_limit=gemm1_limit,
+                   activation_situ_beta=activation_situ_beta,
+                   activation_situ_linear_beta=activation_situ_linear_beta,
+                   global_num_experts=global_num_experts, expert_map=expert_map,
+                   routed_scaling_factor=routed_scaling_factor, output_dtype=output_dtype, out=out)
+
+
+__all__ = ["fused_experts_decode", "fused_moe_decode"]

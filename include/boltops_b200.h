@@ -583,6 +583,78 @@ int bolt_moe_layer_kernel_count(const bolt_layer_args* args);
 size_t bolt_moe_layer_workspace_bytes(const bolt_layer_args* args);
 int bolt_moe_layer(const bolt_layer_args* args, void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* microscaled 4-bit floating point                                            */
+/* ------------------------------------------------------------------------- */
+/* e2m1 codes, two to a byte (the first value in the low bits), blocks along the last dimension:
+ *   NV: 16 values, E4M3 scale byte s = e4m3(min(amax / 6, 448)), value code * s * global_scale;
+ *       values are multiplied with the rounded 1 / global_scale before they are quantised
+ *   MX: 32 values, E8M0 scale byte: the smallest 2^(byte - 127) >= amax / 6 (byte 0 for a block of
+ *       zeros), value code * 2^(byte - 127)
+ * Nearest code, ties to even.  A block that holds a NaN or an infinity gets the NaN scale byte (0x7F,
+ * 0xFF) and codes 0. */
+enum bolt_fp4_format { BOLT_FP4_NV = 0, BOLT_FP4_MX = 1 };
+
+/* x [rows, cols] bf16 / f16 / fp32, dense, 16-byte aligned; cols whole blocks; global_scale optional
+ * (NV; one fp32 value on the device); codes [rows, cols / 2], scales [rows, cols / block] bytes. */
+int bolt_fp4_quant(const void* x, int dtype, int64_t rows, int64_t cols, int format,
+                   const float* global_scale, void* codes, void* scales, void* stream);
+int bolt_fp4_dequant(const void* codes, const void* scales, int64_t rows, int64_t cols, int format,
+                     const float* global_scale, void* out, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* a whole layer for a few tokens                                             */
+/* ------------------------------------------------------------------------- */
+/* storage of the experts' weights and what is multiplied with them */
+enum bolt_decode_kind {
+  BOLT_DECODE_BF16 = 0,
+  BOLT_DECODE_F16 = 1,
+  BOLT_DECODE_FP8_BLOCK = 2,     /* the w8a8 recipes of bolt_moe_layer                        */
+  BOLT_DECODE_INT8_CHANNEL = 3,
+  BOLT_DECODE_FP8_CHANNEL = 4,
+  BOLT_DECODE_INT8_BLOCK = 5,
+  BOLT_DECODE_NVFP4 = 6,         /* e2m1 codes, an E4M3 scale per 16 values, w4a4             */
+  BOLT_DECODE_MXFP4 = 7          /* e2m1 codes, an E8M0 scale per 32 values, w4a4             */
+};
+
+typedef struct bolt_decode_args {
+  int kind;                    /* enum bolt_decode_kind                                       */
+  int x_dtype, out_dtype;      /* 16-bit rows (of the weights' type when these are 16-bit); any float */
+  int num_tokens, topk;        /* 0 to 32, 1 to 32                                            */
+  int hidden, inter, model_dim;
+  int num_experts;             /* experts whose weights are here (at most 1024)               */
+  int global_num_experts;      /* range of topk_ids; number of logits                         */
+  const void* hidden_states;   /* [num_tokens, hidden]                                        */
+  const void* w1;              /* [num_experts, 2 inter, hidden]: gate rows, then up rows     */
+  const void* w2;              /* [num_experts, model_dim, inter]                             */
+  const void* w1_scale;        /* fp32 as in bolt_layer_args; 4-bit: scale bytes per block    */
+  const void* w2_scale;
+  const float* w1_global_scale; /* 4-bit kinds, each optional: [num_experts] on the weights,  */
+  const float* w2_global_scale; /*   [1] on the activations before their blocks' scales       */
+  const float* a1_global_scale;
+  const float* a2_global_scale;
+  const float* topk_weights;   /* [num_tokens, topk], or null with gating                     */
+  const int32_t* topk_ids;     /* [num_tokens, topk]; ids out of range or not local are skipped */
+  const void* gating;          /* optional [num_tokens, global_num_experts] logits: routed as by */
+  int gating_dtype;            /*   bolt_fused_topk (bf16, f16 or fp32)                       */
+  int renormalize, is_softmax;
+  const int32_t* expert_map;   /* optional [global_num_experts]: local expert or -1           */
+  int activation;              /* enum bolt_activation, gated, [gate | up] layout             */
+  float act_alpha, act_limit;
+  float routed_scaling_factor;
+  void* out;                   /* [num_tokens, model_dim] in out_dtype; zeros for a token     */
+                               /*   without a local expert                                    */
+  void* workspace;             /* contents do not matter; one call at a time                  */
+  size_t workspace_bytes;
+  int32_t* status;             /* optional, as in bolt_gemm_args; 30: a weight copy did not land */
+  int sm_count;                /* blocks to launch; 0: one per SM                             */
+} bolt_decode_args;
+
+/* Two kernels on the stream (no sort, no copies of rows).  Sizes: hidden and inter multiples of 8
+ * (16-bit), 16 (per-channel), 128 (block-scaled, MX) or 64 (NV); block-scaled model_dim a multiple of 128. */
+size_t bolt_moe_decode_workspace_bytes(const bolt_decode_args* args);
+int bolt_moe_decode(const bolt_decode_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
