@@ -52,6 +52,8 @@ struct Params {
   float* act_amax;          // [slots][units of an expert] (per-channel kinds)
   int32_t* status;
   int slots_per_warp;
+  int amax_cols;            // units of an expert in the first kernel
+  int unit;                 // columns (first kernel) or rows (second) of a unit
 };
 
 // ---------------------------------------------------------------------------
@@ -68,7 +70,7 @@ struct Routes {
   int touched;
 };
 __host__ __device__ inline int route_bytes(int experts, int routes) {
-  return 4 * (3 * experts + 4 * routes) + 128;
+  return 4 * (3 * experts + 4 * routes) + 64;
 }
 
 template <int NPL>
@@ -93,7 +95,9 @@ __device__ __forceinline__ int local_expert(const Params& p, int id) {
   return e >= 0 && e < p.experts ? e : -1;
 }
 
+template <int kWarps>
 __device__ void build_routes(const Params& p, Routes& r, uint8_t* mem) {
+  constexpr int kThreads = 32 * kWarps;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int routes = p.tokens * p.topk, experts = p.experts;
   r.mask = reinterpret_cast<uint32_t*>(mem);
@@ -103,7 +107,7 @@ __device__ void build_routes(const Params& p, Routes& r, uint8_t* mem) {
   r.token = reinterpret_cast<int*>(r.coef + routes);
   r.ids = r.token + routes;
   r.wts = reinterpret_cast<float*>(r.ids + routes);
-  int* totals = reinterpret_cast<int*>(r.wts + routes);   // [8] per warp
+  int* totals = reinterpret_cast<int*>(r.wts + routes);   // [16] per warp
   for (int e = tid; e < experts; e += kThreads) r.mask[e] = 0;
   if (p.gating != nullptr) {
     const int size = p.gating_dtype == BOLT_F32 ? 4 : 2;
@@ -186,10 +190,11 @@ __device__ __forceinline__ int slot_of(uint32_t mask, int off, int token) {
 // ---------------------------------------------------------------------------
 struct Ring {
   uint32_t base, bars;
-  int slots, bytes;
+  int slots, bytes, bytes_in;      // a slot's size, and what a copy brings
   int s_in = 0, s_out = 0;
   uint32_t ph = 0;
-  __device__ void init(uint32_t smem, uint32_t bar, int n, int box_bytes) {
+  __device__ void init(uint32_t smem, uint32_t bar, int n, int box_bytes, int copy_bytes) {
+    bytes_in = copy_bytes;
     base = smem;
     bars = bar;
     slots = n;
@@ -199,7 +204,7 @@ struct Ring {
   __device__ __forceinline__ uint32_t next_in(uint32_t& dst) {
     const uint32_t bar = bars + 8 * s_in;
     dst = base + s_in * bytes;
-    mbar_expect_tx(bar, bytes);
+    mbar_expect_tx(bar, bytes_in);
     if (++s_in == slots) s_in = 0;
     return bar;
   }
@@ -217,14 +222,16 @@ struct Ring {
 };
 
 constexpr int kCtrlBytes = 1024;   // barriers and the abort flag
-constexpr int kMaxSlots = 14;      // 8 warps x 14 barriers x 8 bytes < 1024
+constexpr int kMaxBarriers = 126;  // 8 bytes each
 
 __device__ __forceinline__ uint8_t* carve(uint8_t* raw) {
   return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
 }
 
 // What both kernels begin with: barriers, the ring.
-__device__ __forceinline__ volatile int* start(Ring& ring, uint8_t* smem, int slots, int box_bytes) {
+template <int kWarps>
+__device__ __forceinline__ volatile int* start(Ring& ring, uint8_t* smem, int slots, int box_bytes,
+                                               int bytes_in) {
   const int warp = threadIdx.x >> 5;
   uint8_t* ctrl = smem + kWarps * slots * box_bytes;
   const uint32_t bars = smem_u32(ctrl);
@@ -233,7 +240,7 @@ __device__ __forceinline__ volatile int* start(Ring& ring, uint8_t* smem, int sl
   if (threadIdx.x == 0) *abort_flag = 0;
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   __syncthreads();
-  ring.init(smem_u32(smem) + warp * slots * box_bytes, bars + 8 * warp * slots, slots, box_bytes);
+  ring.init(smem_u32(smem) + warp * slots * box_bytes, bars + 8 * warp * slots, slots, box_bytes, bytes_in);
   return abort_flag;
 }
 // A wait that ran out leaves copies in flight: give them time to land before the block's memory
@@ -257,7 +264,7 @@ __device__ __forceinline__ void put_sums(float* red, const float (&acc)[MT][NT][
     }
 }
 // Sum over the warps of element (row half r, row g of tile mt, token n).
-template <int MT, int NT>
+template <int kWarps, int MT, int NT>
 __device__ __forceinline__ float get_sum(const float* red, int mt, int r, int g, int n) {
   const int at = ((mt * NT + (n >> 3)) * 4 + 2 * r + (n & 1)) * 32 + 4 * g + ((n & 7) >> 1);
   float v = 0.f;
@@ -266,33 +273,44 @@ __device__ __forceinline__ float get_sum(const float* red, int mt, int r, int g,
   return v;
 }
 
-constexpr int unit_cols(int k) { return k == K_MX4 ? 32 : 16; }
-constexpr int up_box_bytes(int k) { return 2 * unit_cols(k) * 128; }
-constexpr int kDownRows = 16;
-constexpr int kDownBoxBytes = kDownRows * 128;
-// (above: registers would be spilled)
-constexpr int blocks_per_sm(int k, int nt) { return nt == 1 || (nt == 2 && k != K_MX4) ? 2 : 1; }
-constexpr int red_bytes(int mt, int nt) { return kWarps * mt * nt * 128 * 4; }
+// Boxes hold up to 32 weight rows (64 for MX's gate and up rows: a block of 32 columns is quantised
+// at once).  Sixteen warps an SM hide the latencies of a box that eight do not, as far as registers
+// allow: the sums of 32 tokens, and MX with its scales apart, need more than 128.
+constexpr int kMaxRows = 32;
+constexpr int up_tiles(int k) { return k == K_MX4 ? 4 : 2; }
+constexpr int up_box_bytes(int k) { return up_tiles(k) * 2048; }
+constexpr int kDownTiles = kMaxRows / 16;
+constexpr int kDownBoxBytes = kMaxRows * 128;
+constexpr int warps_of(int k, int nt) { return nt == 4 || k == K_MX4 ? 8 : 16; }
+constexpr int red_bytes(int warps, int mt, int nt) { return warps * mt * nt * 128 * 4; }
+// 8-bit kinds, up to eight tokens: the rows' codes are made once and kept
+constexpr bool keeps_codes(int k, int nt) { return is8(k) && nt == 1; }
+// bytes of a kept row of codes: 16 more than it has, so that eight rows lie in different banks
+__host__ __device__ constexpr int code_pitch(int k, int n) { return (int)row_bytes(k, n) + 16; }
 
 // ---------------------------------------------------------------------------
 // gate and up projections, activation
 // ---------------------------------------------------------------------------
 template <int K, int NT>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(K, NT))
+__global__ void __launch_bounds__(32 * warps_of(K, NT), 1)
 k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
-  constexpr int UC = unit_cols(K), MT = UC / 8, kBox = up_box_bytes(K);
+  constexpr int MT = up_tiles(K), kBox = up_box_bytes(K), kWarps = warps_of(K, NT), kThreads = 32 * kWarps;
+  constexpr int kCols = 8 * MT;       // columns a unit may have
+  const int UC = is4(K) ? kCols : p.unit;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = carve(raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   Ring ring;
-  volatile int* abort_flag = start(ring, smem, p.slots_per_warp, kBox);
+  volatile int* abort_flag = start<kWarps>(ring, smem, p.slots_per_warp, kBox, 2 * UC * 128);
   uint8_t* rest = smem + kWarps * p.slots_per_warp * kBox + kCtrlBytes;
   float* red = reinterpret_cast<float*>(rest);
-  rest += red_bytes(MT, NT);
+  rest += red_bytes(kWarps, MT, NT);
+  uint8_t* stage = rest + warp * code_bytes(NT);
+  if (is8(K) && !keeps_codes(K, NT)) rest += kWarps * code_bytes(NT);
   let_next_start();
 
   Routes r;
-  build_routes(p, r, rest);
+  build_routes<kWarps>(p, r, rest);
   rest += (route_bytes(p.experts, p.tokens * p.topk) + 15) & ~15;
 
   const int per_expert = (p.inter + UC - 1) / UC;
@@ -303,26 +321,44 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
   const int n_it = boxes > warp ? (int)((boxes - warp + kWarps - 1) / kWarps) : 0;
 
   // boxes of this block's units in order, every eighth this warp's
-  int in_u = u0, in_kb = warp, in_it = 0;
-  auto bring = [&]() {
-    while (in_kb >= nb) {
-      in_kb -= nb;
-      ++in_u;
+  struct Place {
+    int u, a, c, kb;      // unit: list[a], columns from c * UC; box of the reduction
+  };
+  auto settle = [&](Place& q) {
+    while (q.kb >= nb) {
+      q.kb -= nb;
+      ++q.u;
+      if (++q.c == per_expert) {
+        q.c = 0;
+        ++q.a;
+      }
     }
+  };
+  Place in = {u0, u0 / per_expert, u0 % per_expert, warp}, cur = in;
+  if (n_it > 0) {
+    settle(in);
+    cur = in;
+  }
+  int in_it = 0;
+  auto bring = [&]() {
+    settle(in);
     if (lane == 0) {
       uint32_t dst;
       const uint32_t bar = ring.next_in(dst);
-      tma_load_4d(dst, &map, bar, in_kb * 128, (in_u % per_expert) * UC, 0, r.list[in_u / per_expert]);
+      tma_load_4d(dst, &map, bar, in.kb * 128, in.c * UC, 0, r.list[in.a]);
     }
-    in_kb += kWarps;
+    in.kb += kWarps;
     ++in_it;
   };
   for (int i = 0; i < p.slots_per_warp && in_it < n_it; ++i) bring();
 
   // ---- Q1 that needs whole rows, once per block while the first boxes travel ----
   float* row_scale = reinterpret_cast<float*>(rest);       // [tokens][2]: scale, reciprocal
-  uint8_t* x_codes = rest;                                 // [tokens][hidden / 2], scales behind them
-  uint8_t* x_sf = x_codes + (int64_t)p.tokens * (p.hidden / 2);
+  if (is_channel(K)) rest += (8 * p.tokens + 15) & ~15;
+  uint8_t* x_codes = rest;                                 // [tokens][pitch], scales behind them
+  const int pitch = code_pitch(K, p.hidden);
+  uint8_t* x_sf = x_codes + p.tokens * pitch;              // 4-bit: bytes
+  float* x_scale = reinterpret_cast<float*>(x_sf);         // block-scaled: [hidden / 128][8]
   constexpr int kBlk = K == K_NV4 ? 16 : 32;
   const int sf_row = p.hidden / kBlk;
   if constexpr (is_channel(K)) {
@@ -347,14 +383,34 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
       if (lane == 0) scale8<K>(amax, row_scale[2 * m], row_scale[2 * m + 1]);
     }
     __syncthreads();
-  } else if constexpr (is4(K)) {
+  }
+  if constexpr (keeps_codes(K, NT)) {
+    // a warp per group of 128 values
+    const int per_row = (p.hidden + 127) / 128;
+    for (int i = warp; i < p.tokens * per_row; i += kWarps) {
+      const int m = i / per_row, kb = i - m * per_row, c = kb * 128 + 4 * lane;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c < p.hidden) v = load_values4(static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden, p.x_dtype, c);
+      float scale, inv;
+      if constexpr (is_block(K)) {
+        const float top = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+        scale8<K>(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))), scale, inv);
+        if (lane == 0) x_scale[kb * 8 + m] = scale;
+      } else {
+        inv = row_scale[2 * m + 1];
+      }
+      if (c < p.hidden) *reinterpret_cast<uint32_t*>(x_codes + m * pitch + c) = codes4<K>(v, inv);
+    }
+    __syncthreads();
+  }
+  if constexpr (is4(K)) {
     const bool nv = K == K_NV4;
     const float inv_g = p.a1 != nullptr ? __frcp_rn(*p.a1) : 1.f;
     const int per_row = p.hidden / 32;
     for (int i = tid; i < p.tokens * per_row; i += kThreads) {
       const int m = i / per_row, c = (i - m * per_row) * 32;
       float v[32];
-      load_values32(v, static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden, p.x_dtype, p.hidden, c);
+      load_values32(v, static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden, p.x_dtype, c);
       if (nv && p.a1 != nullptr) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] *= inv_g;
@@ -372,21 +428,16 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
           w[b * (kBlk / 8) + j] = fp4::codes8<K == K_NV4>(v + b * kBlk + 8 * j, sc);
         x_sf[(int64_t)m * sf_row + c / kBlk + b] = (uint8_t)byte;
       }
-      *reinterpret_cast<uint4*>(x_codes + (int64_t)m * (p.hidden / 2) + c / 2) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(x_codes + m * pitch + c / 2) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     __syncthreads();
   }
 
-  int it = 0, kb = warp, ku = u0;   // the box this warp computes next
-  while (kb >= nb) {
-    kb -= nb;
-    ++ku;
-  }
-  const int64_t sf1_row = p.hidden / kBlk;
-  auto row_scales = [&](RowScales<K>(&ws)[MT], int u, int box) {
+  const int sf1_row = p.hidden / kBlk;
+  auto row_scales = [&](RowScales<K>(&ws)[MT], const Place& q) {
+    const int64_t e = r.list[q.a];
+    const int c0 = q.c * UC;
     if constexpr (is4(K)) {
-      const int64_t e = r.list[u / per_expert];
-      const int c0 = (u % per_expert) * UC;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -394,17 +445,27 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
           load_block_scales<K>(ws[mt].sf[h],
                                static_cast<const uint8_t*>(p.s1) +
                                    ((e * 2 + h) * p.inter + c0 + 8 * mt + g) * sf1_row,
-                               (int)sf1_row, box, t);
+                               sf1_row, q.kb, t);
+    } else if constexpr (is_block(K)) {
+      const uint32_t* s1 = static_cast<const uint32_t*>(p.s1) + e * (2 * p.inter / 128) * (p.hidden / 128) + q.kb;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)     // (columns past the unit's are scaled by anything)
+          ws[mt].sf[h][0] = s1[((h * p.inter + min(c0 + 8 * mt + g, p.inter - 1)) / 128) * (p.hidden / 128)];
     }
   };
   RowScales<K> ws[MT], ws_next[MT];
-  if (it < n_it) row_scales(ws_next, ku, kb);
+  int it = 0;
+  if (n_it > 0) row_scales(ws_next, cur);
+  Place unit = {u0, u0 / per_expert, u0 % per_expert, 0};
 
-  for (int u = u0; u < u1; ++u) {
-    const int e = r.list[u / per_expert], c0 = (u % per_expert) * UC;
+  for (; unit.u < u1; unit.kb = nb, settle(unit)) {
+    const int e = r.list[unit.a], c0 = unit.c * UC;
     const uint32_t mask = r.mask[e];
     const int off = r.off[e], cnt = __popc(mask);
     const unsigned live = (1u << ((cnt + 7) / 8)) - 1u;
+    const uint32_t live_cols = cnt == 32 ? ~0u : (1u << cnt) - 1u;
     float acc[MT][NT][4];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -416,63 +477,56 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) tok[nt] = 8 * nt + g < cnt ? r.token[off + 8 * nt + g] : -1;
 
-    while (it < n_it && ku == u) {
+    // tokens of columns 2 t and 2 t + 1 (of one that has none: any)
+    const int tok0 = r.token[off + min(2 * t, cnt - 1)], tok1 = r.token[off + min(2 * t + 1, cnt - 1)];
+
+    while (it < n_it && cur.u == unit.u) {
       // next box's scales travel while this one is computed
-      int nkb = kb + kWarps, nu = ku;
-      while (nkb >= nb) {
-        nkb -= nb;
-        ++nu;
-      }
+      Place nxt = cur;
+      nxt.kb += kWarps;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) ws[mt] = ws_next[mt];
-      if (it + 1 < n_it) row_scales(ws_next, nu, nkb);
+      if (it + 1 < n_it) {
+        settle(nxt);
+        row_scales(ws_next, nxt);
+      }
+      const int kb = cur.kb;
 
       TokenBox<K> x[NT];
-      float xs[NT];
+      float xs = 1.f;
+      if constexpr (keeps_codes(K, NT)) {
+        load_token<K>(x[0], tok[0] < 0 ? nullptr : x_codes + tok[0] * pitch, p.hidden, kb, t);
+      } else if constexpr (is8(K)) {
+        xs = quant_box<K, NT>(
+            x, stage, live_cols, p.x_dtype, p.hidden, kb * 128, lane,
+            [&](int c) { return static_cast<const uint16_t*>(p.x) + (int64_t)r.token[off + c] * p.hidden; },
+            [&](int c) { return row_scale[2 * r.token[off + c] + 1]; });
+      } else {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (!((live >> nt) & 1u)) continue;
-        const int m = tok[nt];
-        if constexpr (is16(K)) {
-          load_token<K>(x[nt], m < 0 ? nullptr : static_cast<const uint8_t*>(p.x) + (int64_t)m * p.hidden * 2,
-                        p.hidden * 2, kb, t);
-        } else if constexpr (is8(K)) {
-          float v[32];
-          load_values32(v, m < 0 ? nullptr : static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden,
-                        p.x_dtype, p.hidden, kb * 128 + 32 * t);
-          float inv;
-          if constexpr (is_block(K)) {
-            float amax = 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) amax = fmaxf(amax, fabsf(v[j]));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            scale8<K>(amax, xs[nt], inv);
+        for (int nt = 0; nt < NT; ++nt) {
+          if (!((live >> nt) & 1u)) continue;
+          const int m = tok[nt];
+          if constexpr (is16(K)) {
+            load_token<K>(x[nt], m < 0 ? nullptr : static_cast<const uint8_t*>(p.x) + (int64_t)m * p.hidden * 2,
+                          p.hidden * 2, kb, t);
           } else {
-            inv = m < 0 ? 0.f : row_scale[2 * m + 1];
-          }
-          codes32<K>(v, inv, x[nt].w);
-        } else {
-          load_token<K>(x[nt], m < 0 ? nullptr : x_codes + (int64_t)m * (p.hidden / 2), p.hidden / 2, kb, t);
-          if constexpr (K == K_NV4) {
-            load_block_scales<K>(x[nt].sf, m < 0 ? nullptr : x_sf + (int64_t)m * sf_row, sf_row, kb, t);
-          } else {
+            load_token<K>(x[nt], m < 0 ? nullptr : x_codes + m * pitch, p.hidden / 2, kb, t);
+            if constexpr (K == K_NV4) {
+              load_block_scales<K>(x[nt].sf, m < 0 ? nullptr : x_sf + (int64_t)m * sf_row, sf_row, kb, t);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int col = 8 * nt + 2 * t + i;
-              load_block_scales<K>(x[nt].sf + 2 * i,
-                                   col < cnt ? x_sf + (int64_t)r.token[off + col] * sf_row : nullptr,
-                                   sf_row, kb, t);
+              for (int i = 0; i < 2; ++i) {
+                const int col = 8 * nt + 2 * t + i;
+                load_block_scales<K>(x[nt].sf + 2 * i,
+                                     col < cnt ? x_sf + (int64_t)r.token[off + col] * sf_row : nullptr,
+                                     sf_row, kb, t);
+              }
             }
           }
         }
       }
       const uint32_t box = ring.wait(abort_flag, p.status);
       if constexpr (is_block(K)) {
-        const float* s1 = static_cast<const float*>(p.s1);
-        const int blocks_n = 2 * p.inter / 128, blocks_k = p.hidden / 128;
-        const float sg = s1[((int64_t)e * blocks_n + c0 / 128) * blocks_k + kb];
-        const float su = s1[((int64_t)e * blocks_n + (p.inter + c0) / 128) * blocks_k + kb];
         float part[MT][NT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -480,14 +534,21 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) part[mt][nt][i] = 0.f;
-        box_mma<K, MT, NT, true>(box, lane, x, ws, live, part);
+        box_mma<K, MT, NT, true>(box, UC, lane, x, ws, live, part);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           if (!((live >> nt) & 1u)) continue;
-          const float x0 = __shfl_sync(0xffffffffu, xs[nt], 8 * t);
-          const float x1 = __shfl_sync(0xffffffffu, xs[nt], 8 * t + 4);
+          float x0, x1;
+          if constexpr (keeps_codes(K, NT)) {
+            x0 = x_scale[kb * 8 + tok0];
+            x1 = x_scale[kb * 8 + tok1];
+          } else {
+            x0 = __shfl_sync(0xffffffffu, xs, 8 * nt + 2 * t);
+            x1 = __shfl_sync(0xffffffffu, xs, 8 * nt + 2 * t + 1);
+          }
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
+            const float sg = __uint_as_float(ws[mt].sf[0][0]), su = __uint_as_float(ws[mt].sf[1][0]);
             acc[mt][nt][0] = fmaf(part[mt][nt][0], x0 * sg, acc[mt][nt][0]);
             acc[mt][nt][1] = fmaf(part[mt][nt][1], x1 * sg, acc[mt][nt][1]);
             acc[mt][nt][2] = fmaf(part[mt][nt][2], x0 * su, acc[mt][nt][2]);
@@ -495,27 +556,26 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
           }
         }
       } else {
-        box_mma<K, MT, NT, true>(box, lane, x, ws, live, acc);
+        box_mma<K, MT, NT, true>(box, UC, lane, x, ws, live, acc);
       }
       ring.release();
       if (in_it < n_it) bring();
-      kb = nkb;
-      ku = nu;
+      cur = nxt;
       ++it;
     }
 
     // ---- sums over the warps, activation, Q2 of the 4-bit kinds ----
     put_sums<MT, NT>(red, acc, warp, lane, live);
     __syncthreads();
-    const int all = ((cnt * UC + 31) / 32) * 32;      // whole warps take part in the exchanges
+    const int all = ((cnt * kCols + 31) / 32) * 32;      // whole warps take part in the exchanges
     for (int i = tid; i < all; i += kThreads) {
-      const int n = i / UC, c = i % UC, col = c0 + c;
-      const bool have = n < cnt && col < p.inter;
+      const int n = i / kCols, c = i % kCols, col = c0 + c;
+      const bool have = n < cnt && c < UC && col < p.inter;
       const int slot = off + n;
       float a = 0.f;
       if (have) {
-        float gate = get_sum<MT, NT>(red, c >> 3, 0, c & 7, n);
-        float up = get_sum<MT, NT>(red, c >> 3, 1, c & 7, n);
+        float gate = get_sum<kWarps, MT, NT>(red, c >> 3, 0, c & 7, n);
+        float up = get_sum<kWarps, MT, NT>(red, c >> 3, 1, c & 7, n);
         if constexpr (is_channel(K)) {
           const float* s1 = static_cast<const float*>(p.s1) + (int64_t)e * 2 * p.inter;
           const float xsc = row_scale[2 * r.token[slot]];
@@ -539,15 +599,15 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
         if constexpr (is_channel(K)) {
           float amax = fabsf(a);
 #pragma unroll
-          for (int o = UC / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-          if (c == 0 && n < cnt) p.act_amax[(int64_t)slot * per_expert + u % per_expert] = amax;
+          for (int o = kCols / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+          if (c == 0 && n < cnt) p.act_amax[(int64_t)slot * per_expert + unit.c] = amax;
         }
       } else {
-        // UC columns of one slot are one block
+        // a unit's columns of one slot are one block
         if (K == K_NV4 && p.a2 != nullptr) a *= __frcp_rn(*p.a2);
         float amax = fabsf(a);
 #pragma unroll
-        for (int o = UC / 2; o > 0; o >>= 1) amax = fp4::amax_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        for (int o = kCols / 2; o > 0; o >>= 1) amax = fp4::amax_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         const uint32_t byte = fp4::scale_byte<K == K_NV4>(amax);
         const fp4::Scaler sc = fp4::scaler_of<K == K_NV4>(byte);
         const float q = sc.r == 0.f ? 0.f : fp4::quotient<K == K_NV4>(a, sc);
@@ -566,23 +626,26 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
 // down projection, sum over a token's experts
 // ---------------------------------------------------------------------------
 template <int K, int NT>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(K, NT))
+__global__ void __launch_bounds__(32 * warps_of(K, NT), 1)
 k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
-  constexpr int kBox = kDownBoxBytes;
+  constexpr int MT = kDownTiles, kBox = kDownBoxBytes, kWarps = warps_of(K, NT), kThreads = 32 * kWarps;
+  const int UR = p.unit;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = carve(raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   Ring ring;
-  volatile int* abort_flag = start(ring, smem, p.slots_per_warp, kBox);
+  volatile int* abort_flag = start<kWarps>(ring, smem, p.slots_per_warp, kBox, UR * 128);
   uint8_t* rest = smem + kWarps * p.slots_per_warp * kBox + kCtrlBytes;
   float* red = reinterpret_cast<float*>(rest);
-  rest += red_bytes(1, NT);
+  rest += red_bytes(kWarps, MT, NT);
+  uint8_t* stage = rest + warp * code_bytes(NT);
+  if (is8(K)) rest += kWarps * code_bytes(NT);
 
   Routes r;
-  build_routes(p, r, rest);
+  build_routes<kWarps>(p, r, rest);
   rest += (route_bytes(p.experts, p.tokens * p.topk) + 15) & ~15;
 
-  const int units = (p.model_dim + kDownRows - 1) / kDownRows;
+  const int units = (p.model_dim + UR - 1) / UR;
   const int u0 = (int)((int64_t)units * blockIdx.x / gridDim.x);
   const int u1 = (int)((int64_t)units * (blockIdx.x + 1) / gridDim.x);
   const int nb = (int)((row_bytes(K, p.inter) + 127) / 128);
@@ -609,7 +672,7 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
     if (lane == 0) {
       uint32_t dst;
       const uint32_t bar = ring.next_in(dst);
-      tma_load_3d(dst, &map, bar, in.kb * 128, in.u * kDownRows, r.list[in.a]);
+      tma_load_3d(dst, &map, bar, in.kb * 128, in.u * UR, r.list[in.a]);
     }
     in.kb += kWarps;
     ++in_it;
@@ -620,28 +683,32 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
   const int sf_row = p.inter / kBlk;
   Place cur = {u0, 0, warp};
   if (n_it > 0) settle(cur);
-  auto row_scales = [&](RowScales<K>& ws, const Place& q) {
-    if constexpr (is4(K)) {
-      const int64_t e = r.list[q.a];
+  auto row_scales = [&](RowScales<K>(&ws)[MT], const Place& q) {
+    const int64_t e = r.list[q.a];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int row = q.u * kDownRows + 8 * h + g;
-        load_block_scales<K>(ws.sf[h],
-                             row < p.model_dim
-                                 ? static_cast<const uint8_t*>(p.s2) + (e * p.model_dim + row) * sf_row
-                                 : nullptr,
-                             sf_row, q.kb, t);
+        // (rows past the unit's are scaled by anything: they go nowhere)
+        const int row = min(q.u * UR + 16 * mt + 8 * h + g, p.model_dim - 1);
+        if constexpr (is4(K))
+          load_block_scales<K>(ws[mt].sf[h], static_cast<const uint8_t*>(p.s2) + (e * p.model_dim + row) * sf_row,
+                               sf_row, q.kb, t);
+        else if constexpr (is_block(K))
+          ws[mt].sf[h][0] = static_cast<const uint32_t*>(
+              p.s2)[(e * (p.model_dim / 128) + row / 128) * (p.inter / 128) + q.kb];
+        else if constexpr (is_channel(K))
+          ws[mt].sf[h][0] = static_cast<const uint32_t*>(p.s2)[e * p.model_dim + row];
       }
-    }
   };
-  RowScales<K> ws[1], ws_next;
+  RowScales<K> ws[MT], ws_next[MT];
   int it = 0;
   if (n_it > 0) row_scales(ws_next, cur);
 
   wait_for_previous();     // the activations
   float* row_scale = reinterpret_cast<float*>(rest);       // [slots][2]
   if constexpr (is_channel(K)) {
-    const int per_expert = (p.inter + unit_cols(K) - 1) / unit_cols(K);
+    const int per_expert = p.amax_cols;
     int slots = 0;
     if (r.touched > 0) {
       const int last = r.list[r.touched - 1];
@@ -657,18 +724,23 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
   }
 
   for (int u = u0; u < u1; ++u) {
-    float acc[1][NT][4];
+    float acc[MT][NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[0][nt][i] = 0.f;
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[mt][nt][i] = 0.f;
 
     while (it < n_it && cur.u == u) {
       Place nxt = cur;
       nxt.kb += kWarps;
-      settle(nxt);
-      ws[0] = ws_next;
-      if (it + 1 < n_it) row_scales(ws_next, nxt);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) ws[mt] = ws_next[mt];
+      if (it + 1 < n_it) {
+        settle(nxt);
+        row_scales(ws_next, nxt);
+      }
 
       const int e = r.list[cur.a], kb = cur.kb;
       const uint32_t mask = r.mask[e];
@@ -678,78 +750,67 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
       for (int nt = 0; nt < NT; ++nt) live |= ((mask >> (8 * nt)) & 0xFFu) != 0u ? 1u << nt : 0u;
 
       TokenBox<K> x[NT];
-      float xs[NT];
+      float xs = 1.f;
+      if constexpr (is8(K)) {
+        xs = quant_box<K, NT>(
+            x, stage, mask, BOLT_F32, p.inter, kb * 128, lane,
+            [&](int c) {
+              return reinterpret_cast<const float*>(p.act_rows) + (int64_t)slot_of(mask, off, c) * p.inter;
+            },
+            [&](int c) { return row_scale[2 * slot_of(mask, off, c) + 1]; });
+      } else {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (!((live >> nt) & 1u)) continue;
-        const int slot = slot_of(mask, off, 8 * nt + g);
-        if constexpr (is16(K)) {
-          load_token<K>(x[nt], slot < 0 ? nullptr : p.act_rows + (int64_t)slot * p.inter * 2, p.inter * 2, kb, t);
-        } else if constexpr (is8(K)) {
-          float v[32];
-          load_values32(v, slot < 0 ? nullptr : reinterpret_cast<const float*>(p.act_rows) + (int64_t)slot * p.inter,
-                        BOLT_F32, p.inter, kb * 128 + 32 * t);
-          float inv;
-          if constexpr (is_block(K)) {
-            float amax = 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) amax = fmaxf(amax, fabsf(v[j]));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            scale8<K>(amax, xs[nt], inv);
+        for (int nt = 0; nt < NT; ++nt) {
+          if (!((live >> nt) & 1u)) continue;
+          const int slot = slot_of(mask, off, 8 * nt + g);
+          if constexpr (is16(K)) {
+            load_token<K>(x[nt], slot < 0 ? nullptr : p.act_rows + (int64_t)slot * p.inter * 2, p.inter * 2, kb, t);
           } else {
-            inv = slot < 0 ? 0.f : row_scale[2 * slot + 1];
-          }
-          codes32<K>(v, inv, x[nt].w);
-        } else {
-          load_token<K>(x[nt], slot < 0 ? nullptr : p.act_rows + (int64_t)slot * (p.inter / 2), p.inter / 2, kb, t);
-          if constexpr (K == K_NV4) {
-            load_block_scales<K>(x[nt].sf, slot < 0 ? nullptr : p.act_sf + (int64_t)slot * sf_row, sf_row, kb, t);
-          } else {
+            load_token<K>(x[nt], slot < 0 ? nullptr : p.act_rows + (int64_t)slot * (p.inter / 2), p.inter / 2, kb, t);
+            if constexpr (K == K_NV4) {
+              load_block_scales<K>(x[nt].sf, slot < 0 ? nullptr : p.act_sf + (int64_t)slot * sf_row, sf_row, kb, t);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int s = slot_of(mask, off, 8 * nt + 2 * t + i);
-              load_block_scales<K>(x[nt].sf + 2 * i, s < 0 ? nullptr : p.act_sf + (int64_t)s * sf_row, sf_row, kb, t);
+              for (int i = 0; i < 2; ++i) {
+                const int s = slot_of(mask, off, 8 * nt + 2 * t + i);
+                load_block_scales<K>(x[nt].sf + 2 * i, s < 0 ? nullptr : p.act_sf + (int64_t)s * sf_row, sf_row, kb, t);
+              }
             }
           }
         }
       }
-      float wr0 = 1.f, wr1 = 1.f;     // scale of weight rows g and g + 8
-      if constexpr (is_block(K)) {
-        wr0 = wr1 = static_cast<const float*>(p.s2)[((int64_t)e * (p.model_dim / 128) + u * kDownRows / 128) *
-                                                        (p.inter / 128) + kb];
-      } else if constexpr (is_channel(K)) {
-        const float* s2 = static_cast<const float*>(p.s2) + (int64_t)e * p.model_dim;
-        const int row = u * kDownRows + g;
-        wr0 = row < p.model_dim ? s2[row] : 0.f;
-        wr1 = row + 8 < p.model_dim ? s2[row + 8] : 0.f;
-      } else if constexpr (is4(K)) {
-        wr0 = wr1 = (p.g2 != nullptr ? p.g2[e] : 1.f) * (p.a2 != nullptr ? *p.a2 : 1.f);
-      }
+      const float whole = is4(K) ? (p.g2 != nullptr ? p.g2[e] : 1.f) * (p.a2 != nullptr ? *p.a2 : 1.f) : 1.f;
       const uint32_t box = ring.wait(abort_flag, p.status);
-      float part[1][NT][4];
+      float part[MT][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) part[0][nt][i] = 0.f;
-      box_mma<K, 1, NT, false>(box, lane, x, ws, live, part);
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) part[mt][nt][i] = 0.f;
+      box_mma<K, MT, NT, false>(box, 0, lane, x, ws, live, part);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         if (!((live >> nt) & 1u)) continue;
         float s01[2] = {1.f, 1.f};
         if constexpr (is_block(K)) {
-          s01[0] = __shfl_sync(0xffffffffu, xs[nt], 8 * t);
-          s01[1] = __shfl_sync(0xffffffffu, xs[nt], 8 * t + 4);
+          s01[0] = __shfl_sync(0xffffffffu, xs, 8 * nt + 2 * t);
+          s01[1] = __shfl_sync(0xffffffffu, xs, 8 * nt + 2 * t + 1);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           // tokens that did not choose the expert get nothing (not even a NaN of its weights)
           const int slot = slot_of(mask, off, 8 * nt + 2 * t + i);
           if (slot < 0) continue;
-          float f = r.coef[slot] * s01[i];
+          float f = r.coef[slot] * s01[i] * whole;
           if constexpr (is_channel(K)) f *= row_scale[2 * slot];
-          acc[0][nt][i] = fmaf(part[0][nt][i], f * wr0, acc[0][nt][i]);
-          acc[0][nt][2 + i] = fmaf(part[0][nt][2 + i], f * wr1, acc[0][nt][2 + i]);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const float f0 = is8(K) ? f * __uint_as_float(ws[mt].sf[0][0]) : f;
+            const float f1 = is8(K) ? f * __uint_as_float(ws[mt].sf[1][0]) : f;
+            acc[mt][nt][i] = fmaf(part[mt][nt][i], f0, acc[mt][nt][i]);
+            acc[mt][nt][2 + i] = fmaf(part[mt][nt][2 + i], f1, acc[mt][nt][2 + i]);
+          }
         }
       }
       ring.release();
@@ -758,12 +819,12 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
       ++it;
     }
 
-    put_sums<1, NT>(red, acc, warp, lane, ~0u);
+    put_sums<MT, NT>(red, acc, warp, lane, ~0u);
     __syncthreads();
-    for (int i = tid; i < p.tokens * kDownRows; i += kThreads) {
-      const int n = i / kDownRows, c = i % kDownRows, col = u * kDownRows + c;
-      if (col >= p.model_dim) continue;
-      const float v = get_sum<1, NT>(red, 0, c >> 3, c & 7, n) * p.out_scale;
+    for (int i = tid; i < p.tokens * kMaxRows; i += kThreads) {
+      const int n = i / kMaxRows, c = i % kMaxRows, col = u * UR + c;
+      if (c >= UR || col >= p.model_dim) continue;
+      const float v = get_sum<kWarps, MT, NT>(red, c >> 4, (c >> 3) & 1, c & 7, n) * p.out_scale;
       const int64_t at = (int64_t)n * p.model_dim + col;
       if (p.out_dtype == BOLT_BF16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
       else if (p.out_dtype == BOLT_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
@@ -815,57 +876,99 @@ int encode(CUtensorMap* map, const void* base, int dims, const cuuint64_t* size,
 inline size_t a256(size_t n) { return (n + 255) & ~size_t(255); }
 inline int a16(int n) { return (n + 15) & ~15; }
 
+constexpr int kMinUnit = 8;
+// Size of a unit, of 8 to `most`: every block gets the same number of units but for one, so the one that
+// makes the largest share smallest (of two alike the larger; a unit costs about a row's time by itself).
+int unit_size(int total, int most, int64_t copies, int blocks) {
+  int best = most;
+  int64_t least = INT64_MAX;
+  for (int u = most; u >= kMinUnit; --u) {
+    const int64_t units = copies * ((total + u - 1) / u);
+    const int64_t share = (units + blocks - 1) / blocks * (u + 1);
+    if (share < least) {
+      least = share;
+      best = u;
+    }
+  }
+  return best;
+}
+
 // bytes of the three parts of the workspace
 void workspace_parts(const bolt_decode_args* a, size_t (&part)[3]) {
   const size_t slots = (size_t)a->num_tokens * a->topk;
   const int k = a->kind;
   part[0] = a256(slots * (is8(k) ? 4 * (size_t)a->inter : (size_t)row_bytes(k, a->inter)));
   part[1] = is4(k) ? a256(slots * (a->inter / (k == K_NV4 ? 16 : 32))) : 0;
-  part[2] = is_channel(k) ? a256(slots * ((a->inter + 15) / 16) * 4) : 0;
+  part[2] = is_channel(k) ? a256(slots * ((a->inter + kMinUnit - 1) / kMinUnit) * 4) : 0;
 }
 
-// Shared memory left over by the fixed parts goes to the rings.  Two blocks of 113 KB share an SM, so
-// that the second kernel's can come in beside the first's; where a ring would then hold less than
-// three boxes a warp (long 4-bit rows of many tokens, the sums of more than 16), one block takes all.
-constexpr int kHalfSm = 113 * 1024, kWholeSm = 226 * 1024;
-int ring_slots(int fixed, int box_bytes, int* total) {
-  int slots = (kHalfSm - fixed) / (kWarps * box_bytes);
-  if (slots < 3) slots = (kWholeSm - fixed) / (kWarps * box_bytes);
-  if (slots > kMaxSlots) slots = kMaxSlots;
-  *total = fixed + slots * kWarps * box_bytes;
-  return slots;
+constexpr int kSmem = 226 * 1024;   // of a block
+int ring_slots(int fixed, int box_bytes, int warps) {
+  int slots = (kSmem - fixed) / (warps * box_bytes);
+  return slots * warps > kMaxBarriers ? kMaxBarriers / warps : slots;
+}
+template <int K, int NT>
+int up_fixed_bytes(const Params& p) {
+  int n = 1024 + kCtrlBytes + red_bytes(warps_of(K, NT), up_tiles(K), NT) +
+          a16(route_bytes(p.experts, p.tokens * p.topk));
+  if (is_channel(K)) n += a16(8 * p.tokens);
+  if (is4(K)) n += p.tokens * (code_pitch(K, p.hidden) + p.hidden / (K == K_NV4 ? 16 : 32));
+  else if (keeps_codes(K, NT)) n += p.tokens * code_pitch(K, p.hidden) + (is_block(K) ? p.hidden / 128 * 32 : 0);
+  else if (is8(K)) n += warps_of(K, NT) * code_bytes(NT);
+  return n;
 }
 
 template <int K, int NT>
-int launch(const bolt_decode_args* a, const CUtensorMap& m1, const CUtensorMap& m2, Params p, cudaStream_t st) {
-  static std::atomic<bool> ready[2][kMaxDevices];
-  int rc = configure_kernel(k_few_up<K, NT>, kWholeSm, ready[0], 0, 0, 0, 0);
-  if (rc == BOLT_OK) rc = configure_kernel(k_few_down<K, NT>, kWholeSm, ready[1], 0, 0, 0, 0);
-  if (rc != BOLT_OK) return rc;
-  const int routes = a16(route_bytes(p.experts, p.tokens * p.topk));
-  int up = 1024 + kCtrlBytes + red_bytes(unit_cols(K) / 8, NT) + routes;
-  int down = 1024 + kCtrlBytes + red_bytes(1, NT) + routes;
-  if (is_channel(K)) {
-    up += 8 * p.tokens;
-    down += 8 * p.tokens * p.topk;
-  }
-  if (is4(K)) up += p.tokens * (p.hidden / 2 + p.hidden / (K == K_NV4 ? 16 : 32));
-  int up_bytes, down_bytes;
-  const int up_slots = ring_slots(up, up_box_bytes(K), &up_bytes);
-  const int down_slots = ring_slots(down, kDownBoxBytes, &down_bytes);
-  if (up_slots < 2 || down_slots < 2) {
-    set_error("moe_decode: %d tokens x hidden size %d do not fit in shared memory", p.tokens, p.hidden);
+int launch(const bolt_decode_args* a, Params p, cudaStream_t st) {
+  constexpr int kWarps = warps_of(K, NT);
+  const int up = up_fixed_bytes<K, NT>(p);
+  const int up_slots = ring_slots(up, up_box_bytes(K), kWarps);
+  if constexpr (NT < 4)     // kept codes that leave no room: the form for more tokens keeps none
+    if (up_slots < 1 && keeps_codes(K, NT)) return launch<K, 2 * NT>(a, p, st);
+  int down = 1024 + kCtrlBytes + red_bytes(kWarps, kDownTiles, NT) + a16(route_bytes(p.experts, p.tokens * p.topk));
+  if (is8(K)) down += kWarps * code_bytes(NT);
+  if (is_channel(K)) down += 8 * p.tokens * p.topk;
+  const int down_slots = ring_slots(down, kDownBoxBytes, kWarps);
+  if (up_slots < 1 || down_slots < 1) {
+    set_error("moe_decode: %d tokens of hidden size %d do not fit in shared memory", p.tokens, p.hidden);
     return BOLT_ERR_UNSUPPORTED;
   }
+  static std::atomic<bool> ready[2][kMaxDevices];
+  int rc = configure_kernel(k_few_up<K, NT>, kSmem, ready[0], 0, 0, 0, 0);
+  if (rc == BOLT_OK) rc = configure_kernel(k_few_down<K, NT>, kSmem, ready[1], 0, 0, 0, 0);
+  if (rc != BOLT_OK) return rc;
+
   const int sms = a->sm_count > 0 ? a->sm_count : sm_count_of_current_device();
+  const int64_t routes = (int64_t)p.tokens * p.topk;
+  const int columns = is4(K) ? 8 * up_tiles(K)
+                             : unit_size(p.inter, 8 * up_tiles(K), routes < p.experts ? routes : p.experts, sms);
+  const int rows = unit_size(p.model_dim, kMaxRows, 1, sms);
+  CUtensorMap m1, m2;
+  {
+    const cuuint64_t kb = (cuuint64_t)row_bytes(K, p.hidden), i = p.inter;
+    const cuuint64_t size[4] = {kb, i, 2, (cuuint64_t)p.experts};
+    const cuuint64_t strides[3] = {kb, kb * i, 2 * kb * i};
+    const cuuint32_t box[4] = {128, (cuuint32_t)columns, 2, 1};
+    if ((rc = encode(&m1, a->w1, 4, size, strides, box)) != BOLT_OK) return rc;
+  }
+  {
+    const cuuint64_t kb = (cuuint64_t)row_bytes(K, p.inter), n = p.model_dim;
+    const cuuint64_t size[3] = {kb, n, (cuuint64_t)p.experts};
+    const cuuint64_t strides[2] = {kb, kb * n};
+    const cuuint32_t box[3] = {128, (cuuint32_t)rows, 1};
+    if ((rc = encode(&m2, a->w2, 3, size, strides, box)) != BOLT_OK) return rc;
+  }
+  p.amax_cols = (p.inter + columns - 1) / columns;
   p.slots_per_warp = up_slots;
-  k_few_up<K, NT><<<sms, kThreads, up_bytes, st>>>(m1, p);
+  p.unit = columns;
+  k_few_up<K, NT><<<sms, 32 * kWarps, up + up_slots * kWarps * up_box_bytes(K), st>>>(m1, p);
   BOLT_LAUNCH_CHECK();
   p.slots_per_warp = down_slots;
+  p.unit = rows;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(sms);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = down_bytes;
+  cfg.blockDim = dim3(32 * kWarps);
+  cfg.dynamicSmemBytes = down + down_slots * kWarps * kDownBoxBytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -877,11 +980,10 @@ int launch(const bolt_decode_args* a, const CUtensorMap& m1, const CUtensorMap& 
 }
 
 template <int K>
-int launch_kind(const bolt_decode_args* a, const CUtensorMap& m1, const CUtensorMap& m2, const Params& p,
-                cudaStream_t st) {
-  if (p.tokens <= 8) return launch<K, 1>(a, m1, m2, p, st);
-  if (p.tokens <= 16) return launch<K, 2>(a, m1, m2, p, st);
-  return launch<K, 4>(a, m1, m2, p, st);
+int launch_kind(const bolt_decode_args* a, const Params& p, cudaStream_t st) {
+  if (p.tokens <= 8) return launch<K, 1>(a, p, st);
+  if (p.tokens <= 16) return launch<K, 2>(a, p, st);
+  return launch<K, 4>(a, p, st);
 }
 
 int check_args(const bolt_decode_args* a) {
@@ -976,30 +1078,15 @@ extern "C" int bolt_moe_decode(const bolt_decode_args* a, void* stream) {
   p.act_amax = reinterpret_cast<float*>(p.act_sf + part[1]);
   p.status = a->status;
 
-  CUtensorMap m1, m2;
-  {
-    const cuuint64_t kb = (cuuint64_t)row_bytes(k, a->hidden), i = a->inter;
-    const cuuint64_t size[4] = {kb, i, 2, (cuuint64_t)a->num_experts};
-    const cuuint64_t strides[3] = {kb, kb * i, 2 * kb * i};
-    const cuuint32_t box[4] = {128, (cuuint32_t)unit_cols(k), 2, 1};
-    if ((rc = encode(&m1, a->w1, 4, size, strides, box)) != BOLT_OK) return rc;
-  }
-  {
-    const cuuint64_t kb = (cuuint64_t)row_bytes(k, a->inter), n = a->model_dim;
-    const cuuint64_t size[3] = {kb, n, (cuuint64_t)a->num_experts};
-    const cuuint64_t strides[2] = {kb, kb * n};
-    const cuuint32_t box[3] = {128, kDownRows, 1};
-    if ((rc = encode(&m2, a->w2, 3, size, strides, box)) != BOLT_OK) return rc;
-  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (k) {
-    case K_BF16: return launch_kind<K_BF16>(a, m1, m2, p, st);
-    case K_F16: return launch_kind<K_F16>(a, m1, m2, p, st);
-    case K_F8_BLOCK: return launch_kind<K_F8_BLOCK>(a, m1, m2, p, st);
-    case K_I8_CHANNEL: return launch_kind<K_I8_CHANNEL>(a, m1, m2, p, st);
-    case K_F8_CHANNEL: return launch_kind<K_F8_CHANNEL>(a, m1, m2, p, st);
-    case K_I8_BLOCK: return launch_kind<K_I8_BLOCK>(a, m1, m2, p, st);
-    case K_NV4: return launch_kind<K_NV4>(a, m1, m2, p, st);
-    default: return launch_kind<K_MX4>(a, m1, m2, p, st);
+    case K_BF16: return launch_kind<K_BF16>(a, p, st);
+    case K_F16: return launch_kind<K_F16>(a, p, st);
+    case K_F8_BLOCK: return launch_kind<K_F8_BLOCK>(a, p, st);
+    case K_I8_CHANNEL: return launch_kind<K_I8_CHANNEL>(a, p, st);
+    case K_F8_CHANNEL: return launch_kind<K_F8_CHANNEL>(a, p, st);
+    case K_I8_BLOCK: return launch_kind<K_I8_BLOCK>(a, p, st);
+    case K_NV4: return launch_kind<K_NV4>(a, p, st);
+    default: return launch_kind<K_MX4>(a, p, st);
   }
 }

@@ -5,7 +5,7 @@
 // HBM, and what matters is that every SM always has enough bytes in flight and spends few
 // instructions per byte:
 //
-// * Each of a block's eight warps owns a ring of shared-memory slots and fills it itself with bulk
+// * Each warp owns a ring of shared-memory slots and fills it itself with bulk
 //   tensor copies of (rows x 128 bytes) boxes; no warp waits for another inside a reduction.  The
 //   warps share out the boxes of a unit (a few weight rows over the whole reduction) and add up
 //   their accumulators through shared memory once per unit.
@@ -27,8 +27,6 @@ namespace bolt {
 namespace few {
 using namespace tc;
 
-constexpr int kWarps = 8;
-constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxTokens = 32;
 
 // values of enum bolt_decode_kind
@@ -128,37 +126,39 @@ struct TokenBox {
   uint32_t w[8];
   uint32_t sf[is4(K) ? (K == K_MX4 ? 4 : 1) : 1];
 };
-// Scales of 4-bit weight rows g and g + 8 of a tile (NV: of the lane's 64 values; MX: of the box).
+// Scales of weight rows g and g + 8 of a tile: the bytes of 4-bit kinds (NV: of the lane's 64 values,
+// MX: of the box), the bits of the box's fp32 scale of block-scaled ones.
 template <int K>
 struct RowScales {
-  uint32_t sf[2][is4(K) ? (K == K_MX4 ? 2 : 1) : 1];
+  uint32_t sf[2][K == K_MX4 ? 2 : 1];
 };
 
-// d[tile][token tile] += (box of weights) . (tokens).  The box: rows of 128 bytes, swizzled.  Tile
-// mt holds the box's rows 8 mt + g and 8 MT + 8 mt + g (UP: a gate row with its up row) or
-// 16 mt + g and 16 mt + 8 + g.  Only the token tiles of `live` are computed.
+// d[tile][token tile] += (box of weights) . (tokens).  The box: rows of 128 bytes, swizzled (16-byte
+// chunk c of row r at chunk c ^ (r % 8)).  Tile mt holds the box's rows 8 mt + g and second + 8 mt + g
+// (UP: gate rows with their up rows) or 16 mt + g and 16 mt + 8 + g; rows that the box does not fill
+// give sums that nobody reads.  Only the token tiles of `live` are computed.
 template <int K, int MT, int NT, bool UP>
-__device__ __forceinline__ void box_mma(uint32_t box, int lane, const TokenBox<K> (&x)[NT],
+__device__ __forceinline__ void box_mma(uint32_t box, int second, int lane, const TokenBox<K> (&x)[NT],
                                         const RowScales<K> (&ws)[MT], unsigned live,
                                         float (&d)[MT][NT][4]) {
   const int g = lane >> 2, t = lane & 3;
-  uint32_t row[MT][2];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    row[mt][0] = box + (uint32_t)((UP ? 8 * mt : 16 * mt) + g) * 128u;
-    row[mt][1] = box + (uint32_t)((UP ? 8 * MT + 8 * mt : 16 * mt + 8) + g) * 128u;
-  }
+  // (the rows of a thread lie 8 apart, so one place in the swizzle serves them all; up rows have
+  // their own)
+  const uint32_t row0 = box + (uint32_t)g * 128u;
+  const uint32_t row1 = UP ? box + (uint32_t)(second + g) * 128u : row0 + 1024u;
+  const int ph0 = g, ph1 = UP ? (second + g) & 7 : g;
+  auto row = [&](int mt, int r) { return (r ? row1 : row0) + (UP ? 1024u : 2048u) * mt; };
   if constexpr (K == K_MX4) {
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
-      const uint32_t at = (uint32_t)((c ^ g) << 4) + 4u * t;
+      const uint32_t at[2] = {(uint32_t)((c ^ ph0) << 4) + 4u * t, (uint32_t)((c ^ ph1) << 4) + 4u * t};
       uint32_t a[MT][2][4];
       float sw[MT][2];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          fp4::halves8(lds32(row[mt][r] + at), a[mt][r]);
+          fp4::halves8(lds32(row(mt, r) + at[r]), a[mt][r]);
           sw[mt][r] = fp4::e8m0_to_f32((ws[mt].sf[r][c >> 2] >> (8 * (c & 3))) & 0xFFu);
         }
 #pragma unroll
@@ -184,13 +184,13 @@ __device__ __forceinline__ void box_mma(uint32_t box, int lane, const TokenBox<K
   } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t at = (uint32_t)(((2 * t + h) ^ g) << 4);
+      const uint32_t at[2] = {(uint32_t)(((2 * t + h) ^ ph0) << 4), (uint32_t)(((2 * t + h) ^ ph1) << 4)};
       uint32_t a[MT][2][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint4 v = lds128(row[mt][r] + at);
+          const uint4 v = lds128(row(mt, r) + at[r]);
           a[mt][r][0] = v.x;
           a[mt][r][1] = v.y;
           a[mt][r][2] = v.z;
@@ -300,68 +300,96 @@ __device__ __forceinline__ void load_block_scales(uint32_t* sf, const uint8_t* r
   }
 }
 
-// 32 values -> 32 8-bit codes, the arithmetic of the row quantisers (quant.cu).
+// A box's 128 values of every live token, quantised by the whole warp: a lane takes four consecutive
+// values of a token, one warp-wide maximum gives its scale, and the codes go through shared memory
+// to the lanes that multiply them.  (A lane that quantised its own 32 bytes of its own column would
+// spend eight times the instructions where one column of eight is live, the usual case.)
 template <int K>
-__device__ __forceinline__ void codes32(const float (&v)[32], float inv, uint32_t (&w)[8]) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float* q = v + 4 * j;
-    if (is_i8(K)) {
-      w[j] = ((uint32_t)(uint8_t)f32_to_i8(q[0] * inv)) | ((uint32_t)(uint8_t)f32_to_i8(q[1] * inv) << 8) |
-             ((uint32_t)(uint8_t)f32_to_i8(q[2] * inv) << 16) |
-             ((uint32_t)(uint8_t)f32_to_i8(q[3] * inv) << 24);
-    } else {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(q[0] * inv, q[1] * inv), __NV_SATFINITE,
-                                                   __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(q[2] * inv, q[3] * inv), __NV_SATFINITE,
-                                                   __NV_E4M3);
-      w[j] = lo | (hi << 16);
-    }
-  }
+__device__ __forceinline__ uint32_t codes4(const float4& v, float inv) {
+  if (is_i8(K))
+    return ((uint32_t)(uint8_t)f32_to_i8(v.x * inv)) | ((uint32_t)(uint8_t)f32_to_i8(v.y * inv) << 8) |
+           ((uint32_t)(uint8_t)f32_to_i8(v.z * inv) << 16) | ((uint32_t)(uint8_t)f32_to_i8(v.w * inv) << 24);
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v.x * inv, v.y * inv), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v.z * inv, v.w * inv), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
 }
+// scale and reciprocal of a row or group, the arithmetic of the row quantisers (quant.cu)
 template <int K>
 __device__ __forceinline__ void scale8(float amax, float& scale, float& inv) {
   scale = __fdiv_rn(fmaxf(amax, 1.0e-10f), is_i8(K) ? 127.0f : 448.0f);
   inv = __frcp_rn(scale);
 }
 
-// 32 consecutive values of a row as floats; dt BOLT_BF16 / BOLT_F16 / BOLT_F32.  Chunks of 16 that
-// begin at or after `cols` are zeros.
-__device__ __forceinline__ void load_values32(float (&v)[32], const void* row, int dt, int cols, int at) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int c = at + 16 * h;
-    const bool ok = row != nullptr && c < cols;
-    if (dt == BOLT_F32) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (ok) f = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + c + 4 * i);
-        v[16 * h + 4 * i] = f.x;
-        v[16 * h + 4 * i + 1] = f.y;
-        v[16 * h + 4 * i + 2] = f.z;
-        v[16 * h + 4 * i + 3] = f.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint4 u = make_uint4(0u, 0u, 0u, 0u);
-        if (ok) u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + c + 8 * i);
-        const uint32_t q[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float2 f;
-          if (dt == BOLT_BF16) {
-            f.x = __uint_as_float(q[j] << 16);
-            f.y = __uint_as_float(q[j] & 0xFFFF0000u);
-          } else {
-            f = __half22float2(*reinterpret_cast<const __half2*>(&q[j]));
-          }
-          v[16 * h + 8 * i + 2 * j] = f.x;
-          v[16 * h + 8 * i + 2 * j + 1] = f.y;
-        }
-      }
+// four consecutive values of a row as floats; dt BOLT_BF16 / BOLT_F16 / BOLT_F32
+__device__ __forceinline__ float4 load_values4(const void* row, int dt, int at) {
+  if (dt == BOLT_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(row) + at);
+  const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(row) + at);
+  if (dt == BOLT_BF16)
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u),
+                       __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u));
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+
+constexpr int kCodePitch = 144;     // bytes between columns: 16-byte reads without bank conflicts
+constexpr int code_bytes(int nt) { return 8 * nt * kCodePitch; }
+
+// `stage`: code_bytes(NT) of the warp's own shared memory.  `row_of(column)`: a live column's values;
+// `live_cols`: bit per column; `inv_of(column)`: per-channel kinds, the reciprocal scale of its row.
+// Returns in lane c the scale of column c's group (block-scaled kinds).
+template <int K, int NT, typename RowOf, typename InvOf>
+__device__ __forceinline__ float quant_box(TokenBox<K> (&x)[NT], uint8_t* stage, uint32_t live_cols, int dt,
+                                           int cols, int at, int lane, RowOf row_of, InvOf inv_of) {
+  const int g = lane >> 2, t = lane & 3, c0 = at + 4 * lane;
+  const bool in = c0 < cols;          // (cols is a multiple of 16)
+  float my_scale = 1.f, my_inv = 1.f;
+  float4 kept = make_float4(0.f, 0.f, 0.f, 0.f);      // the first token's values (often the only one)
+  if constexpr (is_block(K)) {
+    uint32_t my_amax = 0;
+    for (uint32_t left = live_cols; left != 0; left &= left - 1) {
+      const int c = __ffs(left) - 1;
+      const float4 v = load_values4(row_of(c), dt, c0);
+      if (left == live_cols) kept = v;
+      // (non-negative floats order like their bits; fmaxf passes NaNs over)
+      const float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+      if (lane == c) my_amax = top;
     }
+    scale8<K>(__uint_as_float(my_amax), my_scale, my_inv);
+  }
+  __syncwarp();                       // the box before has been read
+  for (uint32_t left = live_cols; left != 0; left &= left - 1) {
+    const int c = __ffs(left) - 1;
+    float4 v = kept;
+    if (in && !(is_block(K) && left == live_cols)) v = load_values4(row_of(c), dt, c0);
+    const float inv = is_block(K) ? __shfl_sync(0xffffffffu, my_inv, c) : inv_of(c);
+    *reinterpret_cast<uint32_t*>(stage + c * kCodePitch + 4 * lane) = codes4<K>(v, inv);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int c = 8 * nt + g;
+    uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
+    if ((live_cols >> c) & 1u) {
+      a = *reinterpret_cast<const uint4*>(stage + c * kCodePitch + 32 * t);
+      b = *reinterpret_cast<const uint4*>(stage + c * kCodePitch + 32 * t + 16);
+    }
+    x[nt].w[0] = a.x; x[nt].w[1] = a.y; x[nt].w[2] = a.z; x[nt].w[3] = a.w;
+    x[nt].w[4] = b.x; x[nt].w[5] = b.y; x[nt].w[6] = b.z; x[nt].w[7] = b.w;
+  }
+  return my_scale;
+}
+
+// 32 consecutive values of a 16-bit row as floats (the block quantiser of 4-bit rows)
+__device__ __forceinline__ void load_values32(float (&v)[32], const uint16_t* row, int dt, int at) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float4 f = load_values4(row, dt, at + 4 * i);
+    v[4 * i] = f.x;
+    v[4 * i + 1] = f.y;
+    v[4 * i + 2] = f.z;
+    v[4 * i + 3] = f.w;
   }
 }
 

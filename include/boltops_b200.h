@@ -647,7 +647,7 @@ typedef struct bolt_decode_args {
   void* workspace;             /* contents do not matter; one call at a time                  */
   size_t workspace_bytes;
   int32_t* status;             /* optional, as in bolt_gemm_args; 30: a weight copy did not land */
-  int sm_count;                /* blocks to launch; 0: one per SM                             */
+  int sm_count;                /* SMs to use; 0: all                                          */
 } bolt_decode_args;
 
 /* Two kernels on the stream (no sort, no copies of rows).  Sizes: hidden and inter multiples of 8
