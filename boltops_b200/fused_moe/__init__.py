@@ -109,10 +109,12 @@ def moe_activation(
 
 
 from .decode import fused_experts_decode, fused_moe_decode  # noqa: E402
+from .w4a4 import fused_experts_fp4  # noqa: E402
 
 __all__ = [
     "fused_experts",
     "fused_experts_decode",
+    "fused_experts_fp4",
     "fused_moe_decode",
     "normalize_moe_activation",
     "moe_activation_output_size",

@@ -87,11 +87,6 @@ def _numel(shape):
     return n
 
 
-def _aligned(t: torch.Tensor, to: int = 16) -> torch.Tensor:
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % to else t
-
-
 def _decode(hidden_states, w1, w2, topk_weights, topk_ids, gating, topk, renormalize, is_softmax, *,
             use_fp8_w8a8, use_int8_w8a8, use_fp4_w4a4, per_channel_quant, block_shape, w1_scale, w2_scale,
             w1_global_scale, w2_global_scale, a1_global_scale, a2_global_scale, activation, gemm1_alpha,
@@ -197,15 +192,15 @@ def _decode(hidden_states, w1, w2, topk_weights, topk_ids, gating, topk, renorma
     if m == 0:
         return out
 
-    x = _aligned(hidden_states)
-    w1, w2 = _aligned(w1), _aligned(w2)
+    x = ops.aligned(hidden_states)
+    w1, w2 = ops.aligned(w1), ops.aligned(w2)
     args.kind, args.x_dtype, args.out_dtype = kind, _cabi.dtype_code(x.dtype), _cabi.dtype_code(out_dtype)
     args.num_tokens, args.topk = m, topk
     args.hidden, args.inter, args.model_dim = hidden, inter, model_dim
     args.num_experts, args.global_num_experts = e, global_num_experts
     args.hidden_states, args.w1, args.w2 = x.data_ptr(), w1.data_ptr(), w2.data_ptr()
     if w1_scale is not None:
-        w1_scale, w2_scale = _aligned(w1_scale), _aligned(w2_scale)
+        w1_scale, w2_scale = ops.aligned(w1_scale), ops.aligned(w2_scale)
         args.w1_scale, args.w2_scale = w1_scale.data_ptr(), w2_scale.data_ptr()
     if fp4:
         for name, t, n in (("w1_global_scale", w1_global_scale, e), ("w2_global_scale", w2_global_scale, e),

@@ -44,6 +44,12 @@ def sort_launches(lib, m: int, topk: int, num_experts: int) -> int:
     return 1 if lib.bolt_moe_sort_workspace_bytes(m, topk, num_experts) <= 16 else 2
 
 
+def aligned(t: torch.Tensor, to: int = 16) -> torch.Tensor:
+    """``t`` contiguous and on a ``to``-byte boundary: itself where it is, else a copy."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % to else t
+
+
 def ceil_to(x: int, m: int) -> int:
     return (x + m - 1) // m * m
 

@@ -1,10 +1,14 @@
-"""Dense block-scaled GEMM on the grouped-GEMM kernel (one "expert").
+"""Dense block-scaled GEMMs.
+
+``gemm_a8w8_blockscale`` and its other names: 8-bit operands, on the grouped-GEMM kernel (one "expert").
 
 Same call surface as the reference's ``gemm_a8w8_blockscale``
 (boltops/gemm/gemm_a8w8_blockscale.py:10-70 in the reference project) and
 ``w8a8_triton_block_scaled_mm`` for the recipe the fused-MoE path uses: e4m3 or int8
 operands, A scales per row and 128 K elements, B scales per 128x128 block.  It is the
 op a DeepSeek-style layer calls next to ``fused_experts`` (shared experts, dense layers).
+
+``gemm_a4w4``: microscaled 4-bit operands (``boltops_b200.fp4``).
 """
 from __future__ import annotations
 
@@ -13,6 +17,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _cabi
+from .fp4 import FORMATS, format_of
 from .fused_moe import ops
 
 
@@ -96,3 +101,60 @@ def w8a8_block_scaled_mm(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, Bs:
 
 w8a8_triton_block_scaled_mm = w8a8_block_scaled_mm
 w8a8_block_int8_matmul = w8a8_block_scaled_mm
+
+
+def gemm_a4w4(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor, w_scale: torch.Tensor,
+              alpha: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = torch.bfloat16,
+              out: Optional[torch.Tensor] = None):
+    """``y[m, n] = alpha * sum_k x[m, k] w[n, k]`` of 4-bit codes with block scales (``fp4.fp4_quant``).
+
+    x [M, K/2] and w [N, K/2] packed codes, x_scale [M, K/block] and w_scale [N, K/block] of one format
+    (float8_e4m3fn: nvfp4, blocks of 16, K a multiple of 64; uint8: mxfp4, blocks of 32, K a multiple
+    of 128); M and N any.  ``alpha``: one fp32 value on the device, the product of both tensors' global
+    scales.  Sums are fp32, rounded once to ``dtype`` (bf16, fp16 or fp32).  All tensors lie on x's
+    device; ``out`` [M, N] has a dense last dimension."""
+    if dtype is None:
+        dtype = torch.bfloat16
+    if not x.is_cuda:
+        raise ValueError("boltops_b200 kernels need CUDA tensors (there is no CPU path)")
+    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"gemm_a4w4 gives bf16, fp16 or fp32, not {dtype}")
+    if x.dtype != torch.uint8 or w.dtype != torch.uint8:
+        raise TypeError("x and w must be packed 4-bit codes (uint8)")
+    fmt = format_of(x_scale)
+    if format_of(w_scale) != fmt:
+        raise TypeError("x and w are of different 4-bit formats")
+    code, block, _ = FORMATS[fmt]
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} and w {tuple(w.shape)} must be [M, K/2] and [N, K/2]")
+    m, n, k = x.shape[0], w.shape[0], 2 * x.shape[1]
+    if tuple(x_scale.shape) != (m, k // block) or tuple(w_scale.shape) != (n, k // block):
+        raise ValueError(f"scale shapes do not match blocks of {block} values")
+    if k == 0 or k % (4 * block):
+        raise NotImplementedError(f"K {k} must be a multiple of {4 * block} ({fmt})")
+    dev = x.device
+    for name, t in (("w", w), ("x_scale", x_scale), ("w_scale", w_scale), ("alpha", alpha), ("out", out)):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, x on {dev}")
+    if alpha is not None and (alpha.numel() != 1 or alpha.dtype != torch.float32):
+        raise ValueError("alpha must be one float32 value")
+    if out is None:
+        out = torch.empty((m, n), dtype=dtype, device=dev)
+    elif tuple(out.shape) != (m, n) or out.dtype != dtype or (n > 1 and out.stride(1) != 1) or \
+            (m > 1 and out.stride(0) < n):
+        raise ValueError(f"out must be [{m}, {n}] in {dtype} with a dense last dimension")
+    if m == 0 or n == 0:
+        return out
+    x, w, x_scale, w_scale = (ops.aligned(t) for t in (x, w, x_scale, w_scale))
+    args = _cabi.Fp4GemmArgs()
+    args.format, args.epilogue = code, _cabi.EPI_STORE
+    args.rows, args.n, args.k, args.num_experts = m, n, k, 1
+    args.a, args.a_scale, args.b, args.b_scale = (t.data_ptr() for t in (x, x_scale, w, w_scale))
+    args.alpha = _cabi.ptr(alpha)
+    args.c, args.c_dtype, args.c_ld = out.data_ptr(), _cabi.dtype_code(dtype), out.stride(0) if m > 1 else n
+    args.status = ops.device_status(dev).data_ptr()
+    args.sm_count = ops.gemm_sm_count(dev)
+    with _cabi.on_device(dev):
+        _cabi.check(_cabi.load().bolt_fp4_gemm(args, _cabi.stream_of(x)))
+    ops._count()
+    return out

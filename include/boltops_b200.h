@@ -602,6 +602,50 @@ int bolt_fp4_quant(const void* x, int dtype, int64_t rows, int64_t cols, int for
 int bolt_fp4_dequant(const void* codes, const void* scales, int64_t rows, int64_t cols, int format,
                      const float* global_scale, void* out, int dtype, void* stream);
 
+/* Products of 4-bit rows with 4-bit weights, both in the same format, scales in the layout that
+ * bolt_fp4_quant writes.
+ *
+ * Dense (sorted_expert_ids null): c[m, n] = f * sum_blocks sa sb (a . b), m < rows, b [n, k / 2].
+ * Grouped: 128-row tiles in the order of bolt_moe_sort_ck; tile i multiplies with expert
+ * sorted_expert_ids[i] of b [num_experts, n, k / 2].  With gather, a and a_scale are in token order
+ * (rows = tokens) and sorted position p reads row sorted_ids[p] & 0xFFFFFF; else they are in sorted
+ * order (rows = capacity).  Results of positions that only pad a tile are not stored (the quantising
+ * epilogue stores zeros).
+ * f = alpha * a_global * b_global[expert] * sorted_weights[position], each optional (null: 1).
+ * BOLT_EPI_STORE: c [rows or capacity, n] in c_dtype, rows c_ld elements apart.
+ * BOLT_EPI_SILU_MUL_QUANT: b's rows are [gate | up]; act(gate, up) in fp32, times 1 / c_global (NV), is
+ * quantised: c [capacity, n / 4] codes, c_scale [capacity, n / 2 / block].  Grouped only.
+ * k: a multiple of 64 (NV) or 128 (MX), n / 2 too with the quantising epilogue.  a, b and their scales
+ * 16-byte aligned. */
+typedef struct bolt_fp4_gemm_args {
+  int format;                  /* enum bolt_fp4_format                                        */
+  int epilogue;                /* BOLT_EPI_STORE or BOLT_EPI_SILU_MUL_QUANT                   */
+  int rows, n, k, num_experts;
+  const void* a;
+  const void* a_scale;
+  const void* b;
+  const void* b_scale;
+  const float* alpha;
+  const float* a_global;
+  const float* b_global;
+  const float* c_global;
+  void* c;
+  int c_dtype;
+  int64_t c_ld;
+  void* c_scale;
+  int capacity, gather, num_tokens;
+  const int32_t* sorted_ids;
+  const float* sorted_weights;
+  const int32_t* sorted_expert_ids;
+  const int32_t* num_valid_ids;
+  int activation;              /* enum bolt_activation, gated                                 */
+  float act_alpha, act_limit;
+  int32_t* status;             /* optional, set to 40 to 43 by a wait that ran out            */
+  int sm_count;                /* blocks to launch; 0: one per SM                             */
+} bolt_fp4_gemm_args;
+
+int bolt_fp4_gemm(const bolt_fp4_gemm_args* args, void* stream);
+
 /* ------------------------------------------------------------------------- */
 /* a whole layer for a few tokens                                             */
 /* ------------------------------------------------------------------------- */
