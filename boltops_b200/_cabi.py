@@ -95,7 +95,7 @@ class Fp4GemmArgs(C.Structure):
     _fields_ = [
         ("format", C.c_int), ("epilogue", C.c_int),
         ("rows", C.c_int), ("n", C.c_int), ("k", C.c_int), ("num_experts", C.c_int),
-        ("a", C.c_void_p), ("a_scale", C.c_void_p), ("b", C.c_void_p), ("b_scale", C.c_void_p),
+        ("a", C.c_void_p), ("a_tiles", C.c_void_p), ("b", C.c_void_p), ("b_tiles", C.c_void_p),
         ("alpha", C.c_void_p), ("a_global", C.c_void_p), ("b_global", C.c_void_p),
         ("c_global", C.c_void_p),
         ("c", C.c_void_p), ("c_dtype", C.c_int), ("c_ld", C.c_int64), ("c_scale", C.c_void_p),
@@ -105,6 +105,18 @@ class Fp4GemmArgs(C.Structure):
         ("activation", C.c_int), ("act_alpha", C.c_float), ("act_limit", C.c_float),
         ("status", C.c_void_p), ("sm_count", C.c_int),
     ]
+
+
+class Fp4TileJob(C.Structure):
+    """struct bolt_fp4_tile_job"""
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("rows", C.c_int), ("row_bytes", C.c_int),
+                ("experts", C.c_int), ("gated_half", C.c_int), ("by_sorted_id", C.c_int)]
+
+
+class Fp4TileArgs(C.Structure):
+    """struct bolt_fp4_tile_args"""
+    _fields_ = [("job", Fp4TileJob * 3), ("jobs", C.c_int), ("num_tokens", C.c_int), ("capacity", C.c_int),
+                ("sorted_ids", C.c_void_p), ("expert_ids", C.c_void_p), ("num_valid_ids", C.c_void_p)]
 
 
 class DecodeArgs(C.Structure):
@@ -214,6 +226,7 @@ _SIGNATURES = {
                                  C.c_void_p, C.c_void_p, C.c_void_p]),
     "bolt_fp4_dequant": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_void_p,
                                    C.c_void_p, C.c_int, C.c_void_p]),
+    "bolt_fp4_tile_scales": (C.c_int, [C.POINTER(Fp4TileArgs), C.c_void_p]),
     "bolt_fp4_gemm": (C.c_int, [C.POINTER(Fp4GemmArgs), C.c_void_p]),
     "bolt_moe_decode_workspace_bytes": (C.c_size_t, [C.POINTER(DecodeArgs)]),
     "bolt_moe_decode": (C.c_int, [C.POINTER(DecodeArgs), C.c_void_p]),

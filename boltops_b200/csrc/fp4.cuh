@@ -1,7 +1,7 @@
 // Microscaled 4-bit floating point: scales of a block, codes of eight values, and back.
 //
 // A code is e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign), two to a byte, the first in the low bits.
-//   NV: blocks of 16, the scale an E4M3 byte: s = e4m3(min(amax / 6, 448)), code = e2m1(v / s)
+//   NV: blocks of 16, the scale an E4M3 byte: s = e4m3(min(amax * (1/6), 448)), code = e2m1(v / s)
 //   MX: blocks of 32, the scale an E8M0 byte: the smallest 2^e with amax <= 6 * 2^e, 0 for a block
 //       of zeros, code = e2m1(v / 2^e)
 // Codes are rounded to the nearest, ties to even, magnitudes above 6 to 6 (only NV has them: its
@@ -29,7 +29,9 @@ template <bool NV>
 __device__ __forceinline__ uint32_t scale_byte(float amax) {
   if (NV) {
     if (!finite_amax(amax)) return 0x7Fu;
-    return __nv_cvt_float_to_fp8(__fdiv_rn(amax, 6.0f), __NV_SATFINITE, __NV_E4M3);
+    // (the product with the rounded 1/6 is exact wherever amax / 6 is the border of two E4M3 values:
+    // 1/6 is rounded by 2^-25 of itself, half a step of any value by more)
+    return __nv_cvt_float_to_fp8(amax * (float)(1.0 / 6.0), __NV_SATFINITE, __NV_E4M3);
   }
   if (!finite_amax(amax)) return 0xFFu;
   const uint32_t bits = __float_as_uint(amax);

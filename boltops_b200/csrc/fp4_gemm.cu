@@ -5,13 +5,15 @@
 // in TMEM over the whole reduction.  A tile is 128 rows x BN weight rows, a K block 256 values: 128
 // bytes of a row, one 128-byte-swizzled box.
 //
-// Warp 0 brings the boxes by TMA, warp 1 issues copies of the scales to TMEM and the instructions, warps
-// 2 and 3 bring the scales (and gathered rows), warps 4 to 11 drain the accumulator.  Scales are
-// read as the quantiser writes them, one line of bytes per row, and go through registers into the
-// instruction's layout (512-byte tiles of 128 rows x 4 scales, byte (r % 32) * 16 + (r / 32) * 4 + i):
-// a thread reads the 32 (NV) or 16 (MX) bytes of a row and two K blocks at once, a whole sector, and 32
-// threads write 128 consecutive bytes of a tile.  So neither weights nor activations need a second
-// layout in memory or a kernel that makes one.
+// The instruction reads scales from TMEM, which takes them from shared memory in 512-byte tiles of 128
+// rows x 4 scales (byte (r % 32) * 16 + (r / 32) * 4 + i).  A small kernel in front, k_tile_scales, lays
+// the scales of rows and weights out like that (an eighth of the codes' bytes); the product then brings
+// them with the operands by bulk copies.  Doing it inside the product, through registers of spare warps,
+// was measured first: the writes have to be made visible to the tensor core's proxy once per K block,
+// and the product ran at 2700 TFLOP/s where it runs at 4000 without any scales (8192 x 7168 x 4096).
+//
+// Warp 0 brings boxes and scales, warp 1 issues the scales' copies to TMEM and the instructions, warps 2
+// and 3 gather rows (expert layers: rows in token order), warps 4 to 11 drain the accumulator.
 #include <cuda.h>
 
 #include <atomic>
@@ -47,7 +49,8 @@ struct Shape {
 };
 
 struct Params {
-  const uint8_t *a, *sfa, *sfb;
+  const uint8_t *a;
+  const uint8_t *sfa, *sfb;              // tiles: [row block][K / 64 or K / 128][512], B per expert
   const float *alpha, *a_global, *b_global, *c_global;
   void* c;
   uint8_t* c_scale;
@@ -55,8 +58,8 @@ struct Params {
   int64_t c_ld;
   int c_vec_ok;
   int rows, n, n_half, k, num_experts, capacity;
-  int num_kb, sf_row;                    // K blocks; scale bytes of a row
-  int sf_vec_ok;                         // scale rows are 16-byte aligned
+  int num_kb, k_tiles;                   // K blocks; scale tiles along K
+  int n_blocks;                          // 128-row blocks of an expert's weights
   int tiles_n, group_m;
   int gather, num_tokens;
   const int32_t *sorted_ids, *expert_ids, *num_valid;
@@ -110,18 +113,6 @@ __device__ __forceinline__ int source_row(const Params& p, int m_blk, int i) {
   }
   return pos < p.rows ? pos : -1;
 }
-// Weight row behind row i of a tile's B operand, or -1.  Gated: 64 gate rows, then the 64 up rows of
-// the same columns, twice.
-template <int BN, bool GATED>
-__device__ __forceinline__ int weight_row(const Params& p, int n_blk, int i) {
-  if (!GATED) {
-    const int r = n_blk * BN + i;
-    return r < p.n ? r : -1;
-  }
-  const int col = n_blk * (BN / 2) + (i >> 7) * 64 + (i & 63);
-  return col < p.n_half ? ((i >> 6) & 1) * p.n_half + col : -1;
-}
-
 template <bool NV, int BN, bool GATED>
 __global__ void __launch_bounds__(kThreads, 1)
 k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const Params p) {
@@ -140,9 +131,9 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    // full: the boxes' bytes (1), the scales (64 threads) and gathered rows (64 more)
+    // full: the bytes of boxes and scales (1), gathered rows (64 threads)
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(bar_full + 8 * s, p.gather ? 129 : 65);
+      mbar_init(bar_full + 8 * s, p.gather ? 65 : 1);
       mbar_init(bar_empty + 8 * s, 1);
     }
     mbar_init(bar_tfull, 1);
@@ -172,11 +163,22 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
       for (int i = blockIdx.x; ok && i < total; i += gridDim.x) {
         const Tile t = tile_of(p, i, num_m);
         if (t.expert < 0) continue;
+        const uint8_t* sfa = p.sfa + (int64_t)t.m * p.k_tiles * 512;
+        const uint8_t* sfb[kNB];       // (a block that does not exist: any, its columns go nowhere)
+#pragma unroll
+        for (int b = 0; b < kNB; ++b)
+          sfb[b] = p.sfb + ((int64_t)t.expert * p.n_blocks + min(t.n * kNB + b, p.n_blocks - 1)) * p.k_tiles * 512;
         for (int kb = 0; kb < p.num_kb; ++kb) {
           ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 40);
           if (!ok) break;
           const uint32_t full = bar_full + 8 * s, sa = smem_base + s * S::kOperandBytes;
-          mbar_expect_tx(full, (p.gather ? 0 : kABytes) + S::kBBytes);
+          const uint32_t sf = sf_base + s * S::kSfBytes;
+          const uint32_t sf_bytes = min(kTiles, p.k_tiles - kb * kTiles) * 512;
+          mbar_expect_tx(full, (p.gather ? 0 : kABytes) + S::kBBytes + S::kBlocks * sf_bytes);
+          bulk_load(sf, sfa + (int64_t)kb * kTiles * 512, sf_bytes, full);
+#pragma unroll
+          for (int b = 0; b < kNB; ++b)
+            bulk_load(sf + (1 + b) * kTiles * 512, sfb[b] + (int64_t)kb * kTiles * 512, sf_bytes, full);
           if (!p.gather) tma_load_2d(sa, &tma_a, full, kb * 128, t.m * kBM);
           if (GATED) {
 #pragma unroll
@@ -195,7 +197,7 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
       int s = 0;
       uint32_t ph = 0, tph = 0;
       bool ok = true;
-      const uint32_t sfa_t = tmem_base + BN, sfb_t = sfa_t + 4 * kTiles;
+      uint32_t kbi = 0;
       for (int i = blockIdx.x; ok && i < total; i += gridDim.x) {
         const Tile t = tile_of(p, i, num_m);
         if (t.expert < 0) continue;
@@ -208,8 +210,13 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
           tc_fence_after();
           if (p.gather) fence_async_smem();   // rows came through the generic proxy
           const uint32_t sa = smem_base + s * S::kOperandBytes, sf = sf_base + s * S::kSfBytes;
+          // (two sets of scale columns: the copies need not wait for the last K block's instructions)
+          const uint32_t sfa_t = tmem_base + BN + (kbi++ & 1u) * (4 * kTiles * S::kBlocks);
+          const uint32_t sfb_t = sfa_t + 4 * kTiles;
+          const int tiles = min(kTiles, p.k_tiles - kb * kTiles);
 #pragma unroll
           for (int j = 0; j < kTiles; ++j) {
+            if (j >= tiles) break;
             tc_cp_sf(sfa_t + 4 * j, make_sf_desc(sf + j * 512));
 #pragma unroll
             for (int b = 0; b < kNB; ++b)
@@ -234,88 +241,31 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
       }
     }
   } else if (warp < 4) {
-    // ------------------------------ scales, gathered rows ------------------------------
-    constexpr int kUnits = S::kBlocks * 2;        // groups of 32 rows this warp brings (of 4 per block)
-    constexpr int kQuads = NV ? 2 : 1;            // 16-byte pieces of a row's two K blocks
-    const int first = (warp - 2) * kUnits;
+    // ------------------------------ gathered rows ------------------------------
+    // 64 threads bring the 128 rows x 128 bytes of a K block, eight neighbours a row, to where the
+    // swizzled box would put them
     const int t64 = threadIdx.x - 64, c16 = t64 & 7, g0 = t64 >> 3;
+    const int k_bytes = p.k / 2;
     int s = 0;
     uint32_t ph = 0;
-    bool ok = true;
+    bool ok = p.gather != 0;
     for (int i = blockIdx.x; ok && i < total; i += gridDim.x) {
       const Tile t = tile_of(p, i, num_m);
       if (t.expert < 0) continue;
-      const uint8_t* src[kUnits];
-      uint32_t dst[kUnits];
-#pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        const int b = (first + u) >> 2, grp = (first + u) & 3;
-        const int r = (lane & 3) * 32 + (lane >> 2) + 8 * grp;
-        dst[u] = (uint32_t)b * kTiles * 512 + (uint32_t)(r & 31) * 16 + (uint32_t)(r >> 5) * 4;
-        if (b == 0) {
-          const int row = source_row(p, t.m, r);
-          src[u] = row < 0 ? nullptr : p.sfa + (int64_t)row * p.sf_row;
-        } else {
-          const int row = weight_row<BN, GATED>(p, t.n, (b - 1) * 128 + r);
-          src[u] = row < 0 ? nullptr : p.sfb + ((int64_t)t.expert * p.n + row) * p.sf_row;
-        }
-      }
       int roff[16];
-      if (p.gather) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) roff[j] = source_row(p, t.m, g0 + 8 * j);
-      }
-      const int k_bytes = p.k / 2;
-      uint32_t w[kUnits][kQuads * 4];
-      auto fetch = [&](int pair) {
-#pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-          const int off = pair * kQuads * 16;
-          if (p.sf_vec_ok) {
-#pragma unroll
-            for (int q = 0; q < kQuads; ++q) {
-              uint4 v = make_uint4(0u, 0u, 0u, 0u);
-              if (src[u] != nullptr && off + 16 * q < p.sf_row)
-                v = *reinterpret_cast<const uint4*>(src[u] + off + 16 * q);
-              w[u][4 * q] = v.x;
-              w[u][4 * q + 1] = v.y;
-              w[u][4 * q + 2] = v.z;
-              w[u][4 * q + 3] = v.w;
-            }
-          } else {
-#pragma unroll
-            for (int q = 0; q < kQuads * 4; ++q)
-              w[u][q] = src[u] != nullptr && off + 4 * q < p.sf_row
-                            ? *reinterpret_cast<const uint32_t*>(src[u] + off + 4 * q)
-                            : 0u;
-          }
-        }
-      };
+      for (int j = 0; j < 16; ++j) roff[j] = source_row(p, t.m, g0 + 8 * j);
       for (int kb = 0; kb < p.num_kb; ++kb) {
-        if ((kb & 1) == 0) fetch(kb >> 1);
         ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 43);
         if (!ok) break;
-        const uint32_t sf = sf_base + s * S::kSfBytes;
+        const uint32_t sa = smem_base + s * S::kOperandBytes + (uint32_t)g0 * 128u + (uint32_t)((c16 ^ (g0 & 7)) << 4);
+        const int kbyte = kb * 128 + c16 * 16;
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u)
-#pragma unroll
-          for (int j = 0; j < kTiles; ++j) {
-            const uint32_t v = (kb & 1) ? w[u][kTiles + j] : w[u][j];
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(sf + dst[u] + j * 512), "r"(v) : "memory");
-          }
-        fence_async_smem();
-        mbar_arrive(bar_full + 8 * s);
-        if (p.gather) {
-          const uint32_t sa = smem_base + s * S::kOperandBytes + (uint32_t)g0 * 128u +
-                              (uint32_t)((c16 ^ (g0 & 7)) << 4);
-          const int kbyte = kb * 128 + c16 * 16;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const bool live = kbyte < k_bytes && roff[j] >= 0;
-            cp_async_16(sa + j * 1024, live ? p.a + (int64_t)roff[j] * k_bytes + kbyte : p.a, live ? 16u : 0u);
-          }
-          cp_async_mbar_arrive_noinc(bar_full + 8 * s);
+        for (int j = 0; j < 16; ++j) {
+          const bool live = kbyte < k_bytes && roff[j] >= 0;
+          cp_async_16(sa + j * 1024, live ? p.a + (int64_t)roff[j] * k_bytes + kbyte : p.a, live ? 16u : 0u);
         }
+        cp_async_mbar_arrive_noinc(bar_full + 8 * s);
         if (++s == kStages) { s = 0; ph ^= 1; }
       }
     }
@@ -392,7 +342,10 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
         const int col0 = t.n * (BN / 2) + 64 * h;
         if (col0 < p.n_half) {
           uint8_t* codes = static_cast<uint8_t*>(p.c) + ((int64_t)row * p.n_half + col0) / 2;
-          uint8_t* scales = p.c_scale + ((int64_t)row * p.n_half + col0) / kBlk;
+          // the next product's A scales, in its tiles already: one word (NV) or half of one (MX)
+          constexpr int kSpan = 4 * kBlk;        // columns of a tile
+          uint8_t* scales = p.c_scale + ((int64_t)t.m * (p.n_half / kSpan) + col0 / kSpan) * 512 +
+                            (row_in_tile & 31) * 16 + (row_in_tile >> 5) * 4 + (NV ? 0 : (col0 / kBlk) & 3);
           uint32_t words[8], bytes = 0;
 #pragma unroll
           for (int b = 0; b < 64 / kBlk; ++b) {
@@ -435,6 +388,83 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
                  : "memory");
 }
 
+// ---------------------------------------------------------------------------
+// scales into the instruction's tiles
+// ---------------------------------------------------------------------------
+// A warp takes 128 rows and 16 bytes of each (four tiles): lane l reads the pieces of rows l, l + 32,
+// l + 64 and l + 96 and writes lane l's 16 bytes of every tile, 512 consecutive bytes a warp.
+struct TileParams {
+  bolt_fp4_tile_job job[BOLT_FP4_TILE_JOBS];
+  int blocks[BOLT_FP4_TILE_JOBS];       // 128-row blocks of an expert
+  int64_t warps[BOLT_FP4_TILE_JOBS];    // blocks * experts * 16-byte pieces of a row
+  int jobs, experts;
+  const int32_t *sorted_ids, *expert_ids, *num_valid;
+  int num_tokens, capacity;
+};
+
+__global__ void __launch_bounds__(256) k_tile_scales(const TileParams p) {
+  const int lane = threadIdx.x & 31;
+  // experts that no tile names are left alone
+  extern __shared__ uint32_t named[];
+  const int num_m = p.num_valid != nullptr ? min(*p.num_valid, p.capacity) / kBM : 0;
+  const int experts = p.experts;
+  if (p.expert_ids != nullptr) {
+    for (int i = threadIdx.x; i < (experts + 31) / 32; i += blockDim.x) named[i] = 0u;
+    __syncthreads();
+    for (int i = threadIdx.x; i < num_m; i += blockDim.x) {
+      const int e = p.expert_ids[i];
+      if (e >= 0 && e < experts) atomicOr(&named[e >> 5], 1u << (e & 31));
+    }
+    __syncthreads();
+  }
+  const int64_t first = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int64_t step = ((int64_t)gridDim.x * blockDim.x) >> 5;
+  for (int j = 0; j < p.jobs; ++j) {
+    const bolt_fp4_tile_job& job = p.job[j];
+    const bool vec_ok = job.row_bytes % 16 == 0;
+    const int pieces = (job.row_bytes + 15) / 16;
+    for (int64_t i = first; i < p.warps[j]; i += step) {
+      const int64_t eb = i / pieces;
+      const int piece = (int)(i - eb * pieces), e = (int)(eb / p.blocks[j]);
+      const int b = (int)(eb - (int64_t)e * p.blocks[j]);
+      if (job.by_sorted_id ? b >= num_m : (p.expert_ids != nullptr && !((named[e >> 5] >> (e & 31)) & 1u))) continue;
+      uint4 v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = lane + 32 * q;
+        int row;
+        if (job.by_sorted_id) {
+          row = p.sorted_ids[b * 128 + r] & 0xFFFFFF;
+          if (row >= p.num_tokens) row = -1;
+        } else if (job.gated_half > 0) {
+          const int col = b * 64 + (r & 63);
+          row = col < job.gated_half ? (r >> 6) * job.gated_half + col : -1;
+        } else {
+          row = b * 128 + r < job.rows ? b * 128 + r : -1;
+        }
+        v[q] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < 0) continue;
+        const uint8_t* src = static_cast<const uint8_t*>(job.src) + ((int64_t)e * job.rows + row) * job.row_bytes + piece * 16;
+        if (vec_ok) {
+          v[q] = *reinterpret_cast<const uint4*>(src);
+        } else {
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[k] = piece * 16 + 4 * k < job.row_bytes ? *reinterpret_cast<const uint32_t*>(src + 4 * k) : 0u;
+          v[q] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      uint8_t* dst = static_cast<uint8_t*>(job.dst) + (eb * (job.row_bytes / 4) + piece * 4) * 512 + lane * 16;
+      const uint4 out[4] = {make_uint4(v[0].x, v[1].x, v[2].x, v[3].x), make_uint4(v[0].y, v[1].y, v[2].y, v[3].y),
+                            make_uint4(v[0].z, v[1].z, v[2].z, v[3].z), make_uint4(v[0].w, v[1].w, v[2].w, v[3].w)};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (piece * 16 + 4 * k < job.row_bytes) *reinterpret_cast<uint4*>(dst + 512 * k) = out[k];
+    }
+  }
+}
+
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                    const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                    const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -470,9 +500,53 @@ int launch_format(bool gated, int bn, const CUtensorMap& ma, const CUtensorMap& 
   return launch<NV, 256, false>(ma, mb, p, grid, st);
 }
 
+int blocks_of(int rows, int gated_half) { return gated_half > 0 ? (gated_half + 63) / 64 : (rows + kBM - 1) / kBM; }
+
 }  // namespace
 }  // namespace fp4gemm
 }  // namespace bolt
+
+extern "C" int bolt_fp4_tile_scales(const bolt_fp4_tile_args* a, void* stream) {
+  using namespace bolt;
+  using namespace bolt::fp4gemm;
+  BOLT_REQUIRE(a != nullptr && a->jobs >= 0 && a->jobs <= BOLT_FP4_TILE_JOBS, "fp4_tile_scales: bad arguments");
+  BOLT_REQUIRE(a->expert_ids == nullptr || (a->num_valid_ids && a->sorted_ids && a->capacity % kBM == 0),
+               "fp4_tile_scales: the sort's arrays go together");
+  TileParams p = {};
+  int64_t warps = 0;
+  for (int j = 0; j < a->jobs; ++j) {
+    const bolt_fp4_tile_job& job = a->job[j];
+    BOLT_REQUIRE(job.rows >= 0 && job.experts > 0 && job.row_bytes >= 0 && job.row_bytes % 4 == 0,
+                 "fp4_tile_scales: bad shape");
+    BOLT_REQUIRE(!job.by_sorted_id || (a->expert_ids && job.experts == 1 && job.gated_half == 0),
+                 "fp4_tile_scales: rows through sorted ids need the sort's arrays");
+    BOLT_REQUIRE(job.gated_half >= 0 && (job.gated_half == 0 || job.rows == 2 * job.gated_half),
+                 "fp4_tile_scales: gated rows are two halves");
+    const int blocks = job.by_sorted_id ? a->capacity / kBM : blocks_of(job.rows, job.gated_half);
+    const int64_t n = (int64_t)blocks * job.experts * ((job.row_bytes + 15) / 16);
+    if (n == 0) continue;
+    BOLT_REQUIRE(job.src && job.dst && reinterpret_cast<uintptr_t>(job.src) % (job.row_bytes % 16 == 0 ? 16 : 4) == 0 &&
+                     reinterpret_cast<uintptr_t>(job.dst) % 16 == 0,
+                 "fp4_tile_scales: scales must be aligned to 16 bytes (rows of whole 16 bytes) or 4");
+    p.job[p.jobs] = job;
+    p.blocks[p.jobs] = blocks;
+    p.warps[p.jobs++] = n;
+    warps += n;
+    if (!job.by_sorted_id && job.experts > p.experts) p.experts = job.experts;
+  }
+  if (p.jobs == 0) return BOLT_OK;
+  p.sorted_ids = a->sorted_ids;
+  p.expert_ids = a->expert_ids;
+  p.num_valid = a->num_valid_ids;
+  p.num_tokens = a->num_tokens;
+  p.capacity = a->capacity;
+  const int64_t want = (warps + 7) / 8, most = (int64_t)sm_count_of_current_device() * 8;
+  const int smem = p.expert_ids != nullptr ? (p.experts + 31) / 32 * 4 : 0;
+  BOLT_REQUIRE(smem <= 48 * 1024, "fp4_tile_scales: too many experts");
+  k_tile_scales<<<(unsigned)(want < most ? want : most), 256, smem, static_cast<cudaStream_t>(stream)>>>(p);
+  BOLT_LAUNCH_CHECK();
+  return BOLT_OK;
+}
 
 extern "C" int bolt_fp4_gemm(const bolt_fp4_gemm_args* a, void* stream) {
   using namespace bolt;
@@ -495,9 +569,9 @@ extern "C" int bolt_fp4_gemm(const bolt_fp4_gemm_args* a, void* stream) {
                "fp4_gemm: grouped operands need the sort's arrays and a capacity in whole tiles");
   const int all_rows = grouped ? a->capacity : a->rows;
   if (all_rows == 0 || a->n == 0 || (grouped && a->num_tokens == 0)) return BOLT_OK;
-  BOLT_REQUIRE(a->a && a->a_scale && a->b && a->b_scale && a->c && (!gated || a->c_scale), "fp4_gemm: null pointer");
-  BOLT_REQUIRE(((reinterpret_cast<uintptr_t>(a->a) | reinterpret_cast<uintptr_t>(a->a_scale) |
-                 reinterpret_cast<uintptr_t>(a->b) | reinterpret_cast<uintptr_t>(a->b_scale)) & 15) == 0,
+  BOLT_REQUIRE(a->a && a->a_tiles && a->b && a->b_tiles && a->c && (!gated || a->c_scale), "fp4_gemm: null pointer");
+  BOLT_REQUIRE(((reinterpret_cast<uintptr_t>(a->a) | reinterpret_cast<uintptr_t>(a->a_tiles) |
+                 reinterpret_cast<uintptr_t>(a->b) | reinterpret_cast<uintptr_t>(a->b_tiles)) & 15) == 0,
                "fp4_gemm: operands must be 16-byte aligned");
   if (gated)
     BOLT_REQUIRE(reinterpret_cast<uintptr_t>(a->c) % 16 == 0 && reinterpret_cast<uintptr_t>(a->c_scale) % 4 == 0,
@@ -509,8 +583,6 @@ extern "C" int bolt_fp4_gemm(const bolt_fp4_gemm_args* a, void* stream) {
 
   Params p = {};
   p.a = static_cast<const uint8_t*>(a->a);
-  p.sfa = static_cast<const uint8_t*>(a->a_scale);
-  p.sfb = static_cast<const uint8_t*>(a->b_scale);
   p.alpha = a->alpha;
   p.a_global = a->a_global;
   p.b_global = a->b_global;
@@ -528,8 +600,10 @@ extern "C" int bolt_fp4_gemm(const bolt_fp4_gemm_args* a, void* stream) {
   p.num_experts = a->num_experts;
   p.capacity = a->capacity;
   p.num_kb = (a->k + 255) / 256;
-  p.sf_row = a->k / block;
-  p.sf_vec_ok = p.sf_row % 16 == 0;
+  p.k_tiles = a->k / (4 * block);
+  p.n_blocks = blocks_of(a->n, gated ? a->n / 2 : 0);
+  p.sfa = static_cast<const uint8_t*>(a->a_tiles);
+  p.sfb = static_cast<const uint8_t*>(a->b_tiles);
   p.gather = a->gather ? 1 : 0;
   p.num_tokens = a->num_tokens;
   p.sorted_ids = a->sorted_ids;

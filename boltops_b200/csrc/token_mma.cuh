@@ -313,10 +313,11 @@ __device__ __forceinline__ uint32_t codes4(const float4& v, float inv) {
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v.z * inv, v.w * inv), __NV_SATFINITE, __NV_E4M3);
   return lo | (hi << 16);
 }
-// scale and reciprocal of a row or group, the arithmetic of the row quantisers (quant.cu)
+// Scale of a row or group and its reciprocal: amax times the rounded 1 / 448 (1 / 127).  (The row
+// quantisers of quant.cu divide; the scales may differ in the last bit.)
 template <int K>
 __device__ __forceinline__ void scale8(float amax, float& scale, float& inv) {
-  scale = __fdiv_rn(fmaxf(amax, 1.0e-10f), is_i8(K) ? 127.0f : 448.0f);
+  scale = fmaxf(amax, 1.0e-10f) * (is_i8(K) ? (float)(1.0 / 127.0) : (float)(1.0 / 448.0));
   inv = __frcp_rn(scale);
 }
 

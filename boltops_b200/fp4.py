@@ -45,7 +45,7 @@ def fp4_quant(x: torch.Tensor, format: str = "nvfp4", global_scale: Optional[tor
               ) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(codes [..., K/2] uint8, scales [..., K/block])`` of ``x`` [..., K] (bf16, fp16 or fp32).
 
-    nvfp4: ``y = x * (1 / global_scale)``, ``scale = e4m3(min(amax(y) / 6, 448))``; mxfp4: the smallest
+    nvfp4: ``y = x * (1 / global_scale)``, ``scale = e4m3(min(amax(y) * (1/6), 448))``; mxfp4: the smallest
     power of two that is at least ``amax / 6`` (byte 0 for a block of zeros).  A code is the nearest of
     ``value / scale``, ties to even.  A block that holds a NaN or an infinity gets the NaN scale and
     reads back as NaNs."""

@@ -9,7 +9,9 @@ experts, and it fills its weight rings while the first one finishes.
 
 Same recipes as ``fused_experts`` (16-bit, fp8 and int8 w8a8 block-scaled and per-channel) and
 ``fused_experts_fp4`` (w4a4), with fewer roundings: GEMM 1 and the routes' results stay in fp32, quantised
-experts quantise the fp32 activation, 16-bit experts round it to the weights' type.
+experts quantise the fp32 activation, 16-bit experts round it to the weights' type.  The w8a8 scales are
+amax times the rounded 1/448 or 1/127, where ``fused_experts`` divides: they may differ in the last bit,
+and with them the codes of values that lie on the border of two.
 """
 from __future__ import annotations
 

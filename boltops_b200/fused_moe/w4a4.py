@@ -3,8 +3,9 @@
     out[m] = s * sum_k w[m, k] * W2[e] . Q2(act(W1[e] . Q1(x[m]))),   e = topk_ids[m, k]
 
 Q1 and Q2 are ``fp4.fp4_quant`` in the weights' format (nvfp4 or mxfp4); between them everything is fp32.
-Five launches: quantise the rows, sort, GEMM 1 (gathers its rows by token and quantises the activation
-in its epilogue), GEMM 2 (router weight in its epilogue), sum over a token's routes.  Products run on the tensor
+Six launches: quantise the rows, sort, lay out the scales for the tensor cores, GEMM 1 (gathers its rows
+by token and quantises the activation in its epilogue), GEMM 2 (router weight in its epilogue), sum
+over a token's routes.  Products run on the tensor
 cores' 4-bit block-scaled kind, four times the rate of 16-bit ones, and read half the bytes of w4a8.
 """
 from __future__ import annotations
@@ -115,7 +116,19 @@ def fused_experts_fp4(
             expert_ids = ops.relabel_tiles(expert_ids, expert_map)
         cap = sorted_ids.shape[0]
         act_codes = torch.empty((cap, inter // 2), dtype=torch.uint8, device=dev)
-        act_scales = torch.empty((cap, inter // block), dtype=scale_dtype, device=dev)
+        # the scales of all four operands in the tensor core's tiles; those of the activation come
+        # out of GEMM 1 like that
+        sizes = (cap * hidden // block, e * ops.ceil_to(inter, 64) * 2 * hidden // block,
+                 e * ops.ceil_to(model_dim, 128) * inter // block, cap * inter // block)
+        tiles = torch.empty(sum(sizes), dtype=torch.uint8, device=dev)
+        at = [tiles.data_ptr() + sum(sizes[:i]) for i in range(4)]
+        lay = _cabi.Fp4TileArgs()
+        lay.jobs, lay.num_tokens, lay.capacity = 3, rows, cap
+        lay.sorted_ids, lay.expert_ids = sorted_ids.data_ptr(), expert_ids.data_ptr()
+        lay.num_valid_ids = num_valid.data_ptr()
+        lay.job[0] = (scales.data_ptr(), at[0], rows, hidden // block, 1, 0, 1)
+        lay.job[1] = (w1_scale.data_ptr(), at[1], 2 * inter, hidden // block, e, inter, 0)
+        lay.job[2] = (w2_scale.data_ptr(), at[2], model_dim, inter // block, e, 0, 0)
         rows_out = torch.empty((cap, model_dim), dtype=out_dtype, device=dev)
         args = _cabi.Fp4GemmArgs()
         args.format, args.num_experts, args.capacity, args.num_tokens = code, e, cap, rows
@@ -125,21 +138,22 @@ def fused_experts_fp4(
         args.sm_count = ops.gemm_sm_count(dev)
         stream = _cabi.stream_of(hidden_states)
         with _cabi.on_device(dev):
+            _cabi.check(lib.bolt_fp4_tile_scales(lay, stream))
             args.epilogue, args.gather = _cabi.EPI_SILU_MUL_QUANT, 1
             args.rows, args.n, args.k = rows, 2 * inter, hidden
-            args.a, args.a_scale, args.b, args.b_scale = (t.data_ptr() for t in (codes, scales, w1, w1_scale))
+            args.a, args.a_tiles, args.b, args.b_tiles = codes.data_ptr(), at[0], w1.data_ptr(), at[1]
             args.a_global, args.b_global, args.c_global = _cabi.ptr(a1), _cabi.ptr(g1), _cabi.ptr(a2)
-            args.c, args.c_scale = act_codes.data_ptr(), act_scales.data_ptr()
+            args.c, args.c_scale = act_codes.data_ptr(), at[3]
             args.activation, args.act_alpha, args.act_limit = act, alpha, limit
             _cabi.check(lib.bolt_fp4_gemm(args, stream))
             args.epilogue, args.gather = _cabi.EPI_STORE, 0
             args.rows, args.n, args.k = cap, model_dim, inter
-            args.a, args.a_scale, args.b, args.b_scale = (t.data_ptr() for t in (act_codes, act_scales, w2, w2_scale))
+            args.a, args.a_tiles, args.b, args.b_tiles = act_codes.data_ptr(), at[3], w2.data_ptr(), at[2]
             args.a_global, args.b_global, args.c_global = _cabi.ptr(a2), _cabi.ptr(g2), None
             args.c, args.c_dtype, args.c_ld = rows_out.data_ptr(), _cabi.dtype_code(out_dtype), model_dim
             args.sorted_weights = sorted_w.data_ptr()
             _cabi.check(lib.bolt_fp4_gemm(args, stream))
-        ops._count(2)
+        ops._count(3)
         ops.gather_sum(rows_out, route_pos, out[begin:end], scale)
     return out
 

@@ -149,12 +149,24 @@ def gemm_a4w4(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor, w_scale: 
     args = _cabi.Fp4GemmArgs()
     args.format, args.epilogue = code, _cabi.EPI_STORE
     args.rows, args.n, args.k, args.num_experts = m, n, k, 1
-    args.a, args.a_scale, args.b, args.b_scale = (t.data_ptr() for t in (x, x_scale, w, w_scale))
+    # the scales in the tensor core's tiles: whole 128-row blocks of both operands
+    row_bytes = k // block
+    blocks_m = (m + 127) // 128
+    tiles = torch.empty((blocks_m + (n + 127) // 128) * 128 * row_bytes, dtype=torch.uint8, device=dev)
+    lay = _cabi.Fp4TileArgs()
+    lay.jobs = 2
+    lay.job[0] = (x_scale.data_ptr(), tiles.data_ptr(), m, row_bytes, 1, 0, 0)
+    lay.job[1] = (w_scale.data_ptr(), tiles.data_ptr() + blocks_m * 128 * row_bytes, n, row_bytes, 1, 0, 0)
+    args.a, args.b = x.data_ptr(), w.data_ptr()
+    args.a_tiles, args.b_tiles = lay.job[0].dst, lay.job[1].dst
     args.alpha = _cabi.ptr(alpha)
     args.c, args.c_dtype, args.c_ld = out.data_ptr(), _cabi.dtype_code(dtype), out.stride(0) if m > 1 else n
     args.status = ops.device_status(dev).data_ptr()
     args.sm_count = ops.gemm_sm_count(dev)
+    lib = _cabi.load()
+    stream = _cabi.stream_of(x)
     with _cabi.on_device(dev):
-        _cabi.check(_cabi.load().bolt_fp4_gemm(args, _cabi.stream_of(x)))
-    ops._count()
+        _cabi.check(lib.bolt_fp4_tile_scales(lay, stream))
+        _cabi.check(lib.bolt_fp4_gemm(args, stream))
+    ops._count(2)
     return out

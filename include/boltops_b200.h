@@ -587,7 +587,7 @@ int bolt_moe_layer(const bolt_layer_args* args, void* stream);
 /* microscaled 4-bit floating point                                            */
 /* ------------------------------------------------------------------------- */
 /* e2m1 codes, two to a byte (the first value in the low bits), blocks along the last dimension:
- *   NV: 16 values, E4M3 scale byte s = e4m3(min(amax / 6, 448)), value code * s * global_scale;
+ *   NV: 16 values, E4M3 scale byte s = e4m3(min(amax * (1/6), 448)), value code * s * global_scale;
  *       values are multiplied with the rounded 1 / global_scale before they are quantised
  *   MX: 32 values, E8M0 scale byte: the smallest 2^(byte - 127) >= amax / 6 (byte 0 for a block of
  *       zeros), value code * 2^(byte - 127)
@@ -602,29 +602,49 @@ int bolt_fp4_quant(const void* x, int dtype, int64_t rows, int64_t cols, int for
 int bolt_fp4_dequant(const void* codes, const void* scales, int64_t rows, int64_t cols, int format,
                      const float* global_scale, void* out, int dtype, void* stream);
 
-/* Products of 4-bit rows with 4-bit weights, both in the same format, scales in the layout that
- * bolt_fp4_quant writes.
+/* Scales as the tensor core takes them: 512-byte tiles of 128 rows x 4 scales, byte
+ * (r % 32) * 16 + (r / 32) * 4 + i, [experts][128-row blocks][row_bytes / 4] of them.  Up to three arrays of
+ * rows of scale bytes [experts, rows, row_bytes] (row_bytes a multiple of 4) in one launch. */
+#define BOLT_FP4_TILE_JOBS 3
+typedef struct bolt_fp4_tile_job {
+  const void* src;
+  void* dst;                   /* rows that do not exist become zeros                         */
+  int rows, row_bytes, experts;
+  int gated_half;              /* > 0: rows are [gate | up], this many each; block b holds gate */
+                               /*   rows 64 b .. and then the up rows of the same columns     */
+  int by_sorted_id;            /* block b holds rows sorted_ids[128 b ..] & 0xFFFFFF          */
+} bolt_fp4_tile_job;
+typedef struct bolt_fp4_tile_args {
+  bolt_fp4_tile_job job[BOLT_FP4_TILE_JOBS];
+  int jobs, num_tokens, capacity;
+  const int32_t* sorted_ids;       /* with expert_ids (the tiles' experts, as in bolt_fp4_gemm): experts */
+  const int32_t* expert_ids;       /*   that no tile names, and blocks past num_valid_ids, are left alone */
+  const int32_t* num_valid_ids;
+} bolt_fp4_tile_args;
+int bolt_fp4_tile_scales(const bolt_fp4_tile_args* args, void* stream);
+
+/* Products of 4-bit rows with 4-bit weights, both in the same format, scales in tiles
+ * (bolt_fp4_tile_scales; b's gated for the quantising epilogue).
  *
  * Dense (sorted_expert_ids null): c[m, n] = f * sum_blocks sa sb (a . b), m < rows, b [n, k / 2].
  * Grouped: 128-row tiles in the order of bolt_moe_sort_ck; tile i multiplies with expert
- * sorted_expert_ids[i] of b [num_experts, n, k / 2].  With gather, a and a_scale are in token order
- * (rows = tokens) and sorted position p reads row sorted_ids[p] & 0xFFFFFF; else they are in sorted
- * order (rows = capacity).  Results of positions that only pad a tile are not stored (the quantising
- * epilogue stores zeros).
+ * sorted_expert_ids[i] of b [num_experts, n, k / 2].  With gather, a is in token order (rows = tokens) and
+ * sorted position p reads row sorted_ids[p] & 0xFFFFFF; else a is in sorted order (rows = capacity); the
+ * scale tiles are in sorted order either way.  Results of positions that only pad a tile are not
+ * stored (the quantising epilogue stores zeros).
  * f = alpha * a_global * b_global[expert] * sorted_weights[position], each optional (null: 1).
  * BOLT_EPI_STORE: c [rows or capacity, n] in c_dtype, rows c_ld elements apart.
  * BOLT_EPI_SILU_MUL_QUANT: b's rows are [gate | up]; act(gate, up) in fp32, times 1 / c_global (NV), is
- * quantised: c [capacity, n / 4] codes, c_scale [capacity, n / 2 / block].  Grouped only.
- * k: a multiple of 64 (NV) or 128 (MX), n / 2 too with the quantising epilogue.  a, b and their scales
- * 16-byte aligned. */
+ * quantised: c [capacity, n / 4] codes, c_scale their scales in tiles.  Grouped only.
+ * k: a multiple of 64 (NV) or 128 (MX), n / 2 too with the quantising epilogue.  All 16-byte aligned. */
 typedef struct bolt_fp4_gemm_args {
   int format;                  /* enum bolt_fp4_format                                        */
   int epilogue;                /* BOLT_EPI_STORE or BOLT_EPI_SILU_MUL_QUANT                   */
   int rows, n, k, num_experts;
   const void* a;
-  const void* a_scale;
+  const void* a_tiles;
   const void* b;
-  const void* b_scale;
+  const void* b_tiles;
   const float* alpha;
   const float* a_global;
   const float* b_global;

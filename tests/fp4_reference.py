@@ -31,7 +31,8 @@ def fp4_scales(fmt: str, y: torch.Tensor):
     """Stored scales and their values for blocks [..., n, block] of finite doubles."""
     amax = y.abs().amax(-1)
     if fmt == "nvfp4":
-        s = (amax / 6).clamp(max=448).float().to(FP8)
+        # (the recipe multiplies in fp32 with the rounded 1/6)
+        s = (amax.float() * torch.tensor(1 / 6, dtype=torch.float32)).clamp(max=448).to(FP8)
         return s, s.double()
     # smallest 2^e >= amax / 6; frexp: amax = part * 2^e', part in [0.5, 1)
     part, e = torch.frexp(amax)
@@ -120,7 +121,7 @@ def quant_rows(kind: str, v: torch.Tensor, g=None, scale_of=None) -> torch.Tenso
     group = 128 if kind.endswith("block") else v.shape[-1]
     largest = 448.0 if kind.startswith("fp8") else 127.0
     z = src.float().unflatten(-1, (-1, group))
-    s = z.abs().amax(-1, keepdim=True).clamp_min(1e-10) / largest
+    s = z.abs().amax(-1, keepdim=True).clamp_min(1e-10) * torch.tensor(1 / largest, dtype=torch.float32)
     y = v.float().unflatten(-1, (-1, group)) * (1.0 / s)      # the recipe scales in fp32
     q = y.clamp(-448, 448).to(FP8).double() if largest == 448 else y.round().clamp(-128, 127).double()
     return (q * s.double()).flatten(-2)
