@@ -99,7 +99,7 @@ class Fp4GemmArgs(C.Structure):
         ("alpha", C.c_void_p), ("a_global", C.c_void_p), ("b_global", C.c_void_p),
         ("c_global", C.c_void_p),
         ("c", C.c_void_p), ("c_dtype", C.c_int), ("c_ld", C.c_int64), ("c_scale", C.c_void_p),
-        ("capacity", C.c_int), ("gather", C.c_int), ("num_tokens", C.c_int),
+        ("capacity", C.c_int), ("num_tokens", C.c_int),
         ("sorted_ids", C.c_void_p), ("sorted_weights", C.c_void_p),
         ("sorted_expert_ids", C.c_void_p), ("num_valid_ids", C.c_void_p),
         ("activation", C.c_int), ("act_alpha", C.c_float), ("act_limit", C.c_float),

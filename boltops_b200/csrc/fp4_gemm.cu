@@ -12,12 +12,13 @@
 // was measured first: the writes have to be made visible to the tensor core's proxy once per K block,
 // and the product ran at 2700 TFLOP/s where it runs at 4000 without any scales (8192 x 7168 x 4096).
 //
-// Warp 0 brings boxes and scales, warp 1 issues the scales' copies to TMEM and the instructions, warps 2
-// and 3 gather rows (expert layers: rows in token order), warps 4 to 11 drain the accumulator.
+// Warp 0 brings boxes and scales, warp 1 issues the instructions, warp 3 the scales' copies to TMEM, warps
+// 4 to 11 drain the accumulator.  Rows are read in sorted order: bringing them by token inside the
+// product, four an instruction (tile::gather4, 68 cycles each) or by 16-byte copies of a spare warp, cost
+// more than a sorted copy of the codes (DeepSeek-V3, 64 experts, 1500 tokens: GEMM 1 905 us by gather4).
 #include <cuda.h>
 
 #include <atomic>
-#include <cstring>
 
 #include "act_pair.cuh"
 #include "fp4.cuh"
@@ -33,6 +34,7 @@ constexpr int kThreads = 384;
 constexpr int kBM = 128;
 constexpr int kTmemCols = 512;
 constexpr int kABytes = kBM * 128;
+constexpr int kSets = 4;                 // of scale columns: 4 x 48 and 256 sums fit TMEM
 constexpr int kOutBytes = 1024;          // per epilogue warp: 32 rows x 32 bytes
 
 template <bool NV, int BN>
@@ -40,6 +42,7 @@ struct Shape {
   static constexpr int kTiles = NV ? 4 : 2;                 // 512-byte scale tiles of a K block
   static constexpr int kBlocks = 1 + BN / 128;              // of 128 rows: A, then B
   static constexpr int kSfBytes = kBlocks * kTiles * 512;
+  static constexpr int kSfCols = kBlocks * kTiles * 4;      // of TMEM
   static constexpr int kBBytes = BN * 128;
   static constexpr int kStageBytes = kABytes + kBBytes + kSfBytes;
   static constexpr int kStages = (226 * 1024 - 2048 - 8 * kOutBytes) / ((kStageBytes + 1023) / 1024 * 1024);
@@ -49,7 +52,6 @@ struct Shape {
 };
 
 struct Params {
-  const uint8_t *a;
   const uint8_t *sfa, *sfb;              // tiles: [row block][K / 64 or K / 128][512], B per expert
   const float *alpha, *a_global, *b_global, *c_global;
   void* c;
@@ -61,7 +63,7 @@ struct Params {
   int num_kb, k_tiles;                   // K blocks; scale tiles along K
   int n_blocks;                          // 128-row blocks of an expert's weights
   int tiles_n, group_m;
-  int gather, num_tokens;
+  int num_tokens;
   const int32_t *sorted_ids, *expert_ids, *num_valid;
   const float* sorted_weights;
   ActParams act;
@@ -104,15 +106,6 @@ __device__ __forceinline__ Tile tile_of(const Params& p, int i, int num_m) {
   if (t.expert >= p.num_experts) t.expert = -1;
   return t;
 }
-// Row of `a` behind row i of a tile, or -1.
-__device__ __forceinline__ int source_row(const Params& p, int m_blk, int i) {
-  const int pos = m_blk * kBM + i;
-  if (p.gather) {
-    const int tok = p.sorted_ids[pos] & 0xFFFFFF;
-    return tok < p.num_tokens ? tok : -1;
-  }
-  return pos < p.rows ? pos : -1;
-}
 template <bool NV, int BN, bool GATED>
 __global__ void __launch_bounds__(kThreads, 1)
 k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const Params p) {
@@ -128,16 +121,20 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
   const uint32_t smem_base = smem_u32(smem), sf_base = smem_u32(sf_mem);
   const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * kStages;
   const uint32_t bar_tfull = bar_empty + 8 * kStages, bar_tempty = bar_tfull + 8;
+  const uint32_t bar_sf = bar_tempty + 8, bar_sf_free = bar_sf + 8 * kSets;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    // full: the bytes of boxes and scales (1), gathered rows (64 threads)
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(bar_full + 8 * s, p.gather ? 65 : 1);
+      mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
     }
     mbar_init(bar_tfull, 1);
     mbar_init(bar_tempty, 8);
+    for (int s = 0; s < kSets; ++s) {
+      mbar_init(bar_sf + 8 * s, 1);
+      mbar_init(bar_sf_free + 8 * s, 1);
+    }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -174,12 +171,12 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
           const uint32_t full = bar_full + 8 * s, sa = smem_base + s * S::kOperandBytes;
           const uint32_t sf = sf_base + s * S::kSfBytes;
           const uint32_t sf_bytes = min(kTiles, p.k_tiles - kb * kTiles) * 512;
-          mbar_expect_tx(full, (p.gather ? 0 : kABytes) + S::kBBytes + S::kBlocks * sf_bytes);
+          mbar_expect_tx(full, kABytes + S::kBBytes + S::kBlocks * sf_bytes);
           bulk_load(sf, sfa + (int64_t)kb * kTiles * 512, sf_bytes, full);
 #pragma unroll
           for (int b = 0; b < kNB; ++b)
             bulk_load(sf + (1 + b) * kTiles * 512, sfb[b] + (int64_t)kb * kTiles * 512, sf_bytes, full);
-          if (!p.gather) tma_load_2d(sa, &tma_a, full, kb * 128, t.m * kBM);
+          tma_load_2d(sa, &tma_a, full, kb * 128, t.m * kBM);
           if (GATED) {
 #pragma unroll
             for (int j = 0; j < BN / 64; ++j)
@@ -195,9 +192,8 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
   } else if (warp == 1) {
     if (lane == 0) {
       int s = 0;
-      uint32_t ph = 0, tph = 0;
+      uint32_t ph = 0, tph = 0, set = 0, sph = 0;
       bool ok = true;
-      uint32_t kbi = 0;
       for (int i = blockIdx.x; ok && i < total; i += gridDim.x) {
         const Tile t = tile_of(p, i, num_m);
         if (t.expert < 0) continue;
@@ -205,24 +201,13 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
         if (!ok) break;
         tc_fence_after();
         for (int kb = 0; kb < p.num_kb; ++kb) {
-          ok = mbar_wait(bar_full + 8 * s, ph, abort_flag, p.status, 42);
+          ok = mbar_wait(bar_full + 8 * s, ph, abort_flag, p.status, 42) &&
+               mbar_wait(bar_sf + 8 * set, sph, abort_flag, p.status, 44);
           if (!ok) break;
           tc_fence_after();
-          if (p.gather) fence_async_smem();   // rows came through the generic proxy
-          const uint32_t sa = smem_base + s * S::kOperandBytes, sf = sf_base + s * S::kSfBytes;
-          // (two sets of scale columns: the copies need not wait for the last K block's instructions)
-          const uint32_t sfa_t = tmem_base + BN + (kbi++ & 1u) * (4 * kTiles * S::kBlocks);
-          const uint32_t sfb_t = sfa_t + 4 * kTiles;
-          const int tiles = min(kTiles, p.k_tiles - kb * kTiles);
-#pragma unroll
-          for (int j = 0; j < kTiles; ++j) {
-            if (j >= tiles) break;
-            tc_cp_sf(sfa_t + 4 * j, make_sf_desc(sf + j * 512));
-#pragma unroll
-            for (int b = 0; b < kNB; ++b)
-              tc_cp_sf(sfb_t + 4 * (kNB * j + b), make_sf_desc(sf + ((1 + b) * kTiles + j) * 512));
-          }
+          const uint32_t sa = smem_base + s * S::kOperandBytes;
           const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + kABytes);
+          const uint32_t sfa_t = tmem_base + BN + set * S::kSfCols, sfb_t = sfa_t + 4 * kTiles;
           const int steps = min(4, (p.k - kb * 256) / 64);    // 64 values an instruction
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -234,43 +219,48 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
                         sfa_t + 4 * tile, sfb_t + 4 * kNB * tile, (kb > 0 || j > 0) ? 1u : 0u);
           }
           tc_commit(bar_empty + 8 * s);
+          tc_commit(bar_sf_free + 8 * set);
           if (++s == kStages) { s = 0; ph ^= 1; }
+          if (++set == kSets) { set = 0; sph ^= 1; }
         }
         if (ok) tc_commit(bar_tfull);
         tph ^= 1;
       }
     }
-  } else if (warp < 4) {
-    // ------------------------------ gathered rows ------------------------------
-    // 64 threads bring the 128 rows x 128 bytes of a K block, eight neighbours a row, to where the
-    // swizzled box would put them
-    const int t64 = threadIdx.x - 64, c16 = t64 & 7, g0 = t64 >> 3;
-    const int k_bytes = p.k / 2;
-    int s = 0;
-    uint32_t ph = 0;
-    bool ok = p.gather != 0;
-    for (int i = blockIdx.x; ok && i < total; i += gridDim.x) {
-      const Tile t = tile_of(p, i, num_m);
-      if (t.expert < 0) continue;
-      int roff[16];
+  } else if (warp == 3) {
+    // ------------------------------ scales to TMEM ------------------------------
+    // A thread of its own issues the copies, into kSets sets of columns by turns: behind the instructions
+    // of the thread that issues those they would wait for them, and they for the copies.
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0, set = 0, sph = 0;
+      bool ok = true;
+      for (int i = blockIdx.x; ok && i < total; i += gridDim.x) {
+        const Tile t = tile_of(p, i, num_m);
+        if (t.expert < 0) continue;
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+          ok = mbar_wait(bar_full + 8 * s, ph, abort_flag, p.status, 42) &&
+               mbar_wait(bar_sf_free + 8 * set, sph ^ 1, abort_flag, p.status, 44);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sf = sf_base + s * S::kSfBytes;
+          const uint32_t sfa_t = tmem_base + BN + set * S::kSfCols, sfb_t = sfa_t + 4 * kTiles;
+          const int tiles = min(kTiles, p.k_tiles - kb * kTiles);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) roff[j] = source_row(p, t.m, g0 + 8 * j);
-      for (int kb = 0; kb < p.num_kb; ++kb) {
-        ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 43);
-        if (!ok) break;
-        const uint32_t sa = smem_base + s * S::kOperandBytes + (uint32_t)g0 * 128u + (uint32_t)((c16 ^ (g0 & 7)) << 4);
-        const int kbyte = kb * 128 + c16 * 16;
+          for (int j = 0; j < kTiles; ++j) {
+            if (j >= tiles) break;
+            tc_cp_sf(sfa_t + 4 * j, make_sf_desc(sf + j * 512));
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const bool live = kbyte < k_bytes && roff[j] >= 0;
-          cp_async_16(sa + j * 1024, live ? p.a + (int64_t)roff[j] * k_bytes + kbyte : p.a, live ? 16u : 0u);
+            for (int b = 0; b < kNB; ++b)
+              tc_cp_sf(sfb_t + 4 * (kNB * j + b), make_sf_desc(sf + ((1 + b) * kTiles + j) * 512));
+          }
+          tc_commit(bar_sf + 8 * set);
+          if (++s == kStages) { s = 0; ph ^= 1; }
+          if (++set == kSets) { set = 0; sph ^= 1; }
         }
-        cp_async_mbar_arrive_noinc(bar_full + 8 * s);
-        if (++s == kStages) { s = 0; ph ^= 1; }
       }
     }
-    if (p.gather) cp_async_wait_all();
-  } else {
+  } else if (warp >= 4) {
     // ------------------------------ epilogue ------------------------------
     constexpr int kCols = BN / 2;                  // columns of this warp's half
     const int q = warp & 3, h = (warp - 4) >> 2, row_in_tile = 32 * q + lane;
@@ -561,11 +551,10 @@ extern "C" int bolt_fp4_gemm(const bolt_fp4_gemm_args* a, void* stream) {
   BOLT_REQUIRE(a->k % step == 0, "fp4_gemm: k %d must be a multiple of %d", a->k, step);
   BOLT_REQUIRE(!gated || (grouped && a->n % 2 == 0 && (a->n / 2) % step == 0),
                "fp4_gemm: the quantising epilogue is grouped and needs n / 2 in multiples of %d", step);
-  BOLT_REQUIRE(grouped || (a->num_experts == 1 && !a->gather && a->sorted_ids == nullptr &&
-                           a->sorted_weights == nullptr && a->num_valid_ids == nullptr),
+  BOLT_REQUIRE(grouped || (a->num_experts == 1 && a->sorted_ids == nullptr && a->sorted_weights == nullptr && a->num_valid_ids == nullptr),
                "fp4_gemm: dense operands have no sorted order");
   BOLT_REQUIRE(!grouped || (a->num_valid_ids && a->sorted_ids && a->capacity >= 0 && a->capacity % kBM == 0 &&
-                            a->num_tokens >= 0 && a->rows >= (a->gather ? a->num_tokens : a->capacity)),
+                            a->num_tokens >= 0 && a->rows >= a->capacity),
                "fp4_gemm: grouped operands need the sort's arrays and a capacity in whole tiles");
   const int all_rows = grouped ? a->capacity : a->rows;
   if (all_rows == 0 || a->n == 0 || (grouped && a->num_tokens == 0)) return BOLT_OK;
@@ -582,7 +571,6 @@ extern "C" int bolt_fp4_gemm(const bolt_fp4_gemm_args* a, void* stream) {
                  "fp4_gemm: bad output");
 
   Params p = {};
-  p.a = static_cast<const uint8_t*>(a->a);
   p.alpha = a->alpha;
   p.a_global = a->a_global;
   p.b_global = a->b_global;
@@ -604,7 +592,6 @@ extern "C" int bolt_fp4_gemm(const bolt_fp4_gemm_args* a, void* stream) {
   p.n_blocks = blocks_of(a->n, gated ? a->n / 2 : 0);
   p.sfa = static_cast<const uint8_t*>(a->a_tiles);
   p.sfb = static_cast<const uint8_t*>(a->b_tiles);
-  p.gather = a->gather ? 1 : 0;
   p.num_tokens = a->num_tokens;
   p.sorted_ids = a->sorted_ids;
   p.expert_ids = a->sorted_expert_ids;
@@ -615,7 +602,10 @@ extern "C" int bolt_fp4_gemm(const bolt_fp4_gemm_args* a, void* stream) {
 
   const int sms = a->sm_count > 0 ? a->sm_count : sm_count_of_current_device();
   const int64_t tiles_m = (all_rows + kBM - 1) / kBM;
-  const int bn = !gated && tiles_m * ((a->n + 255) / 256) < sms ? 128 : 256;
+  // Column tiles of 128 where they save a wave: a K block of one takes about 0.6 of the time of one of
+  // 256 (8192 x 7168 x 4096, NV: 256 columns 148 us; 777 x 4096 x 7168, MX: 128 columns 33 us, 256 22).
+  auto waves = [&](int cols) { return (tiles_m * ((a->n + cols - 1) / cols) + sms - 1) / sms; };
+  const int bn = !gated && 6 * waves(128) < 10 * waves(256) ? 128 : 256;
   p.tiles_n = gated ? (p.n_half + 127) / 128 : (a->n + bn - 1) / bn;
   p.group_m = grouped ? 4 : 16;
   // e2m1 x e2m1 (format 1), E4M3 or (bit 23) E8M0 scales, N >> 3 at bit 17, M >> 4 at bit 24
@@ -627,10 +617,9 @@ extern "C" int bolt_fp4_gemm(const bolt_fp4_gemm_args* a, void* stream) {
     return BOLT_ERR_CUDA;
   }
   CUtensorMap ma, mb;
-  std::memset(&ma, 0, sizeof(ma));
   const cuuint32_t ones[3] = {1, 1, 1};
   const cuuint64_t kb = (cuuint64_t)a->k / 2;
-  if (!p.gather) {
+  {
     const cuuint64_t size[2] = {kb, (cuuint64_t)a->rows}, strides[1] = {kb};
     const cuuint32_t box[2] = {128, kBM};
     const CUresult rc = encode(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(a->a), size, strides, box, ones,

@@ -3,9 +3,9 @@
     out[m] = s * sum_k w[m, k] * W2[e] . Q2(act(W1[e] . Q1(x[m]))),   e = topk_ids[m, k]
 
 Q1 and Q2 are ``fp4.fp4_quant`` in the weights' format (nvfp4 or mxfp4); between them everything is fp32.
-Six launches: quantise the rows, sort, lay out the scales for the tensor cores, GEMM 1 (gathers its rows
-by token and quantises the activation in its epilogue), GEMM 2 (router weight in its epilogue), sum
-over a token's routes.  Products run on the tensor
+Seven launches: quantise the rows, sort, copy the rows' codes into sorted order, lay out the scales for
+the tensor cores, GEMM 1 (quantises the activation in its epilogue), GEMM 2 (router weight in its
+epilogue), sum over a token's routes.  Products run on the tensor
 cores' 4-bit block-scaled kind, four times the rate of 16-bit ones, and read half the bytes of w4a8.
 """
 from __future__ import annotations
@@ -115,6 +115,7 @@ def fused_experts_fp4(
         if expert_map is not None:
             expert_ids = ops.relabel_tiles(expert_ids, expert_map)
         cap = sorted_ids.shape[0]
+        codes, _ = ops.gather_rows(codes, sorted_ids, num_valid, cap)
         act_codes = torch.empty((cap, inter // 2), dtype=torch.uint8, device=dev)
         # the scales of all four operands in the tensor core's tiles; those of the activation come
         # out of GEMM 1 like that
@@ -139,14 +140,14 @@ def fused_experts_fp4(
         stream = _cabi.stream_of(hidden_states)
         with _cabi.on_device(dev):
             _cabi.check(lib.bolt_fp4_tile_scales(lay, stream))
-            args.epilogue, args.gather = _cabi.EPI_SILU_MUL_QUANT, 1
-            args.rows, args.n, args.k = rows, 2 * inter, hidden
+            args.epilogue = _cabi.EPI_SILU_MUL_QUANT
+            args.rows, args.n, args.k = cap, 2 * inter, hidden
             args.a, args.a_tiles, args.b, args.b_tiles = codes.data_ptr(), at[0], w1.data_ptr(), at[1]
             args.a_global, args.b_global, args.c_global = _cabi.ptr(a1), _cabi.ptr(g1), _cabi.ptr(a2)
             args.c, args.c_scale = act_codes.data_ptr(), at[3]
             args.activation, args.act_alpha, args.act_limit = act, alpha, limit
             _cabi.check(lib.bolt_fp4_gemm(args, stream))
-            args.epilogue, args.gather = _cabi.EPI_STORE, 0
+            args.epilogue = _cabi.EPI_STORE
             args.rows, args.n, args.k = cap, model_dim, inter
             args.a, args.a_tiles, args.b, args.b_tiles = act_codes.data_ptr(), at[3], w2.data_ptr(), at[2]
             args.a_global, args.b_global, args.c_global = _cabi.ptr(a2), _cabi.ptr(g2), None

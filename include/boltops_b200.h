@@ -628,10 +628,8 @@ int bolt_fp4_tile_scales(const bolt_fp4_tile_args* args, void* stream);
  *
  * Dense (sorted_expert_ids null): c[m, n] = f * sum_blocks sa sb (a . b), m < rows, b [n, k / 2].
  * Grouped: 128-row tiles in the order of bolt_moe_sort_ck; tile i multiplies with expert
- * sorted_expert_ids[i] of b [num_experts, n, k / 2].  With gather, a is in token order (rows = tokens) and
- * sorted position p reads row sorted_ids[p] & 0xFFFFFF; else a is in sorted order (rows = capacity); the
- * scale tiles are in sorted order either way.  Results of positions that only pad a tile are not
- * stored (the quantising epilogue stores zeros).
+ * sorted_expert_ids[i] of b [num_experts, n, k / 2]; a is in sorted order (rows = capacity).  Results of
+ * positions that only pad a tile are not stored (the quantising epilogue stores zeros).
  * f = alpha * a_global * b_global[expert] * sorted_weights[position], each optional (null: 1).
  * BOLT_EPI_STORE: c [rows or capacity, n] in c_dtype, rows c_ld elements apart.
  * BOLT_EPI_SILU_MUL_QUANT: b's rows are [gate | up]; act(gate, up) in fp32, times 1 / c_global (NV), is
@@ -653,7 +651,7 @@ typedef struct bolt_fp4_gemm_args {
   int c_dtype;
   int64_t c_ld;
   void* c_scale;
-  int capacity, gather, num_tokens;
+  int capacity, num_tokens;
   const int32_t* sorted_ids;
   const float* sorted_weights;
   const int32_t* sorted_expert_ids;
