@@ -119,6 +119,14 @@ class Fp4TileArgs(C.Structure):
                 ("sorted_ids", C.c_void_p), ("expert_ids", C.c_void_p), ("num_valid_ids", C.c_void_p)]
 
 
+class Fp4FewArgs(C.Structure):
+    """struct bolt_fp4_few_args"""
+    _fields_ = [("format", C.c_int), ("rows", C.c_int), ("n", C.c_int), ("k", C.c_int),
+                ("x", C.c_void_p), ("x_scale", C.c_void_p), ("w", C.c_void_p), ("w_scale", C.c_void_p),
+                ("alpha", C.c_void_p), ("out", C.c_void_p), ("out_dtype", C.c_int), ("out_ld", C.c_int64),
+                ("status", C.c_void_p), ("sm_count", C.c_int)]
+
+
 class DecodeArgs(C.Structure):
     """struct bolt_decode_args"""
     _fields_ = [
@@ -228,6 +236,7 @@ _SIGNATURES = {
                                    C.c_void_p, C.c_int, C.c_void_p]),
     "bolt_fp4_tile_scales": (C.c_int, [C.POINTER(Fp4TileArgs), C.c_void_p]),
     "bolt_fp4_gemm": (C.c_int, [C.POINTER(Fp4GemmArgs), C.c_void_p]),
+    "bolt_fp4_gemm_few": (C.c_int, [C.POINTER(Fp4FewArgs), C.c_void_p]),
     "bolt_moe_decode_workspace_bytes": (C.c_size_t, [C.POINTER(DecodeArgs)]),
     "bolt_moe_decode": (C.c_int, [C.POINTER(DecodeArgs), C.c_void_p]),
 }

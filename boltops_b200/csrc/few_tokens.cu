@@ -836,6 +836,136 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
 }
 
 // ---------------------------------------------------------------------------
+// dense 4-bit product with a few rows
+// ---------------------------------------------------------------------------
+// The second kernel's work without routing: units of weight rows, every row of x a column.
+struct DenseParams {
+  const uint8_t *x, *x_sf, *w_sf;     // codes [rows, k / 2], scale bytes [rows or n, k / block]
+  const float* alpha;
+  void* out;
+  int out_dtype, rows, n, k, unit, slots_per_warp;
+  int64_t out_ld;
+  int32_t* status;
+};
+
+template <int K, int NT>
+__global__ void __launch_bounds__(32 * warps_of(K, NT), 1)
+k_few_dense(const __grid_constant__ CUtensorMap map, const DenseParams p) {
+  constexpr int MT = kDownTiles, kBox = kDownBoxBytes, kWarps = warps_of(K, NT), kThreads = 32 * kWarps;
+  const int UR = p.unit;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = carve(raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  Ring ring;
+  volatile int* abort_flag = start<kWarps>(ring, smem, p.slots_per_warp, kBox, UR * 128);
+  float* red = reinterpret_cast<float*>(smem + kWarps * p.slots_per_warp * kBox + kCtrlBytes);
+
+  const int units = (p.n + UR - 1) / UR;
+  const int u0 = (int)((int64_t)units * blockIdx.x / gridDim.x);
+  const int u1 = (int)((int64_t)units * (blockIdx.x + 1) / gridDim.x);
+  const int nb = (p.k / 2 + 127) / 128;
+  const int64_t boxes = (int64_t)(u1 - u0) * nb;
+  const int n_it = boxes > warp ? (int)((boxes - warp + kWarps - 1) / kWarps) : 0;
+  struct Place {
+    int u, kb;
+  };
+  auto settle = [&](Place& q) {
+    while (q.kb >= nb) {
+      q.kb -= nb;
+      ++q.u;
+    }
+  };
+  Place in = {u0, warp};
+  int in_it = 0;
+  auto bring = [&]() {
+    settle(in);
+    if (lane == 0) {
+      uint32_t dst;
+      const uint32_t bar = ring.next_in(dst);
+      tma_load_3d(dst, &map, bar, in.kb * 128, in.u * UR, 0);
+    }
+    in.kb += kWarps;
+    ++in_it;
+  };
+  for (int i = 0; i < p.slots_per_warp && in_it < n_it; ++i) bring();
+
+  constexpr int kBlk = K == K_NV4 ? 16 : 32;
+  const int sf_row = p.k / kBlk, row_len = p.k / 2;
+  Place cur = {u0, warp};
+  settle(cur);
+  auto row_scales = [&](RowScales<K>(&ws)[MT], const Place& q) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t row = min(q.u * UR + 16 * mt + 8 * h + g, p.n - 1);
+        load_block_scales<K>(ws[mt].sf[h], p.w_sf + row * sf_row, sf_row, q.kb, t);
+      }
+  };
+  RowScales<K> ws[MT], ws_next[MT];
+  int it = 0;
+  if (n_it > 0) row_scales(ws_next, cur);
+  const unsigned live = (1u << ((p.rows + 7) / 8)) - 1u;
+  const float alpha = p.alpha != nullptr ? *p.alpha : 1.f;
+
+  for (int u = u0; u < u1; ++u) {
+    float acc[MT][NT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[mt][nt][i] = 0.f;
+    while (it < n_it && cur.u == u) {
+      Place nxt = cur;
+      nxt.kb += kWarps;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) ws[mt] = ws_next[mt];
+      if (it + 1 < n_it) {
+        settle(nxt);
+        row_scales(ws_next, nxt);
+      }
+      TokenBox<K> x[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (!((live >> nt) & 1u)) continue;
+        const int m = 8 * nt + g;
+        load_token<K>(x[nt], m < p.rows ? p.x + (int64_t)m * row_len : nullptr, row_len, cur.kb, t);
+        if constexpr (K == K_NV4) {
+          load_block_scales<K>(x[nt].sf, m < p.rows ? p.x_sf + (int64_t)m * sf_row : nullptr, sf_row, cur.kb, t);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int c = 8 * nt + 2 * t + i;
+            load_block_scales<K>(x[nt].sf + 2 * i, c < p.rows ? p.x_sf + (int64_t)c * sf_row : nullptr, sf_row,
+                                 cur.kb, t);
+          }
+        }
+      }
+      const uint32_t box = ring.wait(abort_flag, p.status);
+      box_mma<K, MT, NT, false>(box, 0, lane, x, ws, live, acc);
+      ring.release();
+      if (in_it < n_it) bring();
+      cur = nxt;
+      ++it;
+    }
+    put_sums<MT, NT>(red, acc, warp, lane, live);
+    __syncthreads();
+    for (int i = tid; i < p.rows * kMaxRows; i += kThreads) {
+      const int n = i / kMaxRows, c = i % kMaxRows, col = u * UR + c;
+      if (c >= UR || col >= p.n) continue;
+      const float v = get_sum<kWarps, MT, NT>(red, c >> 4, (c >> 3) & 1, c & 7, n) * alpha;
+      const int64_t at = (int64_t)n * p.out_ld + col;
+      if (p.out_dtype == BOLT_BF16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+      else if (p.out_dtype == BOLT_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
+      else static_cast<float*>(p.out)[at] = v;
+    }
+    __syncthreads();
+  }
+  finish(abort_flag);
+}
+
+// ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -986,6 +1116,33 @@ int launch_kind(const bolt_decode_args* a, const Params& p, cudaStream_t st) {
   return launch<K, 4>(a, p, st);
 }
 
+template <int K, int NT>
+int launch_dense(const bolt_fp4_few_args* a, DenseParams p, int sms, cudaStream_t st) {
+  constexpr int kWarps = warps_of(K, NT);
+  static std::atomic<bool> ready[kMaxDevices];
+  int rc = configure_kernel(k_few_dense<K, NT>, kSmem, ready, 0, 0, 0, 0);
+  if (rc != BOLT_OK) return rc;
+  const int fixed = 1024 + kCtrlBytes + red_bytes(kWarps, kDownTiles, NT);
+  p.slots_per_warp = ring_slots(fixed, kDownBoxBytes, kWarps);
+  p.unit = unit_size(p.n, kMaxRows, 1, sms);
+  const cuuint64_t kb = (cuuint64_t)p.k / 2;
+  const cuuint64_t size[3] = {kb, (cuuint64_t)p.n, 1}, strides[2] = {kb, kb * p.n};
+  const cuuint32_t box[3] = {128, (cuuint32_t)p.unit, 1};
+  CUtensorMap map;
+  if ((rc = encode(&map, a->w, 3, size, strides, box)) != BOLT_OK) return rc;
+  const int units = (p.n + p.unit - 1) / p.unit;
+  k_few_dense<K, NT><<<units < sms ? units : sms, 32 * kWarps, fixed + p.slots_per_warp * kWarps * kDownBoxBytes, st>>>(
+      map, p);
+  BOLT_LAUNCH_CHECK();
+  return BOLT_OK;
+}
+template <int K>
+int launch_dense_kind(const bolt_fp4_few_args* a, const DenseParams& p, int sms, cudaStream_t st) {
+  if (p.rows <= 8) return launch_dense<K, 1>(a, p, sms, st);
+  if (p.rows <= 16) return launch_dense<K, 2>(a, p, sms, st);
+  return launch_dense<K, 4>(a, p, sms, st);
+}
+
 int check_args(const bolt_decode_args* a) {
   BOLT_REQUIRE(a != nullptr, "moe_decode: null args");
   BOLT_REQUIRE(a->kind >= K_BF16 && a->kind <= K_MX4, "moe_decode: unknown kind %d", a->kind);
@@ -1089,4 +1246,38 @@ extern "C" int bolt_moe_decode(const bolt_decode_args* a, void* stream) {
     case K_NV4: return launch_kind<K_NV4>(a, p, st);
     default: return launch_kind<K_MX4>(a, p, st);
   }
+}
+
+extern "C" int bolt_fp4_gemm_few(const bolt_fp4_few_args* a, void* stream) {
+  using namespace bolt;
+  using namespace bolt::few;
+  BOLT_REQUIRE(a != nullptr, "fp4_gemm_few: null args");
+  BOLT_REQUIRE(a->format == BOLT_FP4_NV || a->format == BOLT_FP4_MX, "fp4_gemm_few: unknown format %d", a->format);
+  const bool nv = a->format == BOLT_FP4_NV;
+  BOLT_REQUIRE(a->rows >= 0 && a->rows <= kMaxTokens && a->n >= 0 && a->k > 0 && a->k % (nv ? 64 : 128) == 0,
+               "fp4_gemm_few: %d rows (at most %d) of %d columns (multiples of %d)", a->rows, kMaxTokens, a->k,
+               nv ? 64 : 128);
+  if (a->rows == 0 || a->n == 0) return BOLT_OK;
+  BOLT_REQUIRE(a->x && a->x_scale && a->w && a->w_scale && a->out, "fp4_gemm_few: null pointer");
+  BOLT_REQUIRE(((reinterpret_cast<uintptr_t>(a->x) | reinterpret_cast<uintptr_t>(a->w) |
+                 reinterpret_cast<uintptr_t>(a->x_scale) | reinterpret_cast<uintptr_t>(a->w_scale)) & 15) == 0,
+               "fp4_gemm_few: operands must be 16-byte aligned");
+  BOLT_REQUIRE((a->out_dtype == BOLT_BF16 || a->out_dtype == BOLT_F16 || a->out_dtype == BOLT_F32) &&
+                   a->out_ld >= a->n && reinterpret_cast<uintptr_t>(a->out) % dtype_bytes(a->out_dtype) == 0,
+               "fp4_gemm_few: bad output");
+  DenseParams p = {};
+  p.x = static_cast<const uint8_t*>(a->x);
+  p.x_sf = static_cast<const uint8_t*>(a->x_scale);
+  p.w_sf = static_cast<const uint8_t*>(a->w_scale);
+  p.alpha = a->alpha;
+  p.out = a->out;
+  p.out_dtype = a->out_dtype;
+  p.rows = a->rows;
+  p.n = a->n;
+  p.k = a->k;
+  p.out_ld = a->out_ld;
+  p.status = a->status;
+  const int sms = a->sm_count > 0 ? a->sm_count : sm_count_of_current_device();
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return nv ? launch_dense_kind<K_NV4>(a, p, sms, st) : launch_dense_kind<K_MX4>(a, p, sms, st);
 }

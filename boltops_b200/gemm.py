@@ -103,6 +103,9 @@ w8a8_triton_block_scaled_mm = w8a8_block_scaled_mm
 w8a8_block_int8_matmul = w8a8_block_scaled_mm
 
 
+_FEW_ROWS = 32
+
+
 def gemm_a4w4(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor, w_scale: torch.Tensor,
               alpha: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = torch.bfloat16,
               out: Optional[torch.Tensor] = None):
@@ -146,6 +149,20 @@ def gemm_a4w4(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor, w_scale: 
     if m == 0 or n == 0:
         return out
     x, w, x_scale, w_scale = (ops.aligned(t) for t in (x, w, x_scale, w_scale))
+    lib = _cabi.load()
+    stream = _cabi.stream_of(x)
+    if m <= _FEW_ROWS:
+        few = _cabi.Fp4FewArgs()
+        few.format, few.rows, few.n, few.k = code, m, n, k
+        few.x, few.x_scale, few.w, few.w_scale = (t.data_ptr() for t in (x, x_scale, w, w_scale))
+        few.alpha, few.out, few.out_dtype = _cabi.ptr(alpha), out.data_ptr(), _cabi.dtype_code(dtype)
+        few.out_ld = out.stride(0) if m > 1 else n
+        few.status = ops.device_status(dev).data_ptr()
+        few.sm_count = ops.gemm_sm_count(dev)
+        with _cabi.on_device(dev):
+            _cabi.check(lib.bolt_fp4_gemm_few(few, stream))
+        ops._count()
+        return out
     args = _cabi.Fp4GemmArgs()
     args.format, args.epilogue = code, _cabi.EPI_STORE
     args.rows, args.n, args.k, args.num_experts = m, n, k, 1
@@ -163,8 +180,6 @@ def gemm_a4w4(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor, w_scale: 
     args.c, args.c_dtype, args.c_ld = out.data_ptr(), _cabi.dtype_code(dtype), out.stride(0) if m > 1 else n
     args.status = ops.device_status(dev).data_ptr()
     args.sm_count = ops.gemm_sm_count(dev)
-    lib = _cabi.load()
-    stream = _cabi.stream_of(x)
     with _cabi.on_device(dev):
         _cabi.check(lib.bolt_fp4_tile_scales(lay, stream))
         _cabi.check(lib.bolt_fp4_gemm(args, stream))

@@ -664,6 +664,23 @@ typedef struct bolt_fp4_gemm_args {
 
 int bolt_fp4_gemm(const bolt_fp4_gemm_args* args, void* stream);
 
+/* The dense product for 1 to 32 rows, bound by the weights' bytes: scales as bolt_fp4_quant writes them. */
+typedef struct bolt_fp4_few_args {
+  int format;                  /* enum bolt_fp4_format                                        */
+  int rows, n, k;              /* k a multiple of 64 (NV) or 128 (MX)                         */
+  const void* x;               /* [rows, k / 2]; all operands 16-byte aligned                 */
+  const void* x_scale;
+  const void* w;               /* [n, k / 2]                                                  */
+  const void* w_scale;
+  const float* alpha;          /* optional                                                    */
+  void* out;                   /* [rows, n], rows out_ld elements apart                       */
+  int out_dtype;
+  int64_t out_ld;
+  int32_t* status;             /* optional, set to 30 by a wait that ran out                  */
+  int sm_count;                /* blocks to launch; 0: one per SM                             */
+} bolt_fp4_few_args;
+int bolt_fp4_gemm_few(const bolt_fp4_few_args* args, void* stream);
+
 /* ------------------------------------------------------------------------- */
 /* a whole layer for a few tokens                                             */
 /* ------------------------------------------------------------------------- */
