@@ -54,6 +54,7 @@ struct Params {
   int slots_per_warp;
   int amax_cols;            // units of an expert in the first kernel
   int unit;                 // columns (first kernel) or rows (second) of a unit
+  int group_warps;          // warps that share a unit (first kernel)
 };
 
 // ---------------------------------------------------------------------------
@@ -264,12 +265,12 @@ __device__ __forceinline__ void put_sums(float* red, const float (&acc)[MT][NT][
     }
 }
 // Sum over the warps of element (row half r, row g of tile mt, token n).
-template <int kWarps, int MT, int NT>
-__device__ __forceinline__ float get_sum(const float* red, int mt, int r, int g, int n) {
+template <int MT, int NT>
+__device__ __forceinline__ float get_sum(const float* red, int warps, int mt, int r, int g, int n) {
   const int at = ((mt * NT + (n >> 3)) * 4 + 2 * r + (n & 1)) * 32 + 4 * g + ((n & 7) >> 1);
   float v = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) v += red[w * MT * NT * 128 + at];
+#pragma unroll 4
+  for (int w = 0; w < warps; ++w) v += red[w * MT * NT * 128 + at];
   return v;
 }
 
@@ -317,24 +318,28 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
   const int64_t units = (int64_t)r.touched * per_expert;
   const int u0 = (int)(units * blockIdx.x / gridDim.x), u1 = (int)(units * (blockIdx.x + 1) / gridDim.x);
   const int nb = (int)((row_bytes(K, p.hidden) + 127) / 128);
-  const int64_t boxes = (int64_t)(u1 - u0) * nb;
-  const int n_it = boxes > warp ? (int)((boxes - warp + kWarps - 1) / kWarps) : 0;
 
-  // boxes of this block's units in order, every eighth this warp's
+  // The block's units go to its groups of warps in turn, the boxes of a group's units to its warps.
+  const int per_group = p.group_warps, groups = kWarps / per_group;
+  const int group = warp / per_group, in_group = warp - group * per_group;
   struct Place {
     int u, a, c, kb;      // unit: list[a], columns from c * UC; box of the reduction
   };
   auto settle = [&](Place& q) {
     while (q.kb >= nb) {
       q.kb -= nb;
-      ++q.u;
-      if (++q.c == per_expert) {
-        q.c = 0;
+      q.u += groups;
+      q.c += groups;
+      while (q.c >= per_expert) {
+        q.c -= per_expert;
         ++q.a;
       }
     }
   };
-  Place in = {u0, u0 / per_expert, u0 % per_expert, warp}, cur = in;
+  const int mine = u0 + group < u1 ? (u1 - u0 - group + groups - 1) / groups : 0;     // units of the group
+  const int n_it = mine * nb > in_group ? (mine * nb - in_group + per_group - 1) / per_group : 0;
+  const int first_u = u0 + group;
+  Place in = {first_u, first_u / per_expert, first_u % per_expert, in_group}, cur = in;
   if (n_it > 0) {
     settle(in);
     cur = in;
@@ -347,7 +352,7 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
       const uint32_t bar = ring.next_in(dst);
       tma_load_4d(dst, &map, bar, in.kb * 128, in.c * UC, 0, r.list[in.a]);
     }
-    in.kb += kWarps;
+    in.kb += per_group;
     ++in_it;
   };
   for (int i = 0; i < p.slots_per_warp && in_it < n_it; ++i) bring();
@@ -447,18 +452,22 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
                                    ((e * 2 + h) * p.inter + c0 + 8 * mt + g) * sf1_row,
                                sf1_row, q.kb, t);
     } else if constexpr (is_block(K)) {
-      const uint32_t* s1 = static_cast<const uint32_t*>(p.s1) + e * (2 * p.inter / 128) * (p.hidden / 128) + q.kb;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)     // (columns past the unit's are scaled by anything)
-          ws[mt].sf[h][0] = s1[((h * p.inter + min(c0 + 8 * mt + g, p.inter - 1)) / 128) * (p.hidden / 128)];
+      // (a unit of 8 or 16 columns lies in one block of 128)
+      const uint32_t* s1 = static_cast<const uint32_t*>(p.s1) +
+                           (e * (2 * p.inter / 128) + c0 / 128) * (p.hidden / 128) + q.kb;
+      ws[0].sf[0][0] = s1[0];
+      ws[0].sf[1][0] = s1[(p.inter / 128) * (p.hidden / 128)];
     }
   };
   RowScales<K> ws[MT], ws_next[MT];
   int it = 0;
   if (n_it > 0) row_scales(ws_next, cur);
-  Place unit = {u0, u0 / per_expert, u0 % per_expert, 0};
+  Place unit = {first_u, first_u / per_expert, first_u % per_expert, 0};
+  // (the group's own barrier, named 1 to 8; a warp by itself needs none)
+  auto group_sync = [&]() {
+    if (per_group == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * per_group) : "memory");
+  };
 
   for (; unit.u < u1; unit.kb = nb, settle(unit)) {
     const int e = r.list[unit.a], c0 = unit.c * UC;
@@ -483,7 +492,7 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
     while (it < n_it && cur.u == unit.u) {
       // next box's scales travel while this one is computed
       Place nxt = cur;
-      nxt.kb += kWarps;
+      nxt.kb += per_group;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) ws[mt] = ws_next[mt];
       if (it + 1 < n_it) {
@@ -546,13 +555,14 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
             x0 = __shfl_sync(0xffffffffu, xs, 8 * nt + 2 * t);
             x1 = __shfl_sync(0xffffffffu, xs, 8 * nt + 2 * t + 1);
           }
+          const float sg = __uint_as_float(ws[0].sf[0][0]), su = __uint_as_float(ws[0].sf[1][0]);
+          const float s0g = x0 * sg, s1g = x1 * sg, s0u = x0 * su, s1u = x1 * su;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            const float sg = __uint_as_float(ws[mt].sf[0][0]), su = __uint_as_float(ws[mt].sf[1][0]);
-            acc[mt][nt][0] = fmaf(part[mt][nt][0], x0 * sg, acc[mt][nt][0]);
-            acc[mt][nt][1] = fmaf(part[mt][nt][1], x1 * sg, acc[mt][nt][1]);
-            acc[mt][nt][2] = fmaf(part[mt][nt][2], x0 * su, acc[mt][nt][2]);
-            acc[mt][nt][3] = fmaf(part[mt][nt][3], x1 * su, acc[mt][nt][3]);
+            acc[mt][nt][0] = fmaf(part[mt][nt][0], s0g, acc[mt][nt][0]);
+            acc[mt][nt][1] = fmaf(part[mt][nt][1], s1g, acc[mt][nt][1]);
+            acc[mt][nt][2] = fmaf(part[mt][nt][2], s0u, acc[mt][nt][2]);
+            acc[mt][nt][3] = fmaf(part[mt][nt][3], s1u, acc[mt][nt][3]);
           }
         }
       } else {
@@ -566,16 +576,17 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
 
     // ---- sums over the warps, activation, Q2 of the 4-bit kinds ----
     put_sums<MT, NT>(red, acc, warp, lane, live);
-    __syncthreads();
+    group_sync();
+    const float* mine_red = red + group * per_group * MT * NT * 128;
     const int all = ((cnt * kCols + 31) / 32) * 32;      // whole warps take part in the exchanges
-    for (int i = tid; i < all; i += kThreads) {
+    for (int i = in_group * 32 + lane; i < all; i += 32 * per_group) {
       const int n = i / kCols, c = i % kCols, col = c0 + c;
       const bool have = n < cnt && c < UC && col < p.inter;
       const int slot = off + n;
       float a = 0.f;
       if (have) {
-        float gate = get_sum<kWarps, MT, NT>(red, c >> 3, 0, c & 7, n);
-        float up = get_sum<kWarps, MT, NT>(red, c >> 3, 1, c & 7, n);
+        float gate = get_sum<MT, NT>(mine_red, per_group, c >> 3, 0, c & 7, n);
+        float up = get_sum<MT, NT>(mine_red, per_group, c >> 3, 1, c & 7, n);
         if constexpr (is_channel(K)) {
           const float* s1 = static_cast<const float*>(p.s1) + (int64_t)e * 2 * p.inter;
           const float xsc = row_scale[2 * r.token[slot]];
@@ -617,7 +628,7 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
         if (have && c == 0) p.act_sf[(int64_t)slot * (p.inter / kBlk) + col / kBlk] = (uint8_t)byte;
       }
     }
-    __syncthreads();
+    group_sync();
   }
   finish(abort_flag);
 }
@@ -685,21 +696,23 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
   if (n_it > 0) settle(cur);
   auto row_scales = [&](RowScales<K>(&ws)[MT], const Place& q) {
     const int64_t e = r.list[q.a];
+    // (rows past the unit's are scaled by anything: they go nowhere)
+    const int row0 = q.u * UR + g, last = p.model_dim - 1;
+    if constexpr (is_block(K)) {
+      const int per = p.inter / 128;
+      const uint32_t* s2 = static_cast<const uint32_t*>(p.s2) + e * (p.model_dim / 128) * per + q.kb;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+      for (int i = 0; i < 2 * MT; ++i) ws[i >> 1].sf[i & 1][0] = s2[(min(row0 + 8 * i, last) >> 7) * per];
+    } else if constexpr (is_channel(K)) {
+      const uint32_t* s2 = static_cast<const uint32_t*>(p.s2) + e * p.model_dim;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        // (rows past the unit's are scaled by anything: they go nowhere)
-        const int row = min(q.u * UR + 16 * mt + 8 * h + g, p.model_dim - 1);
-        if constexpr (is4(K))
-          load_block_scales<K>(ws[mt].sf[h], static_cast<const uint8_t*>(p.s2) + (e * p.model_dim + row) * sf_row,
-                               sf_row, q.kb, t);
-        else if constexpr (is_block(K))
-          ws[mt].sf[h][0] = static_cast<const uint32_t*>(
-              p.s2)[(e * (p.model_dim / 128) + row / 128) * (p.inter / 128) + q.kb];
-        else if constexpr (is_channel(K))
-          ws[mt].sf[h][0] = static_cast<const uint32_t*>(p.s2)[e * p.model_dim + row];
-      }
+      for (int i = 0; i < 2 * MT; ++i) ws[i >> 1].sf[i & 1][0] = s2[min(row0 + 8 * i, last)];
+    } else if constexpr (is4(K)) {
+      const uint8_t* s2 = static_cast<const uint8_t*>(p.s2) + e * p.model_dim * sf_row;
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i)
+        load_block_scales<K>(ws[i >> 1].sf[i & 1], s2 + (int64_t)min(row0 + 8 * i, last) * sf_row, sf_row, q.kb, t);
+    }
   };
   RowScales<K> ws[MT], ws_next[MT];
   int it = 0;
@@ -824,7 +837,7 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
     for (int i = tid; i < p.tokens * kMaxRows; i += kThreads) {
       const int n = i / kMaxRows, c = i % kMaxRows, col = u * UR + c;
       if (c >= UR || col >= p.model_dim) continue;
-      const float v = get_sum<kWarps, MT, NT>(red, c >> 4, (c >> 3) & 1, c & 7, n) * p.out_scale;
+      const float v = get_sum<MT, NT>(red, kWarps, c >> 4, (c >> 3) & 1, c & 7, n) * p.out_scale;
       const int64_t at = (int64_t)n * p.model_dim + col;
       if (p.out_dtype == BOLT_BF16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
       else if (p.out_dtype == BOLT_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
@@ -954,7 +967,7 @@ k_few_dense(const __grid_constant__ CUtensorMap map, const DenseParams p) {
     for (int i = tid; i < p.rows * kMaxRows; i += kThreads) {
       const int n = i / kMaxRows, c = i % kMaxRows, col = u * UR + c;
       if (c >= UR || col >= p.n) continue;
-      const float v = get_sum<kWarps, MT, NT>(red, c >> 4, (c >> 3) & 1, c & 7, n) * alpha;
+      const float v = get_sum<MT, NT>(red, kWarps, c >> 4, (c >> 3) & 1, c & 7, n) * alpha;
       const int64_t at = (int64_t)n * p.out_ld + col;
       if (p.out_dtype == BOLT_BF16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
       else if (p.out_dtype == BOLT_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
@@ -1009,10 +1022,10 @@ inline int a16(int n) { return (n + 15) & ~15; }
 constexpr int kMinUnit = 8;
 // Size of a unit, of 8 to `most`: every block gets the same number of units but for one, so the one that
 // makes the largest share smallest (of two alike the larger; a unit costs about a row's time by itself).
-int unit_size(int total, int most, int64_t copies, int blocks) {
+int unit_size(int total, int most, int64_t copies, int blocks, int step = 1) {
   int best = most;
   int64_t least = INT64_MAX;
-  for (int u = most; u >= kMinUnit; --u) {
+  for (int u = most; u >= kMinUnit; u -= step) {
     const int64_t units = copies * ((total + u - 1) / u);
     const int64_t share = (units + blocks - 1) / blocks * (u + 1);
     if (share < least) {
@@ -1021,6 +1034,13 @@ int unit_size(int total, int most, int64_t copies, int blocks) {
     }
   }
   return best;
+}
+
+// Warps to a unit: as many as have four boxes of its reduction each.  With fewer boxes a warp, the end of
+// a unit (sums over the warps, activation) is not covered by other units' copies.
+int group_warps(int warps, int boxes) {
+  while (warps > 1 && boxes < 4 * warps) warps /= 2;
+  return warps;
 }
 
 // bytes of the three parts of the workspace
@@ -1071,7 +1091,8 @@ int launch(const bolt_decode_args* a, Params p, cudaStream_t st) {
   const int sms = a->sm_count > 0 ? a->sm_count : sm_count_of_current_device();
   const int64_t routes = (int64_t)p.tokens * p.topk;
   const int columns = is4(K) ? 8 * up_tiles(K)
-                             : unit_size(p.inter, 8 * up_tiles(K), routes < p.experts ? routes : p.experts, sms);
+                             : unit_size(p.inter, 8 * up_tiles(K), routes < p.experts ? routes : p.experts, sms,
+                                         is_block(K) ? 8 : 1);
   const int rows = unit_size(p.model_dim, kMaxRows, 1, sms);
   CUtensorMap m1, m2;
   {
@@ -1091,6 +1112,7 @@ int launch(const bolt_decode_args* a, Params p, cudaStream_t st) {
   p.amax_cols = (p.inter + columns - 1) / columns;
   p.slots_per_warp = up_slots;
   p.unit = columns;
+  p.group_warps = group_warps(kWarps, (int)((row_bytes(K, p.hidden) + 127) / 128));
   k_few_up<K, NT><<<sms, 32 * kWarps, up + up_slots * kWarps * up_box_bytes(K), st>>>(m1, p);
   BOLT_LAUNCH_CHECK();
   p.slots_per_warp = down_slots;
