@@ -55,23 +55,25 @@ struct Params {
   int amax_cols;            // units of an expert in the first kernel
   int unit;                 // columns (first kernel) or rows (second) of a unit
   int group_warps;          // warps that share a unit (first kernel)
+  int keep_act;             // codes of the activations are kept in shared memory (second kernel)
 };
 
 // ---------------------------------------------------------------------------
 // routing
 // ---------------------------------------------------------------------------
+// The touched experts in ascending order, a slot for every (expert, token) in that order.
 struct Routes {
-  uint32_t* mask;   // [experts] tokens of an expert
-  int* off;         // [experts] slot of its first token: slots go by (expert, token)
-  int* list;        // touched experts, ascending
+  int* list;        // [touched] expert
+  uint32_t* mask;   // [touched] its tokens
+  int* off;         // [touched] slot of its first token
   float* coef;      // [slots] router weight (of all routes of a token to the expert)
   int* token;       // [slots]
-  int* ids;         // [routes] local expert or -1
-  float* wts;       // [routes]
-  int touched;
+  int touched, slots;
 };
+// shared memory of it: per touched expert (at most one a route) 3 words, per slot 2, per route 2, and the
+// masks of all experts where the routes are more than a warp has lanes
 __host__ __device__ inline int route_bytes(int experts, int routes) {
-  return 4 * (3 * experts + 4 * routes) + 64;
+  return 4 * (7 * routes + (routes > 32 ? experts : 0)) + 64;
 }
 
 template <int NPL>
@@ -101,15 +103,18 @@ __device__ void build_routes(const Params& p, Routes& r, uint8_t* mem) {
   constexpr int kThreads = 32 * kWarps;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int routes = p.tokens * p.topk, experts = p.experts;
-  r.mask = reinterpret_cast<uint32_t*>(mem);
-  r.off = reinterpret_cast<int*>(r.mask + experts);
-  r.list = r.off + experts;
-  r.coef = reinterpret_cast<float*>(r.list + experts);
+  r.list = reinterpret_cast<int*>(mem);
+  r.mask = reinterpret_cast<uint32_t*>(r.list + routes);
+  r.off = reinterpret_cast<int*>(r.mask + routes);
+  r.coef = reinterpret_cast<float*>(r.off + routes);
   r.token = reinterpret_cast<int*>(r.coef + routes);
-  r.ids = r.token + routes;
-  r.wts = reinterpret_cast<float*>(r.ids + routes);
-  int* totals = reinterpret_cast<int*>(r.wts + routes);   // [16] per warp
-  for (int e = tid; e < experts; e += kThreads) r.mask[e] = 0;
+  int* ids = r.token + routes;                               // [routes] local expert or -1
+  float* wts = reinterpret_cast<float*>(ids + routes);       // [routes]
+  int* totals = reinterpret_cast<int*>(wts + routes);        // [16]
+  uint32_t* mask = reinterpret_cast<uint32_t*>(totals + 16); // [experts]
+  const bool small = routes <= 32;
+  if (!small)
+    for (int e = tid; e < experts; e += kThreads) mask[e] = 0;
   if (p.gating != nullptr) {
     const int size = p.gating_dtype == BOLT_F32 ? 4 : 2;
     const int npl = (p.global_experts + 31) / 32;
@@ -122,25 +127,76 @@ __device__ void build_routes(const Params& p, Routes& r, uint8_t* mem) {
       else if (npl <= 8) route_token<8>(row, p.gating_dtype, p.global_experts, p.topk, p.renormalize, p.softmax, lane, w, id);
       else route_token<32>(row, p.gating_dtype, p.global_experts, p.topk, p.renormalize, p.softmax, lane, w, id);
       if (lane < p.topk) {
-        r.ids[m * p.topk + lane] = local_expert(p, id);
-        r.wts[m * p.topk + lane] = w;
+        ids[m * p.topk + lane] = local_expert(p, id);
+        wts[m * p.topk + lane] = w;
       }
     }
-  } else {
-    for (int i = tid; i < routes; i += kThreads) {
-      r.ids[i] = local_expert(p, p.ids[i]);
-      r.wts[i] = p.wts[i];
-    }
+    __syncthreads();
   }
+  if (small) {
+    // one warp, a route a lane
+    if (warp == 0) {
+      int e = -1;
+      float w = 0.f;
+      if (lane < routes) {
+        e = p.gating != nullptr ? ids[lane] : local_expert(p, p.ids[lane]);
+        w = p.gating != nullptr ? wts[lane] : p.wts[lane];
+      }
+      const int m = lane / p.topk;
+      // routes of the same token to the same expert are one slot, the first of them its owner
+      const unsigned same = __match_any_sync(0xffffffffu, e);
+      const unsigned row = p.topk == 32 ? ~0u : ((1u << p.topk) - 1u) << (m * p.topk);
+      const unsigned twins = e >= 0 ? same & row : 0u;
+      const bool owner = e >= 0 && lane == __ffs(twins) - 1;
+      const bool leads = e >= 0 && lane == __ffs(same) - 1;          // of its expert
+      float sum = 0.f;
+      int before = 0, lower = 0;      // slots in front of this one, touched experts below this one
+      uint32_t tokens = 0;
+#pragma unroll 4
+      for (int j = 0; j < routes; ++j) {
+        const int ej = __shfl_sync(0xffffffffu, e, j);
+        const float wj = __shfl_sync(0xffffffffu, w, j);
+        const bool own = __shfl_sync(0xffffffffu, (int)owner, j) != 0, lead = __shfl_sync(0xffffffffu, (int)leads, j) != 0;
+        if ((twins >> j) & 1u) sum += wj;
+        if (own && (ej < e || (ej == e && j < lane))) ++before;
+        if (lead && ej < e) ++lower;
+        if (ej == e) tokens |= 1u << (j / p.topk);
+      }
+      if (owner) {
+        r.coef[before] = sum;
+        r.token[before] = m;
+      }
+      if (leads) {
+        r.list[lower] = e;
+        r.mask[lower] = tokens;
+        r.off[lower] = before;
+      }
+      const unsigned leaders = __ballot_sync(0xffffffffu, leads), owners = __ballot_sync(0xffffffffu, owner);
+      if (lane == 0) {
+        totals[0] = __popc(leaders);
+        totals[1] = __popc(owners);
+      }
+    }
+    __syncthreads();
+    r.touched = totals[0];
+    r.slots = totals[1];
+    return;
+  }
+  if (p.gating == nullptr)
+    for (int i = tid; i < routes; i += kThreads) {
+      ids[i] = local_expert(p, p.ids[i]);
+      wts[i] = p.wts[i];
+    }
   __syncthreads();
   for (int i = tid; i < routes; i += kThreads)
-    if (r.ids[i] >= 0) atomicOr(&r.mask[r.ids[i]], 1u << (i / p.topk));
+    if (ids[i] >= 0) atomicOr(&mask[ids[i]], 1u << (i / p.topk));
   __syncthreads();
   // exclusive sums over the experts: tokens (low half), touched experts (high half)
   int base = 0;
   for (int e0 = 0; e0 < experts; e0 += kThreads) {
     const int e = e0 + tid;
-    const int c = e < experts ? __popc(r.mask[e]) : 0;
+    const uint32_t tokens = e < experts ? mask[e] : 0u;
+    const int c = __popc(tokens);
     const int mine = c | (c > 0 ? 0x10000 : 0);
     int sum = mine;
 #pragma unroll
@@ -157,25 +213,31 @@ __device__ void build_routes(const Params& p, Routes& r, uint8_t* mem) {
       all += totals[w];
     }
     before += sum - mine;
-    if (e < experts) {
-      r.off[e] = before & 0xFFFF;
-      if (c > 0) r.list[before >> 16] = e;
+    if (c > 0) {
+      const int at = before >> 16;
+      r.list[at] = e;
+      r.mask[at] = tokens;
+      r.off[at] = before & 0xFFFF;
+      mask[e] = at;               // from here on: the expert's place in the list
     }
     base += all;
     __syncthreads();
   }
   r.touched = base >> 16;
+  r.slots = base & 0xFFFF;
   for (int i = tid; i < routes; i += kThreads) {
-    const int e = r.ids[i];
+    const int e = ids[i];
     if (e < 0) continue;
     const int m = i / p.topk, first = m * p.topk, last = first + p.topk;
     bool again = false;
-    for (int j = first; j < i; ++j) again |= r.ids[j] == e;
-    if (again) continue;       // the same expert twice for a token: one slot, the weights' sum
     float w = 0.f;
-    for (int j = i; j < last; ++j)
-      if (r.ids[j] == e) w += r.wts[j];
-    const int slot = r.off[e] + __popc(r.mask[e] & ((1u << m) - 1u));
+    for (int j = first; j < last; ++j) {
+      const bool same = ids[j] == e;
+      again |= same && j < i;
+      if (same) w += wts[j];
+    }
+    if (again) continue;       // the same expert twice for a token: one slot, the weights' sum
+    const int at = mask[e], slot = r.off[at] + __popc(r.mask[at] & ((1u << m) - 1u));
     r.coef[slot] = w;
     r.token[slot] = m;
   }
@@ -471,8 +533,7 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
 
   for (; unit.u < u1; unit.kb = nb, settle(unit)) {
     const int e = r.list[unit.a], c0 = unit.c * UC;
-    const uint32_t mask = r.mask[e];
-    const int off = r.off[e], cnt = __popc(mask);
+    const int off = r.off[unit.a], cnt = __popc(r.mask[unit.a]);
     const unsigned live = (1u << ((cnt + 7) / 8)) - 1u;
     const uint32_t live_cols = cnt == 32 ? ~0u : (1u << cnt) - 1u;
     float acc[MT][NT][4];
@@ -722,18 +783,37 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
   float* row_scale = reinterpret_cast<float*>(rest);       // [slots][2]
   if constexpr (is_channel(K)) {
     const int per_expert = p.amax_cols;
-    int slots = 0;
-    if (r.touched > 0) {
-      const int last = r.list[r.touched - 1];
-      slots = r.off[last] + __popc(r.mask[last]);
-    }
-    for (int s = warp; s < slots; s += kWarps) {
+    for (int s = warp; s < r.slots; s += kWarps) {
       float amax = 0.f;
       for (int i = lane; i < per_expert; i += 32) amax = fmaxf(amax, p.act_amax[(int64_t)s * per_expert + i]);
       for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
       if (lane == 0) scale8<K>(amax, row_scale[2 * s], row_scale[2 * s + 1]);
     }
     __syncthreads();
+  }
+
+  // 8-bit codes of all slots, made once where they fit beside the rings
+  uint8_t* a_codes = rest + (is_channel(K) ? (8 * p.tokens * p.topk + 15) & ~15 : 0);
+  const int a_pitch = code_pitch(K, p.inter);
+  float* a_scale = reinterpret_cast<float*>(a_codes + p.tokens * p.topk * a_pitch);     // [slots][boxes]
+  if constexpr (keeps_codes(K, NT)) {
+    if (p.keep_act) {
+      for (int i = warp; i < r.slots * nb; i += kWarps) {
+        const int s = i / nb, kb = i - s * nb, c = kb * 128 + 4 * lane;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < p.inter) v = load_values4(reinterpret_cast<const float*>(p.act_rows) + (int64_t)s * p.inter, BOLT_F32, c);
+        float scale, inv;
+        if constexpr (is_block(K)) {
+          const float top = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+          scale8<K>(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))), scale, inv);
+          if (lane == 0) a_scale[i] = scale;
+        } else {
+          inv = row_scale[2 * s + 1];
+        }
+        if (c < p.inter) *reinterpret_cast<uint32_t*>(a_codes + s * a_pitch + c) = codes4<K>(v, inv);
+      }
+      __syncthreads();
+    }
   }
 
   for (int u = u0; u < u1; ++u) {
@@ -756,15 +836,19 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
       }
 
       const int e = r.list[cur.a], kb = cur.kb;
-      const uint32_t mask = r.mask[e];
-      const int off = r.off[e];
+      const uint32_t mask = r.mask[cur.a];
+      const int off = r.off[cur.a];
       unsigned live = 0;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) live |= ((mask >> (8 * nt)) & 0xFFu) != 0u ? 1u << nt : 0u;
 
       TokenBox<K> x[NT];
       float xs = 1.f;
-      if constexpr (is8(K)) {
+      const bool kept = keeps_codes(K, NT) && p.keep_act;
+      if (kept) {
+        const int slot = slot_of(mask, off, g);
+        load_token<K>(x[0], slot < 0 ? nullptr : a_codes + slot * a_pitch, p.inter, kb, t);
+      } else if constexpr (is8(K)) {
         xs = quant_box<K, NT>(
             x, stage, mask, BOLT_F32, p.inter, kb * 128, lane,
             [&](int c) {
@@ -806,7 +890,7 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
       for (int nt = 0; nt < NT; ++nt) {
         if (!((live >> nt) & 1u)) continue;
         float s01[2] = {1.f, 1.f};
-        if constexpr (is_block(K)) {
+        if (is_block(K) && !kept) {
           s01[0] = __shfl_sync(0xffffffffu, xs, 8 * nt + 2 * t);
           s01[1] = __shfl_sync(0xffffffffu, xs, 8 * nt + 2 * t + 1);
         }
@@ -816,6 +900,7 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
           const int slot = slot_of(mask, off, 8 * nt + 2 * t + i);
           if (slot < 0) continue;
           float f = r.coef[slot] * s01[i] * whole;
+          if (is_block(K) && kept) f *= a_scale[slot * nb + kb];
           if constexpr (is_channel(K)) f *= row_scale[2 * slot];
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
@@ -1053,6 +1138,7 @@ void workspace_parts(const bolt_decode_args* a, size_t (&part)[3]) {
 }
 
 constexpr int kSmem = 226 * 1024;   // of a block
+constexpr int kKeepBytes = 64 * 1024;
 int ring_slots(int fixed, int box_bytes, int warps) {
   int slots = (kSmem - fixed) / (warps * box_bytes);
   return slots * warps > kMaxBarriers ? kMaxBarriers / warps : slots;
@@ -1077,7 +1163,14 @@ int launch(const bolt_decode_args* a, Params p, cudaStream_t st) {
     if (up_slots < 1 && keeps_codes(K, NT)) return launch<K, 2 * NT>(a, p, st);
   int down = 1024 + kCtrlBytes + red_bytes(kWarps, kDownTiles, NT) + a16(route_bytes(p.experts, p.tokens * p.topk));
   if (is8(K)) down += kWarps * code_bytes(NT);
-  if (is_channel(K)) down += 8 * p.tokens * p.topk;
+  if (is_channel(K)) down += a16(8 * p.tokens * p.topk);
+  if (keeps_codes(K, NT)) {
+    // up to kKeepBytes of them: beyond, the rings would shrink
+    const int64_t bytes = (int64_t)p.tokens * p.topk *
+                          (code_pitch(K, p.inter) + (is_block(K) ? p.inter / 128 * 4 : 0));
+    p.keep_act = bytes <= kKeepBytes ? 1 : 0;
+    if (p.keep_act) down += a16((int)bytes);
+  }
   const int down_slots = ring_slots(down, kDownBoxBytes, kWarps);
   if (up_slots < 1 || down_slots < 1) {
     set_error("moe_decode: %d tokens of hidden size %d do not fit in shared memory", p.tokens, p.hidden);
