@@ -98,8 +98,9 @@ __device__ __forceinline__ int local_expert(const Params& p, int id) {
   return e >= 0 && e < p.experts ? e : -1;
 }
 
-template <int kWarps>
-__device__ void build_routes(const Params& p, Routes& r, uint8_t* mem) {
+// `work(warp, warps)`: what else has to be done in front, by warps that routing does not need.
+template <int kWarps, typename Work>
+__device__ __forceinline__ void build_routes(const Params& p, Routes& r, uint8_t* mem, Work work) {
   constexpr int kThreads = 32 * kWarps;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int routes = p.tokens * p.topk, experts = p.experts;
@@ -112,13 +113,15 @@ __device__ void build_routes(const Params& p, Routes& r, uint8_t* mem) {
   float* wts = reinterpret_cast<float*>(ids + routes);       // [routes]
   int* totals = reinterpret_cast<int*>(wts + routes);        // [16]
   uint32_t* mask = reinterpret_cast<uint32_t*>(totals + 16); // [experts]
-  const bool small = routes <= 32;
+  const bool small = routes <= 32, one_warp = small && (p.gating == nullptr || p.tokens == 1);
+  if (!one_warp) work(warp, kWarps);
+  else if (warp > 0) work(warp - 1, kWarps - 1);
   if (!small)
     for (int e = tid; e < experts; e += kThreads) mask[e] = 0;
-  if (p.gating != nullptr) {
+  if (p.gating != nullptr && (!one_warp || warp == 0)) {
     const int size = p.gating_dtype == BOLT_F32 ? 4 : 2;
     const int npl = (p.global_experts + 31) / 32;
-    for (int m = warp; m < p.tokens; m += kWarps) {
+    for (int m = one_warp ? 0 : warp; m < p.tokens; m += kWarps) {
       const void* row = static_cast<const uint8_t*>(p.gating) + (int64_t)m * p.global_experts * size;
       float w;
       int id;
@@ -131,7 +134,8 @@ __device__ void build_routes(const Params& p, Routes& r, uint8_t* mem) {
         wts[m * p.topk + lane] = w;
       }
     }
-    __syncthreads();
+    if (one_warp) __syncwarp();
+    else __syncthreads();
   }
   if (small) {
     // one warp, a route a lane
@@ -264,12 +268,14 @@ struct Ring {
     bytes = box_bytes;
   }
   // lane 0 only: the barrier and the address of the next box to bring
-  __device__ __forceinline__ uint32_t next_in(uint32_t& dst) {
+  __device__ __forceinline__ uint32_t next_in(uint32_t& dst) const {
     const uint32_t bar = bars + 8 * s_in;
     dst = base + s_in * bytes;
     mbar_expect_tx(bar, bytes_in);
-    if (++s_in == slots) s_in = 0;
     return bar;
+  }
+  __device__ __forceinline__ void advance_in() {
+    if (++s_in == slots) s_in = 0;
   }
   __device__ __forceinline__ uint32_t wait(volatile int* abort_flag, int32_t* status) {
     mbar_wait(bars + 8 * s_out, ph, abort_flag, status, 30);
@@ -289,6 +295,13 @@ constexpr int kMaxBarriers = 126;  // 8 bytes each
 
 __device__ __forceinline__ uint8_t* carve(uint8_t* raw) {
   return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+}
+
+// This block's run of `units`: the first units % blocks blocks have one more.
+__device__ __forceinline__ void share_of(int units, int& first, int& end) {
+  const int each = units / (int)gridDim.x, more = units - each * (int)gridDim.x, b = (int)blockIdx.x;
+  first = b * each + min(b, more);
+  end = first + each + (b < more ? 1 : 0);
 }
 
 // What both kernels begin with: barriers, the ring.
@@ -344,6 +357,9 @@ constexpr int up_tiles(int k) { return k == K_MX4 ? 4 : 2; }
 constexpr int up_box_bytes(int k) { return up_tiles(k) * 2048; }
 constexpr int kDownTiles = kMaxRows / 16;
 constexpr int kDownBoxBytes = kMaxRows * 128;
+constexpr int up_scale_bytes(int k) {      // of a slot
+  return k == K_NV4 ? 512 : k == K_MX4 ? 512 : is_block(k) ? 64 : 0;
+}
 constexpr int warps_of(int k, int nt) { return nt == 4 || k == K_MX4 ? 8 : 16; }
 constexpr int red_bytes(int warps, int mt, int nt) { return warps * mt * nt * 128 * 4; }
 // 8-bit kinds, up to eight tokens: the rows' codes are made once and kept
@@ -359,10 +375,14 @@ __global__ void __launch_bounds__(32 * warps_of(K, NT), 1)
 k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
   constexpr int MT = up_tiles(K), kBox = up_box_bytes(K), kWarps = warps_of(K, NT), kThreads = 32 * kWarps;
   constexpr int kCols = 8 * MT;       // columns a unit may have
+  // rows of scales: of every gate and up row of a thread (4-bit), of the unit's gate and up block
+  using Scales = ScaleRing<is_channel(K) ? (int)K_BF16 : K, is4(K) ? 2 * MT : 2>;
+  static_assert(Scales::kBytes == up_scale_bytes(K), "the host reckons with a slot of this size");
   const int UC = is4(K) ? kCols : p.unit;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = carve(raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  if (tid == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
   Ring ring;
   volatile int* abort_flag = start<kWarps>(ring, smem, p.slots_per_warp, kBox, 2 * UC * 128);
   uint8_t* rest = smem + kWarps * p.slots_per_warp * kBox + kCtrlBytes;
@@ -372,13 +392,100 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
   if (is8(K) && !keeps_codes(K, NT)) rest += kWarps * code_bytes(NT);
   let_next_start();
 
-  Routes r;
-  build_routes<kWarps>(p, r, rest);
+  uint8_t* const route_mem = rest;
   rest += (route_bytes(p.experts, p.tokens * p.topk) + 15) & ~15;
+  const uint32_t scale_mem = smem_u32(rest);
+  rest += kWarps * p.slots_per_warp * Scales::kBytes;
+  float* row_scale = reinterpret_cast<float*>(rest);       // [tokens][2]: scale, reciprocal
+  if (is_channel(K)) rest += (8 * p.tokens + 15) & ~15;
+  uint8_t* x_codes = rest;                                 // [tokens][pitch], scales behind them
+  const int pitch = code_pitch(K, p.hidden);
+  uint8_t* x_sf = x_codes + p.tokens * pitch;              // 4-bit: bytes
+  float* x_scale = reinterpret_cast<float*>(x_sf);         // block-scaled: [hidden / 128][8]
+  constexpr int kBlk = K == K_NV4 ? 16 : 32;
+  const int sf_row = p.hidden / kBlk;
+
+  // Q1 that needs whole rows, once per block.  In front of the first weights' copies: behind them a load
+  // waits until they have all come.
+  auto quantise = [&](int w0, int wn) {
+    if constexpr (is_channel(K)) {
+      for (int m = w0; m < p.tokens; m += wn) {
+        const uint16_t* row = static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden;
+        float amax = 0.f;
+#pragma unroll 4
+        for (int c = lane * 8; c < p.hidden; c += 256) {
+          const uint4 u = *reinterpret_cast<const uint4*>(row + c);
+          const uint32_t q[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (p.x_dtype == BOLT_BF16) {
+              amax = fmaxf(amax, fabsf(__uint_as_float(q[j] << 16)));
+              amax = fmaxf(amax, fabsf(__uint_as_float(q[j] & 0xFFFF0000u)));
+            } else {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q[j]));
+              amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          }
+        }
+        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if (lane == 0) scale8<K>(amax, row_scale[2 * m], row_scale[2 * m + 1]);
+      }
+      if (keeps_codes(K, NT)) asm volatile("bar.sync 15, %0;" ::"r"(32 * wn) : "memory");
+    }
+    if constexpr (keeps_codes(K, NT)) {
+      // a warp per group of 128 values
+      const int per_row = (p.hidden + 127) / 128;
+#pragma unroll 4
+      for (int i = w0; i < p.tokens * per_row; i += wn) {
+        const int m = i / per_row, kb = i - m * per_row, c = kb * 128 + 4 * lane;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < p.hidden) v = load_values4(static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden, p.x_dtype, c);
+        float scale, inv;
+        if constexpr (is_block(K)) {
+          const float top = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+          scale8<K>(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))), scale, inv);
+          if (lane == 0) x_scale[kb * 8 + m] = scale;
+        } else {
+          inv = row_scale[2 * m + 1];
+        }
+        if (c < p.hidden) *reinterpret_cast<uint32_t*>(x_codes + m * pitch + c) = codes4<K>(v, inv);
+      }
+    }
+    if constexpr (is4(K)) {
+      const bool nv = K == K_NV4;
+      const float inv_g = p.a1 != nullptr ? __frcp_rn(*p.a1) : 1.f;
+      const int per_row = p.hidden / 32;
+      for (int i = w0 * 32 + lane; i < p.tokens * per_row; i += wn * 32) {
+        const int m = i / per_row, c = (i - m * per_row) * 32;
+        float v[32];
+        load_values32(v, static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden, p.x_dtype, c);
+        if (nv && p.a1 != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= inv_g;
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int b = 0; b < 32 / kBlk; ++b) {
+          float amax = 0.f;
+#pragma unroll
+          for (int j = 0; j < kBlk; ++j) amax = fp4::amax_nan(amax, v[b * kBlk + j]);
+          const uint32_t byte = fp4::scale_byte<K == K_NV4>(amax);
+          const fp4::Scaler sc = fp4::scaler_of<K == K_NV4>(byte);
+#pragma unroll
+          for (int j = 0; j < kBlk / 8; ++j)
+            w[b * (kBlk / 8) + j] = fp4::codes8<K == K_NV4>(v + b * kBlk + 8 * j, sc);
+          x_sf[(int64_t)m * sf_row + c / kBlk + b] = (uint8_t)byte;
+        }
+        *reinterpret_cast<uint4*>(x_codes + m * pitch + c / 2) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  };
+  Routes r;
+  build_routes<kWarps>(p, r, route_mem, quantise);
 
   const int per_expert = (p.inter + UC - 1) / UC;
-  const int64_t units = (int64_t)r.touched * per_expert;
-  const int u0 = (int)(units * blockIdx.x / gridDim.x), u1 = (int)(units * (blockIdx.x + 1) / gridDim.x);
+  int u0, u1;
+  share_of(r.touched * per_expert, u0, u1);
   const int nb = (int)((row_bytes(K, p.hidden) + 127) / 128);
 
   // The block's units go to its groups of warps in turn, the boxes of a group's units to its warps.
@@ -407,123 +514,36 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
     cur = in;
   }
   int in_it = 0;
+  const Scales scales = {scale_mem + (uint32_t)(warp * p.slots_per_warp) * Scales::kBytes};
+  // the next box and its scales; past the last an empty group, so that groups stay one a box
   auto bring = [&]() {
-    settle(in);
-    if (lane == 0) {
-      uint32_t dst;
-      const uint32_t bar = ring.next_in(dst);
-      tma_load_4d(dst, &map, bar, in.kb * 128, in.c * UC, 0, r.list[in.a]);
+    if (in_it < n_it) {
+      settle(in);
+      const int e = r.list[in.a], c0 = in.c * UC;
+      if (lane == 0) {
+        uint32_t dst;
+        const uint32_t bar = ring.next_in(dst);
+        tma_load_4d(dst, &map, bar, in.kb * 128, c0, 0, e);
+      }
+      if constexpr (is4(K)) {
+        const uint8_t* s1 = static_cast<const uint8_t*>(p.s1) + ((int64_t)e * 2 * p.inter + c0 + g) * sf_row;
+        const int half = p.inter * sf_row;
+        scales.bring(ring.s_in, lane, in.kb, sf_row, [&](int i) { return s1 + (i & 1) * half + 8 * (i >> 1) * sf_row; });
+      } else if constexpr (is_block(K)) {
+        // (a unit of 8 or 16 columns lies in one block of 128)
+        const int per = p.hidden / 128, half = p.inter / 128;
+        const float* s1 = static_cast<const float*>(p.s1) + ((int64_t)e * 2 * half + c0 / 128) * per + in.kb;
+        scales.bring(ring.s_in, lane, in.kb, 0, [&](int i) { return s1 + i * half * per; });
+      }
+      ring.advance_in();
+      in.kb += per_group;
+      ++in_it;
     }
-    in.kb += per_group;
-    ++in_it;
+    cp_async_commit();
   };
-  for (int i = 0; i < p.slots_per_warp && in_it < n_it; ++i) bring();
+  for (int i = 0; i < p.slots_per_warp; ++i) bring();
 
-  // ---- Q1 that needs whole rows, once per block while the first boxes travel ----
-  float* row_scale = reinterpret_cast<float*>(rest);       // [tokens][2]: scale, reciprocal
-  if (is_channel(K)) rest += (8 * p.tokens + 15) & ~15;
-  uint8_t* x_codes = rest;                                 // [tokens][pitch], scales behind them
-  const int pitch = code_pitch(K, p.hidden);
-  uint8_t* x_sf = x_codes + p.tokens * pitch;              // 4-bit: bytes
-  float* x_scale = reinterpret_cast<float*>(x_sf);         // block-scaled: [hidden / 128][8]
-  constexpr int kBlk = K == K_NV4 ? 16 : 32;
-  const int sf_row = p.hidden / kBlk;
-  if constexpr (is_channel(K)) {
-    for (int m = warp; m < p.tokens; m += kWarps) {
-      const uint16_t* row = static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden;
-      float amax = 0.f;
-      for (int c = lane * 8; c < p.hidden; c += 256) {
-        const uint4 u = *reinterpret_cast<const uint4*>(row + c);
-        const uint32_t q[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (p.x_dtype == BOLT_BF16) {
-            amax = fmaxf(amax, fabsf(__uint_as_float(q[j] << 16)));
-            amax = fmaxf(amax, fabsf(__uint_as_float(q[j] & 0xFFFF0000u)));
-          } else {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q[j]));
-            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-        }
-      }
-      for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      if (lane == 0) scale8<K>(amax, row_scale[2 * m], row_scale[2 * m + 1]);
-    }
-    __syncthreads();
-  }
-  if constexpr (keeps_codes(K, NT)) {
-    // a warp per group of 128 values
-    const int per_row = (p.hidden + 127) / 128;
-    for (int i = warp; i < p.tokens * per_row; i += kWarps) {
-      const int m = i / per_row, kb = i - m * per_row, c = kb * 128 + 4 * lane;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (c < p.hidden) v = load_values4(static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden, p.x_dtype, c);
-      float scale, inv;
-      if constexpr (is_block(K)) {
-        const float top = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-        scale8<K>(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))), scale, inv);
-        if (lane == 0) x_scale[kb * 8 + m] = scale;
-      } else {
-        inv = row_scale[2 * m + 1];
-      }
-      if (c < p.hidden) *reinterpret_cast<uint32_t*>(x_codes + m * pitch + c) = codes4<K>(v, inv);
-    }
-    __syncthreads();
-  }
-  if constexpr (is4(K)) {
-    const bool nv = K == K_NV4;
-    const float inv_g = p.a1 != nullptr ? __frcp_rn(*p.a1) : 1.f;
-    const int per_row = p.hidden / 32;
-    for (int i = tid; i < p.tokens * per_row; i += kThreads) {
-      const int m = i / per_row, c = (i - m * per_row) * 32;
-      float v[32];
-      load_values32(v, static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden, p.x_dtype, c);
-      if (nv && p.a1 != nullptr) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] *= inv_g;
-      }
-      uint32_t w[4];
-#pragma unroll
-      for (int b = 0; b < 32 / kBlk; ++b) {
-        float amax = 0.f;
-#pragma unroll
-        for (int j = 0; j < kBlk; ++j) amax = fp4::amax_nan(amax, v[b * kBlk + j]);
-        const uint32_t byte = fp4::scale_byte<K == K_NV4>(amax);
-        const fp4::Scaler sc = fp4::scaler_of<K == K_NV4>(byte);
-#pragma unroll
-        for (int j = 0; j < kBlk / 8; ++j)
-          w[b * (kBlk / 8) + j] = fp4::codes8<K == K_NV4>(v + b * kBlk + 8 * j, sc);
-        x_sf[(int64_t)m * sf_row + c / kBlk + b] = (uint8_t)byte;
-      }
-      *reinterpret_cast<uint4*>(x_codes + m * pitch + c / 2) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    __syncthreads();
-  }
-
-  const int sf1_row = p.hidden / kBlk;
-  auto row_scales = [&](RowScales<K>(&ws)[MT], const Place& q) {
-    const int64_t e = r.list[q.a];
-    const int c0 = q.c * UC;
-    if constexpr (is4(K)) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          load_block_scales<K>(ws[mt].sf[h],
-                               static_cast<const uint8_t*>(p.s1) +
-                                   ((e * 2 + h) * p.inter + c0 + 8 * mt + g) * sf1_row,
-                               sf1_row, q.kb, t);
-    } else if constexpr (is_block(K)) {
-      // (a unit of 8 or 16 columns lies in one block of 128)
-      const uint32_t* s1 = static_cast<const uint32_t*>(p.s1) +
-                           (e * (2 * p.inter / 128) + c0 / 128) * (p.hidden / 128) + q.kb;
-      ws[0].sf[0][0] = s1[0];
-      ws[0].sf[1][0] = s1[(p.inter / 128) * (p.hidden / 128)];
-    }
-  };
-  RowScales<K> ws[MT], ws_next[MT];
   int it = 0;
-  if (n_it > 0) row_scales(ws_next, cur);
   Place unit = {first_u, first_u / per_expert, first_u % per_expert, 0};
   // (the group's own barrier, named 1 to 8; a warp by itself needs none)
   auto group_sync = [&]() {
@@ -551,15 +571,6 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
     const int tok0 = r.token[off + min(2 * t, cnt - 1)], tok1 = r.token[off + min(2 * t + 1, cnt - 1)];
 
     while (it < n_it && cur.u == unit.u) {
-      // next box's scales travel while this one is computed
-      Place nxt = cur;
-      nxt.kb += per_group;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) ws[mt] = ws_next[mt];
-      if (it + 1 < n_it) {
-        settle(nxt);
-        row_scales(ws_next, nxt);
-      }
       const int kb = cur.kb;
 
       TokenBox<K> x[NT];
@@ -594,6 +605,12 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
             }
           }
         }
+      }
+      RowScales<K> ws[MT];
+      if constexpr (is4(K) || is_block(K)) {
+        cp_async_wait(p.slots_per_warp - 1);
+        if (K != K_NV4) __syncwarp();
+        scales.read(ws, ring.s_out, lane);
       }
       const uint32_t box = ring.wait(abort_flag, p.status);
       if constexpr (is_block(K)) {
@@ -630,9 +647,9 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
         box_mma<K, MT, NT, true>(box, UC, lane, x, ws, live, acc);
       }
       ring.release();
-      if (in_it < n_it) bring();
-      cur = nxt;
-      ++it;
+      bring();
+      cur.kb += per_group;
+      if (++it < n_it) settle(cur);
     }
 
     // ---- sums over the warps, activation, Q2 of the 4-bit kinds ----
@@ -705,6 +722,7 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
   extern __shared__ uint8_t raw[];
   uint8_t* smem = carve(raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  if (tid == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
   Ring ring;
   volatile int* abort_flag = start<kWarps>(ring, smem, p.slots_per_warp, kBox, UR * 128);
   uint8_t* rest = smem + kWarps * p.slots_per_warp * kBox + kCtrlBytes;
@@ -714,12 +732,15 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
   if (is8(K)) rest += kWarps * code_bytes(NT);
 
   Routes r;
-  build_routes<kWarps>(p, r, rest);
+  build_routes<kWarps>(p, r, rest, [](int, int) {});
   rest += (route_bytes(p.experts, p.tokens * p.topk) + 15) & ~15;
+  using Scales = ScaleRing<K, 2 * MT>;
+  const Scales scales = {smem_u32(rest) + (uint32_t)(warp * p.slots_per_warp) * Scales::kBytes};
+  rest += kWarps * p.slots_per_warp * Scales::kBytes;
 
   const int units = (p.model_dim + UR - 1) / UR;
-  const int u0 = (int)((int64_t)units * blockIdx.x / gridDim.x);
-  const int u1 = (int)((int64_t)units * (blockIdx.x + 1) / gridDim.x);
+  int u0, u1;
+  share_of(units, u0, u1);
   const int nb = (int)((row_bytes(K, p.inter) + 127) / 128);
   const int64_t boxes = (int64_t)(u1 - u0) * r.touched * nb;
   const int n_it = boxes > warp ? (int)((boxes - warp + kWarps - 1) / kWarps) : 0;
@@ -739,45 +760,42 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
   };
   Place in = {u0, 0, warp};
   int in_it = 0;
-  auto bring = [&]() {
-    settle(in);
-    if (lane == 0) {
-      uint32_t dst;
-      const uint32_t bar = ring.next_in(dst);
-      tma_load_3d(dst, &map, bar, in.kb * 128, in.u * UR, r.list[in.a]);
-    }
-    in.kb += kWarps;
-    ++in_it;
-  };
-  for (int i = 0; i < p.slots_per_warp && in_it < n_it; ++i) bring();
-
   constexpr int kBlk = K == K_NV4 ? 16 : 32;
   const int sf_row = p.inter / kBlk;
+  auto bring = [&]() {
+    if (in_it < n_it) {
+      settle(in);
+      const int e = r.list[in.a];
+      if (lane == 0) {
+        uint32_t dst;
+        const uint32_t bar = ring.next_in(dst);
+        tma_load_3d(dst, &map, bar, in.kb * 128, in.u * UR, e);
+      }
+      // (rows past the unit's are scaled by anything: they go nowhere)
+      const int row0 = in.u * UR + g, last = p.model_dim - 1;
+      if constexpr (is4(K)) {
+        const uint8_t* s2 = static_cast<const uint8_t*>(p.s2) + (int64_t)e * p.model_dim * sf_row;
+        scales.bring(ring.s_in, lane, in.kb, sf_row,
+                     [&](int i) { return s2 + (int64_t)min(row0 + 8 * i, last) * sf_row; });
+      } else if constexpr (is_block(K)) {
+        const int per = p.inter / 128;
+        const float* s2 = static_cast<const float*>(p.s2) + (int64_t)e * (p.model_dim / 128) * per + in.kb;
+        scales.bring(ring.s_in, lane, in.kb, 0, [&](int i) { return s2 + (min(row0 + 8 * i, last) >> 7) * per; });
+      } else if constexpr (is_channel(K)) {
+        const float* s2 = static_cast<const float*>(p.s2) + (int64_t)e * p.model_dim;
+        scales.bring(ring.s_in, lane, in.kb, 0, [&](int i) { return s2 + min(row0 + 8 * i, last); });
+      }
+      ring.advance_in();
+      in.kb += kWarps;
+      ++in_it;
+    }
+    cp_async_commit();
+  };
+  for (int i = 0; i < p.slots_per_warp; ++i) bring();
+
   Place cur = {u0, 0, warp};
   if (n_it > 0) settle(cur);
-  auto row_scales = [&](RowScales<K>(&ws)[MT], const Place& q) {
-    const int64_t e = r.list[q.a];
-    // (rows past the unit's are scaled by anything: they go nowhere)
-    const int row0 = q.u * UR + g, last = p.model_dim - 1;
-    if constexpr (is_block(K)) {
-      const int per = p.inter / 128;
-      const uint32_t* s2 = static_cast<const uint32_t*>(p.s2) + e * (p.model_dim / 128) * per + q.kb;
-#pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) ws[i >> 1].sf[i & 1][0] = s2[(min(row0 + 8 * i, last) >> 7) * per];
-    } else if constexpr (is_channel(K)) {
-      const uint32_t* s2 = static_cast<const uint32_t*>(p.s2) + e * p.model_dim;
-#pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) ws[i >> 1].sf[i & 1][0] = s2[min(row0 + 8 * i, last)];
-    } else if constexpr (is4(K)) {
-      const uint8_t* s2 = static_cast<const uint8_t*>(p.s2) + e * p.model_dim * sf_row;
-#pragma unroll
-      for (int i = 0; i < 2 * MT; ++i)
-        load_block_scales<K>(ws[i >> 1].sf[i & 1], s2 + (int64_t)min(row0 + 8 * i, last) * sf_row, sf_row, q.kb, t);
-    }
-  };
-  RowScales<K> ws[MT], ws_next[MT];
   int it = 0;
-  if (n_it > 0) row_scales(ws_next, cur);
 
   wait_for_previous();     // the activations
   float* row_scale = reinterpret_cast<float*>(rest);       // [slots][2]
@@ -826,15 +844,6 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
         for (int i = 0; i < 4; ++i) acc[mt][nt][i] = 0.f;
 
     while (it < n_it && cur.u == u) {
-      Place nxt = cur;
-      nxt.kb += kWarps;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) ws[mt] = ws_next[mt];
-      if (it + 1 < n_it) {
-        settle(nxt);
-        row_scales(ws_next, nxt);
-      }
-
       const int e = r.list[cur.a], kb = cur.kb;
       const uint32_t mask = r.mask[cur.a];
       const int off = r.off[cur.a];
@@ -877,6 +886,10 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
         }
       }
       const float whole = is4(K) ? (p.g2 != nullptr ? p.g2[e] : 1.f) * (p.a2 != nullptr ? *p.a2 : 1.f) : 1.f;
+      RowScales<K> ws[MT];
+      cp_async_wait(p.slots_per_warp - 1);
+      if (K != K_NV4) __syncwarp();
+      scales.read(ws, ring.s_out, lane);
       const uint32_t box = ring.wait(abort_flag, p.status);
       float part[MT][NT][4];
 #pragma unroll
@@ -912,9 +925,9 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
         }
       }
       ring.release();
-      if (in_it < n_it) bring();
-      cur = nxt;
-      ++it;
+      bring();
+      cur.kb += kWarps;
+      if (++it < n_it) settle(cur);
     }
 
     put_sums<MT, NT>(red, acc, warp, lane, ~0u);
@@ -954,13 +967,18 @@ k_few_dense(const __grid_constant__ CUtensorMap map, const DenseParams p) {
   extern __shared__ uint8_t raw[];
   uint8_t* smem = carve(raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  if (tid == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
   Ring ring;
   volatile int* abort_flag = start<kWarps>(ring, smem, p.slots_per_warp, kBox, UR * 128);
-  float* red = reinterpret_cast<float*>(smem + kWarps * p.slots_per_warp * kBox + kCtrlBytes);
+  uint8_t* rest = smem + kWarps * p.slots_per_warp * kBox + kCtrlBytes;
+  float* red = reinterpret_cast<float*>(rest);
+  rest += red_bytes(kWarps, MT, NT);
+  using Scales = ScaleRing<K, 2 * MT>;
+  const Scales scales = {smem_u32(rest) + (uint32_t)(warp * p.slots_per_warp) * Scales::kBytes};
 
   const int units = (p.n + UR - 1) / UR;
-  const int u0 = (int)((int64_t)units * blockIdx.x / gridDim.x);
-  const int u1 = (int)((int64_t)units * (blockIdx.x + 1) / gridDim.x);
+  int u0, u1;
+  share_of(units, u0, u1);
   const int nb = (p.k / 2 + 127) / 128;
   const int64_t boxes = (int64_t)(u1 - u0) * nb;
   const int n_it = boxes > warp ? (int)((boxes - warp + kWarps - 1) / kWarps) : 0;
@@ -975,34 +993,30 @@ k_few_dense(const __grid_constant__ CUtensorMap map, const DenseParams p) {
   };
   Place in = {u0, warp};
   int in_it = 0;
-  auto bring = [&]() {
-    settle(in);
-    if (lane == 0) {
-      uint32_t dst;
-      const uint32_t bar = ring.next_in(dst);
-      tma_load_3d(dst, &map, bar, in.kb * 128, in.u * UR, 0);
-    }
-    in.kb += kWarps;
-    ++in_it;
-  };
-  for (int i = 0; i < p.slots_per_warp && in_it < n_it; ++i) bring();
-
   constexpr int kBlk = K == K_NV4 ? 16 : 32;
   const int sf_row = p.k / kBlk, row_len = p.k / 2;
+  auto bring = [&]() {
+    if (in_it < n_it) {
+      settle(in);
+      if (lane == 0) {
+        uint32_t dst;
+        const uint32_t bar = ring.next_in(dst);
+        tma_load_3d(dst, &map, bar, in.kb * 128, in.u * UR, 0);
+      }
+      const int row0 = in.u * UR + g, last = p.n - 1;
+      scales.bring(ring.s_in, lane, in.kb, sf_row,
+                   [&](int i) { return p.w_sf + (int64_t)min(row0 + 8 * i, last) * sf_row; });
+      ring.advance_in();
+      in.kb += kWarps;
+      ++in_it;
+    }
+    cp_async_commit();
+  };
+  for (int i = 0; i < p.slots_per_warp; ++i) bring();
+
   Place cur = {u0, warp};
   settle(cur);
-  auto row_scales = [&](RowScales<K>(&ws)[MT], const Place& q) {
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t row = min(q.u * UR + 16 * mt + 8 * h + g, p.n - 1);
-        load_block_scales<K>(ws[mt].sf[h], p.w_sf + row * sf_row, sf_row, q.kb, t);
-      }
-  };
-  RowScales<K> ws[MT], ws_next[MT];
   int it = 0;
-  if (n_it > 0) row_scales(ws_next, cur);
   const unsigned live = (1u << ((p.rows + 7) / 8)) - 1u;
   const float alpha = p.alpha != nullptr ? *p.alpha : 1.f;
 
@@ -1015,14 +1029,6 @@ k_few_dense(const __grid_constant__ CUtensorMap map, const DenseParams p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[mt][nt][i] = 0.f;
     while (it < n_it && cur.u == u) {
-      Place nxt = cur;
-      nxt.kb += kWarps;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) ws[mt] = ws_next[mt];
-      if (it + 1 < n_it) {
-        settle(nxt);
-        row_scales(ws_next, nxt);
-      }
       TokenBox<K> x[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -1040,12 +1046,16 @@ k_few_dense(const __grid_constant__ CUtensorMap map, const DenseParams p) {
           }
         }
       }
+      RowScales<K> ws[MT];
+      cp_async_wait(p.slots_per_warp - 1);
+      if (K != K_NV4) __syncwarp();
+      scales.read(ws, ring.s_out, lane);
       const uint32_t box = ring.wait(abort_flag, p.status);
       box_mma<K, MT, NT, false>(box, 0, lane, x, ws, live, acc);
       ring.release();
-      if (in_it < n_it) bring();
-      cur = nxt;
-      ++it;
+      bring();
+      cur.kb += kWarps;
+      if (++it < n_it) settle(cur);
     }
     put_sums<MT, NT>(red, acc, warp, lane, live);
     __syncthreads();
@@ -1139,8 +1149,8 @@ void workspace_parts(const bolt_decode_args* a, size_t (&part)[3]) {
 
 constexpr int kSmem = 226 * 1024;   // of a block
 constexpr int kKeepBytes = 64 * 1024;
-int ring_slots(int fixed, int box_bytes, int warps) {
-  int slots = (kSmem - fixed) / (warps * box_bytes);
+int ring_slots(int fixed, int slot_bytes, int warps) {
+  int slots = (kSmem - fixed) / (warps * slot_bytes);
   return slots * warps > kMaxBarriers ? kMaxBarriers / warps : slots;
 }
 template <int K, int NT>
@@ -1158,7 +1168,8 @@ template <int K, int NT>
 int launch(const bolt_decode_args* a, Params p, cudaStream_t st) {
   constexpr int kWarps = warps_of(K, NT);
   const int up = up_fixed_bytes<K, NT>(p);
-  const int up_slots = ring_slots(up, up_box_bytes(K), kWarps);
+  constexpr int kUpSlot = up_box_bytes(K) + up_scale_bytes(K), kDownSlot = kDownBoxBytes + ScaleRing<K, 2 * kDownTiles>::kBytes;
+  const int up_slots = ring_slots(up, kUpSlot, kWarps);
   if constexpr (NT < 4)     // kept codes that leave no room: the form for more tokens keeps none
     if (up_slots < 1 && keeps_codes(K, NT)) return launch<K, 2 * NT>(a, p, st);
   int down = 1024 + kCtrlBytes + red_bytes(kWarps, kDownTiles, NT) + a16(route_bytes(p.experts, p.tokens * p.topk));
@@ -1171,7 +1182,7 @@ int launch(const bolt_decode_args* a, Params p, cudaStream_t st) {
     p.keep_act = bytes <= kKeepBytes ? 1 : 0;
     if (p.keep_act) down += a16((int)bytes);
   }
-  const int down_slots = ring_slots(down, kDownBoxBytes, kWarps);
+  const int down_slots = ring_slots(down, kDownSlot, kWarps);
   if (up_slots < 1 || down_slots < 1) {
     set_error("moe_decode: %d tokens of hidden size %d do not fit in shared memory", p.tokens, p.hidden);
     return BOLT_ERR_UNSUPPORTED;
@@ -1206,14 +1217,14 @@ int launch(const bolt_decode_args* a, Params p, cudaStream_t st) {
   p.slots_per_warp = up_slots;
   p.unit = columns;
   p.group_warps = group_warps(kWarps, (int)((row_bytes(K, p.hidden) + 127) / 128));
-  k_few_up<K, NT><<<sms, 32 * kWarps, up + up_slots * kWarps * up_box_bytes(K), st>>>(m1, p);
+  k_few_up<K, NT><<<sms, 32 * kWarps, up + up_slots * kWarps * kUpSlot, st>>>(m1, p);
   BOLT_LAUNCH_CHECK();
   p.slots_per_warp = down_slots;
   p.unit = rows;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(sms);
   cfg.blockDim = dim3(32 * kWarps);
-  cfg.dynamicSmemBytes = down + down_slots * kWarps * kDownBoxBytes;
+  cfg.dynamicSmemBytes = down + down_slots * kWarps * kDownSlot;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1238,7 +1249,8 @@ int launch_dense(const bolt_fp4_few_args* a, DenseParams p, int sms, cudaStream_
   int rc = configure_kernel(k_few_dense<K, NT>, kSmem, ready, 0, 0, 0, 0);
   if (rc != BOLT_OK) return rc;
   const int fixed = 1024 + kCtrlBytes + red_bytes(kWarps, kDownTiles, NT);
-  p.slots_per_warp = ring_slots(fixed, kDownBoxBytes, kWarps);
+  constexpr int kSlot = kDownBoxBytes + ScaleRing<K, 2 * kDownTiles>::kBytes;
+  p.slots_per_warp = ring_slots(fixed, kSlot, kWarps);
   p.unit = unit_size(p.n, kMaxRows, 1, sms);
   const cuuint64_t kb = (cuuint64_t)p.k / 2;
   const cuuint64_t size[3] = {kb, (cuuint64_t)p.n, 1}, strides[2] = {kb, kb * p.n};
@@ -1246,7 +1258,7 @@ int launch_dense(const bolt_fp4_few_args* a, DenseParams p, int sms, cudaStream_
   CUtensorMap map;
   if ((rc = encode(&map, a->w, 3, size, strides, box)) != BOLT_OK) return rc;
   const int units = (p.n + p.unit - 1) / p.unit;
-  k_few_dense<K, NT><<<units < sms ? units : sms, 32 * kWarps, fixed + p.slots_per_warp * kWarps * kDownBoxBytes, st>>>(
+  k_few_dense<K, NT><<<units < sms ? units : sms, 32 * kWarps, fixed + p.slots_per_warp * kWarps * kSlot, st>>>(
       map, p);
   BOLT_LAUNCH_CHECK();
   return BOLT_OK;

@@ -283,6 +283,74 @@ __device__ __forceinline__ void load_token(TokenBox<K>& x, const uint8_t* row, i
     }
   }
 }
+// Asynchronous copy of four bytes; `have` false: zeros, nothing is read.
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool have) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(have ? 4u : 0u) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the newest `pending` groups of this thread have landed.
+__device__ __forceinline__ void cp_async_wait(int pending) {
+  if (pending <= 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  else if (pending == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else if (pending == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else asm volatile("cp.async.wait_group 3;" ::: "memory");
+}
+
+// A warp's ring of weight scales, beside its ring of boxes and as far ahead: read when they are needed,
+// one box ahead, they came too late (a load takes as long as a box's copy, thousands of cycles while
+// HBM is busy; DeepSeek-V3 fp8, one token: a third of the first kernel's time).  kRows rows per lane
+// group g.  NV: word [row][lane], the lane's own 64 values.  MX: word [2 row + half][g].  fp32 scales:
+// word [row][g].  Words are shared out to the lanes; a slot is kBytes.
+template <int K, int ROWS>
+struct ScaleRing {
+  static constexpr int kWords = K == K_NV4 ? ROWS * 32 : K == K_MX4 ? ROWS * 16 : is8(K) ? ROWS * 8 : 0;
+  static constexpr int kBytes = (kWords * 4 + 15) / 16 * 16;
+  uint32_t base;
+  // src(row, ok): start of the scales of row i (0 .. ROWS - 1) of lane group g: a row's bytes (4-bit) or
+  // the scale itself (fp32)
+  template <typename Src>
+  __device__ __forceinline__ void bring(int slot, int lane, int kb, int row_bytes, Src src) const {
+    const int g = lane >> 2, t = lane & 3;
+    const uint32_t dst = base + slot * kBytes;
+    if constexpr (K == K_NV4) {
+      const int off = kb * 16 + 4 * t;
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) cp_async_4(dst + (i * 32 + lane) * 4, src(i) + (off < row_bytes ? off : 0), off < row_bytes);
+    } else if constexpr (K == K_MX4) {
+#pragma unroll
+      for (int q = 0; q < ROWS / 2; ++q) {
+        const int w = t * (ROWS / 2) + q, off = kb * 8 + 4 * (w & 1);
+        cp_async_4(dst + (w * 8 + g) * 4, src(w >> 1) + (off < row_bytes ? off : 0), off < row_bytes);
+      }
+    } else if constexpr (is8(K)) {
+      if (ROWS >= 4 || t < ROWS) {
+#pragma unroll
+        for (int q = 0; q < (ROWS + 3) / 4; ++q) {
+          const int i = t + 4 * q;
+          cp_async_4(dst + (i * 8 + g) * 4, src(i), true);
+        }
+      }
+    }
+  }
+  // after cp_async_wait (and, but for NV, __syncwarp)
+  template <int MT>
+  __device__ __forceinline__ void read(RowScales<K> (&ws)[MT], int slot, int lane) const {
+    const int g = lane >> 2;
+    const uint32_t src = base + slot * kBytes;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      if constexpr (K == K_NV4) {
+        ws[i >> 1].sf[i & 1][0] = lds32(src + (i * 32 + lane) * 4);
+      } else if constexpr (K == K_MX4) {
+        ws[i >> 1].sf[i & 1][0] = lds32(src + ((2 * i) * 8 + g) * 4);
+        ws[i >> 1].sf[i & 1][1] = lds32(src + ((2 * i + 1) * 8 + g) * 4);
+      } else if constexpr (is8(K)) {
+        ws[i >> 1].sf[i & 1][0] = lds32(src + (i * 8 + g) * 4);
+      }
+    }
+  }
+};
+
 // Block scales of box kb out of a row of `bytes` scale bytes (a multiple of four): NV the word of
 // the lane's own 64 values, MX both words of the box.
 template <int K>
