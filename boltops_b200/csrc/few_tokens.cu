@@ -515,26 +515,38 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
   }
   int in_it = 0;
   const Scales scales = {scale_mem + (uint32_t)(warp * p.slots_per_warp) * Scales::kBytes};
-  // the next box and its scales; past the last an empty group, so that groups stay one a box
+  // the next box and its scales; past the last an empty group, so that groups stay one a box.  What
+  // depends on the unit alone is kept from box to box.
+  int in_e = 0;
+  const uint8_t* in_scale = nullptr;
+  auto enter = [&]() {
+    in_e = r.list[in.a];
+    if constexpr (is4(K)) {
+      in_scale = static_cast<const uint8_t*>(p.s1) + ((int64_t)in_e * 2 * p.inter + in.c * UC + g) * sf_row;
+    } else if constexpr (is_block(K)) {
+      // (a unit of 8 or 16 columns lies in one block of 128)
+      in_scale = static_cast<const uint8_t*>(p.s1) +
+                 ((int64_t)in_e * (2 * p.inter / 128) + in.c * UC / 128) * (p.hidden / 128) * 4;
+    }
+  };
+  if (n_it > 0) enter();
+  const int half_rows = is4(K) ? p.inter * sf_row : p.inter / 128 * (p.hidden / 128) * 4;
   auto bring = [&]() {
     if (in_it < n_it) {
-      settle(in);
-      const int e = r.list[in.a], c0 = in.c * UC;
+      if (in.kb >= nb) {
+        settle(in);
+        enter();
+      }
       if (lane == 0) {
         uint32_t dst;
         const uint32_t bar = ring.next_in(dst);
-        tma_load_4d(dst, &map, bar, in.kb * 128, c0, 0, e);
+        tma_load_4d(dst, &map, bar, in.kb * 128, in.c * UC, 0, in_e);
       }
-      if constexpr (is4(K)) {
-        const uint8_t* s1 = static_cast<const uint8_t*>(p.s1) + ((int64_t)e * 2 * p.inter + c0 + g) * sf_row;
-        const int half = p.inter * sf_row;
-        scales.bring(ring.s_in, lane, in.kb, sf_row, [&](int i) { return s1 + (i & 1) * half + 8 * (i >> 1) * sf_row; });
-      } else if constexpr (is_block(K)) {
-        // (a unit of 8 or 16 columns lies in one block of 128)
-        const int per = p.hidden / 128, half = p.inter / 128;
-        const float* s1 = static_cast<const float*>(p.s1) + ((int64_t)e * 2 * half + c0 / 128) * per + in.kb;
-        scales.bring(ring.s_in, lane, in.kb, 0, [&](int i) { return s1 + i * half * per; });
-      }
+      if constexpr (is4(K))
+        scales.bring(ring.s_in, lane, in.kb, sf_row,
+                     [&](int i) { return in_scale + (i & 1) * half_rows + 8 * (i >> 1) * sf_row; });
+      else if constexpr (is_block(K))
+        scales.bring(ring.s_in, lane, in.kb, 0, [&](int i) { return in_scale + i * half_rows + in.kb * 4; });
       ring.advance_in();
       in.kb += per_group;
       ++in_it;
@@ -762,28 +774,45 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
   int in_it = 0;
   constexpr int kBlk = K == K_NV4 ? 16 : 32;
   const int sf_row = p.inter / kBlk;
+  // what depends on expert and unit alone is kept from box to box
+  int in_e = 0;
+  const uint8_t* in_scale = nullptr;
+  int in_row[2 * MT];          // offsets of a thread's rows (those past the unit's: of any)
+  auto enter = [&]() {
+    in_e = r.list[in.a];
+    const int row0 = in.u * UR + g, last = p.model_dim - 1;
+    const int64_t rows_before = (int64_t)in_e * (is_block(K) ? p.model_dim / 128 : p.model_dim);
+    const int row_len = is4(K) ? sf_row : is_block(K) ? p.inter / 128 * 4 : 4;
+    in_scale = static_cast<const uint8_t*>(p.s2) + rows_before * row_len;
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) {
+      const int row = min(row0 + 8 * i, last);
+      in_row[i] = (is_block(K) ? row >> 7 : row) * row_len;
+    }
+  };
+  if (n_it > 0) {
+    settle(in);
+    enter();
+  }
   auto bring = [&]() {
     if (in_it < n_it) {
-      settle(in);
-      const int e = r.list[in.a];
+      if (in.kb >= nb) {
+        settle(in);
+        if (!is16(K)) enter();
+        else in_e = r.list[in.a];
+      }
       if (lane == 0) {
         uint32_t dst;
         const uint32_t bar = ring.next_in(dst);
-        tma_load_3d(dst, &map, bar, in.kb * 128, in.u * UR, e);
+        tma_load_3d(dst, &map, bar, in.kb * 128, in.u * UR, in_e);
       }
-      // (rows past the unit's are scaled by anything: they go nowhere)
-      const int row0 = in.u * UR + g, last = p.model_dim - 1;
-      if constexpr (is4(K)) {
-        const uint8_t* s2 = static_cast<const uint8_t*>(p.s2) + (int64_t)e * p.model_dim * sf_row;
-        scales.bring(ring.s_in, lane, in.kb, sf_row,
-                     [&](int i) { return s2 + (int64_t)min(row0 + 8 * i, last) * sf_row; });
-      } else if constexpr (is_block(K)) {
-        const int per = p.inter / 128;
-        const float* s2 = static_cast<const float*>(p.s2) + (int64_t)e * (p.model_dim / 128) * per + in.kb;
-        scales.bring(ring.s_in, lane, in.kb, 0, [&](int i) { return s2 + (min(row0 + 8 * i, last) >> 7) * per; });
-      } else if constexpr (is_channel(K)) {
-        const float* s2 = static_cast<const float*>(p.s2) + (int64_t)e * p.model_dim;
-        scales.bring(ring.s_in, lane, in.kb, 0, [&](int i) { return s2 + min(row0 + 8 * i, last); });
+      if constexpr (is4(K))
+        scales.bring(ring.s_in, lane, in.kb, sf_row, [&](int i) { return in_scale + in_row[i]; });
+      else if constexpr (is8(K)) {
+        // (each lane of four brings one of the four rows)
+        static_assert(MT == 2, "four rows a thread");
+        const int mine = t < 2 ? (t == 0 ? in_row[0] : in_row[1]) : (t == 2 ? in_row[2] : in_row[3]);
+        scales.bring(ring.s_in, lane, in.kb, 0, [&](int) { return in_scale + mine + (is_block(K) ? in.kb * 4 : 0); });
       }
       ring.advance_in();
       in.kb += kWarps;
@@ -995,17 +1024,25 @@ k_few_dense(const __grid_constant__ CUtensorMap map, const DenseParams p) {
   int in_it = 0;
   constexpr int kBlk = K == K_NV4 ? 16 : 32;
   const int sf_row = p.k / kBlk, row_len = p.k / 2;
+  int64_t in_row[2 * MT];      // a thread's rows of scales (those past the unit's: any)
+  auto enter = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) in_row[i] = (int64_t)min(in.u * UR + g + 8 * i, p.n - 1) * sf_row;
+  };
+  settle(in);
+  enter();
   auto bring = [&]() {
     if (in_it < n_it) {
-      settle(in);
+      if (in.kb >= nb) {
+        settle(in);
+        enter();
+      }
       if (lane == 0) {
         uint32_t dst;
         const uint32_t bar = ring.next_in(dst);
         tma_load_3d(dst, &map, bar, in.kb * 128, in.u * UR, 0);
       }
-      const int row0 = in.u * UR + g, last = p.n - 1;
-      scales.bring(ring.s_in, lane, in.kb, sf_row,
-                   [&](int i) { return p.w_sf + (int64_t)min(row0 + 8 * i, last) * sf_row; });
+      scales.bring(ring.s_in, lane, in.kb, sf_row, [&](int i) { return p.w_sf + in_row[i]; });
       ring.advance_in();
       in.kb += kWarps;
       ++in_it;
