@@ -309,3 +309,14 @@ def on_device(device: torch.device):
     if index is None or index == torch._C._cuda_getDevice():
         return _NO_GUARD
     return torch.cuda.device(device)
+
+
+def call(device: torch.device, fn, *args) -> None:
+    """``check(fn(*args))`` with ``device`` current."""
+    if device.index == torch._C._cuda_getDevice():
+        status = fn(*args)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args)
+    if status != BOLT_OK:
+        check(status)

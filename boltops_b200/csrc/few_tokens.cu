@@ -55,7 +55,7 @@ struct Params {
   int amax_cols;            // units of an expert in the first kernel
   int unit;                 // columns (first kernel) or rows (second) of a unit
   int group_warps;          // warps that share a unit (first kernel)
-  int keep_act;             // codes of the activations are kept in shared memory (second kernel)
+  int keep_x, keep_act;     // 8-bit codes of the rows, of the activations are made once and kept
 };
 
 // ---------------------------------------------------------------------------
@@ -362,10 +362,42 @@ constexpr int up_scale_bytes(int k) {      // of a slot
 }
 constexpr int warps_of(int k, int nt) { return nt == 4 || k == K_MX4 ? 8 : 16; }
 constexpr int red_bytes(int warps, int mt, int nt) { return warps * mt * nt * 128 * 4; }
-// 8-bit kinds, up to eight tokens: the rows' codes are made once and kept
-constexpr bool keeps_codes(int k, int nt) { return is8(k) && nt == 1; }
 // bytes of a kept row of codes: 16 more than it has, so that eight rows lie in different banks
 __host__ __device__ constexpr int code_pitch(int k, int n) { return (int)row_bytes(k, n) + 16; }
+
+// Rows of `cols` values to 8-bit codes in shared memory, a group of 128 values a warp and four groups at
+// once: their loads travel together.
+template <int K, typename RowOf, typename InvOf, typename Scale>
+__device__ __forceinline__ void keep_codes(int w0, int wn, int lane, int rows, int cols, uint8_t* codes, int pitch,
+                                           RowOf row_of, int dt, InvOf inv_of, Scale put_scale) {
+  const int per_row = (cols + 127) / 128, all = rows * per_row;
+  for (int i0 = w0; i0 < all; i0 += 4 * wn) {
+    float4 v[4];
+    int m[4], kb[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + j * wn;
+      m[j] = i / per_row;
+      kb[j] = i - m[j] * per_row;
+      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < all && kb[j] * 128 + 4 * lane < cols) v[j] = load_values4(row_of(m[j]), dt, kb[j] * 128 + 4 * lane);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i0 + j * wn >= all) break;
+      float scale, inv;
+      if constexpr (is_block(K)) {
+        const float top = fmaxf(fmaxf(fabsf(v[j].x), fabsf(v[j].y)), fmaxf(fabsf(v[j].z), fabsf(v[j].w)));
+        scale8<K>(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))), scale, inv);
+        if (lane == 0) put_scale(m[j], kb[j], scale);
+      } else {
+        inv = inv_of(m[j]);
+      }
+      const int c = kb[j] * 128 + 4 * lane;
+      if (c < cols) *reinterpret_cast<uint32_t*>(codes + m[j] * pitch + c) = codes4<K>(v[j], inv);
+    }
+  }
+}
 
 // ---------------------------------------------------------------------------
 // gate and up projections, activation
@@ -389,7 +421,7 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
   float* red = reinterpret_cast<float*>(rest);
   rest += red_bytes(kWarps, MT, NT);
   uint8_t* stage = rest + warp * code_bytes(NT);
-  if (is8(K) && !keeps_codes(K, NT)) rest += kWarps * code_bytes(NT);
+  if (is8(K) && !p.keep_x) rest += kWarps * code_bytes(NT);
   let_next_start();
 
   uint8_t* const route_mem = rest;
@@ -401,7 +433,7 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
   uint8_t* x_codes = rest;                                 // [tokens][pitch], scales behind them
   const int pitch = code_pitch(K, p.hidden);
   uint8_t* x_sf = x_codes + p.tokens * pitch;              // 4-bit: bytes
-  float* x_scale = reinterpret_cast<float*>(x_sf);         // block-scaled: [hidden / 128][8]
+  float* x_scale = reinterpret_cast<float*>(x_sf);         // block-scaled: [hidden / 128][tokens]
   constexpr int kBlk = K == K_NV4 ? 16 : 32;
   const int sf_row = p.hidden / kBlk;
 
@@ -430,26 +462,12 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
         for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         if (lane == 0) scale8<K>(amax, row_scale[2 * m], row_scale[2 * m + 1]);
       }
-      if (keeps_codes(K, NT)) asm volatile("bar.sync 15, %0;" ::"r"(32 * wn) : "memory");
+      if (p.keep_x) asm volatile("bar.sync 15, %0;" ::"r"(32 * wn) : "memory");
     }
-    if constexpr (keeps_codes(K, NT)) {
-      // a warp per group of 128 values
-      const int per_row = (p.hidden + 127) / 128;
-#pragma unroll 4
-      for (int i = w0; i < p.tokens * per_row; i += wn) {
-        const int m = i / per_row, kb = i - m * per_row, c = kb * 128 + 4 * lane;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c < p.hidden) v = load_values4(static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden, p.x_dtype, c);
-        float scale, inv;
-        if constexpr (is_block(K)) {
-          const float top = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-          scale8<K>(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))), scale, inv);
-          if (lane == 0) x_scale[kb * 8 + m] = scale;
-        } else {
-          inv = row_scale[2 * m + 1];
-        }
-        if (c < p.hidden) *reinterpret_cast<uint32_t*>(x_codes + m * pitch + c) = codes4<K>(v, inv);
-      }
+    if (is8(K) && p.keep_x) {
+      keep_codes<K>(w0, wn, lane, p.tokens, p.hidden, x_codes, pitch, [&](int m) {
+        return static_cast<const void*>(static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden); }, p.x_dtype,
+        [&](int m) { return row_scale[2 * m + 1]; }, [&](int m, int kb, float scale) { x_scale[kb * p.tokens + m] = scale; });
     }
     if constexpr (is4(K)) {
       const bool nv = K == K_NV4;
@@ -579,16 +597,24 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) tok[nt] = 8 * nt + g < cnt ? r.token[off + 8 * nt + g] : -1;
 
-    // tokens of columns 2 t and 2 t + 1 (of one that has none: any)
-    const int tok0 = r.token[off + min(2 * t, cnt - 1)], tok1 = r.token[off + min(2 * t + 1, cnt - 1)];
+    int tok_of[NT][2];     // tokens of columns 2 t and 2 t + 1 (of a column without one: any)
+    if constexpr (is_block(K)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) tok_of[nt][i] = r.token[off + min(8 * nt + 2 * t + i, cnt - 1)];
+    }
 
     while (it < n_it && cur.u == unit.u) {
       const int kb = cur.kb;
 
       TokenBox<K> x[NT];
       float xs = 1.f;
-      if constexpr (keeps_codes(K, NT)) {
-        load_token<K>(x[0], tok[0] < 0 ? nullptr : x_codes + tok[0] * pitch, p.hidden, kb, t);
+      if (is8(K) && p.keep_x) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          if ((live >> nt) & 1u)
+            load_token<K>(x[nt], tok[nt] < 0 ? nullptr : x_codes + tok[nt] * pitch, p.hidden, kb, t);
       } else if constexpr (is8(K)) {
         xs = quant_box<K, NT>(
             x, stage, live_cols, p.x_dtype, p.hidden, kb * 128, lane,
@@ -638,9 +664,9 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
         for (int nt = 0; nt < NT; ++nt) {
           if (!((live >> nt) & 1u)) continue;
           float x0, x1;
-          if constexpr (keeps_codes(K, NT)) {
-            x0 = x_scale[kb * 8 + tok0];
-            x1 = x_scale[kb * 8 + tok1];
+          if (p.keep_x) {
+            x0 = x_scale[kb * p.tokens + tok_of[nt][0]];
+            x1 = x_scale[kb * p.tokens + tok_of[nt][1]];
           } else {
             x0 = __shfl_sync(0xffffffffu, xs, 8 * nt + 2 * t);
             x1 = __shfl_sync(0xffffffffu, xs, 8 * nt + 2 * t + 1);
@@ -843,22 +869,11 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
   uint8_t* a_codes = rest + (is_channel(K) ? (8 * p.tokens * p.topk + 15) & ~15 : 0);
   const int a_pitch = code_pitch(K, p.inter);
   float* a_scale = reinterpret_cast<float*>(a_codes + p.tokens * p.topk * a_pitch);     // [slots][boxes]
-  if constexpr (keeps_codes(K, NT)) {
+  if constexpr (is8(K)) {
     if (p.keep_act) {
-      for (int i = warp; i < r.slots * nb; i += kWarps) {
-        const int s = i / nb, kb = i - s * nb, c = kb * 128 + 4 * lane;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c < p.inter) v = load_values4(reinterpret_cast<const float*>(p.act_rows) + (int64_t)s * p.inter, BOLT_F32, c);
-        float scale, inv;
-        if constexpr (is_block(K)) {
-          const float top = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-          scale8<K>(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))), scale, inv);
-          if (lane == 0) a_scale[i] = scale;
-        } else {
-          inv = row_scale[2 * s + 1];
-        }
-        if (c < p.inter) *reinterpret_cast<uint32_t*>(a_codes + s * a_pitch + c) = codes4<K>(v, inv);
-      }
+      keep_codes<K>(warp, kWarps, lane, r.slots, p.inter, a_codes, a_pitch, [&](int m) {
+        return static_cast<const void*>(reinterpret_cast<const float*>(p.act_rows) + (int64_t)m * p.inter); }, BOLT_F32,
+        [&](int m) { return row_scale[2 * m + 1]; }, [&](int m, int kb, float scale) { a_scale[m * nb + kb] = scale; });
       __syncthreads();
     }
   }
@@ -882,10 +897,14 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
 
       TokenBox<K> x[NT];
       float xs = 1.f;
-      const bool kept = keeps_codes(K, NT) && p.keep_act;
+      const bool kept = is8(K) && p.keep_act;
       if (kept) {
-        const int slot = slot_of(mask, off, g);
-        load_token<K>(x[0], slot < 0 ? nullptr : a_codes + slot * a_pitch, p.inter, kb, t);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (!((live >> nt) & 1u)) continue;
+          const int slot = slot_of(mask, off, 8 * nt + g);
+          load_token<K>(x[nt], slot < 0 ? nullptr : a_codes + slot * a_pitch, p.inter, kb, t);
+        }
       } else if constexpr (is8(K)) {
         xs = quant_box<K, NT>(
             x, stage, mask, BOLT_F32, p.inter, kb * 128, lane,
@@ -1185,41 +1204,35 @@ void workspace_parts(const bolt_decode_args* a, size_t (&part)[3]) {
 }
 
 constexpr int kSmem = 226 * 1024;   // of a block
-constexpr int kKeepBytes = 64 * 1024;
 int ring_slots(int fixed, int slot_bytes, int warps) {
   int slots = (kSmem - fixed) / (warps * slot_bytes);
   return slots * warps > kMaxBarriers ? kMaxBarriers / warps : slots;
 }
 template <int K, int NT>
-int up_fixed_bytes(const Params& p) {
-  int n = 1024 + kCtrlBytes + red_bytes(warps_of(K, NT), up_tiles(K), NT) +
-          a16(route_bytes(p.experts, p.tokens * p.topk));
-  if (is_channel(K)) n += a16(8 * p.tokens);
-  if (is4(K)) n += p.tokens * (code_pitch(K, p.hidden) + p.hidden / (K == K_NV4 ? 16 : 32));
-  else if (keeps_codes(K, NT)) n += p.tokens * code_pitch(K, p.hidden) + (is_block(K) ? p.hidden / 128 * 32 : 0);
-  else if (is8(K)) n += warps_of(K, NT) * code_bytes(NT);
-  return n;
-}
-
-template <int K, int NT>
 int launch(const bolt_decode_args* a, Params p, cudaStream_t st) {
   constexpr int kWarps = warps_of(K, NT);
-  const int up = up_fixed_bytes<K, NT>(p);
   constexpr int kUpSlot = up_box_bytes(K) + up_scale_bytes(K), kDownSlot = kDownBoxBytes + ScaleRing<K, 2 * kDownTiles>::kBytes;
-  const int up_slots = ring_slots(up, kUpSlot, kWarps);
-  if constexpr (NT < 4)     // kept codes that leave no room: the form for more tokens keeps none
-    if (up_slots < 1 && keeps_codes(K, NT)) return launch<K, 2 * NT>(a, p, st);
-  int down = 1024 + kCtrlBytes + red_bytes(kWarps, kDownTiles, NT) + a16(route_bytes(p.experts, p.tokens * p.topk));
-  if (is8(K)) down += kWarps * code_bytes(NT);
-  if (is_channel(K)) down += a16(8 * p.tokens * p.topk);
-  if (keeps_codes(K, NT)) {
-    // up to kKeepBytes of them: beyond, the rings would shrink
-    const int64_t bytes = (int64_t)p.tokens * p.topk *
-                          (code_pitch(K, p.inter) + (is_block(K) ? p.inter / 128 * 4 : 0));
-    p.keep_act = bytes <= kKeepBytes ? 1 : 0;
-    if (p.keep_act) down += a16((int)bytes);
+  const int routes = p.tokens * p.topk;
+  int up = 1024 + kCtrlBytes + red_bytes(kWarps, up_tiles(K), NT) + a16(route_bytes(p.experts, routes));
+  int down = 1024 + kCtrlBytes + red_bytes(kWarps, kDownTiles, NT) + a16(route_bytes(p.experts, routes));
+  if (is_channel(K)) {
+    up += a16(8 * p.tokens);
+    down += a16(8 * routes);
   }
-  const int down_slots = ring_slots(down, kDownSlot, kWarps);
+  if (is4(K)) up += p.tokens * (code_pitch(K, p.hidden) + p.hidden / (K == K_NV4 ? 16 : 32));
+  if (is8(K)) {
+    // codes are kept where they leave the rings two boxes a warp, else made again for every box
+    const auto kept = [&](int rows, int cols) {
+      return (int64_t)rows * (code_pitch(K, cols) + (is_block(K) ? cols / 128 * 4 : 0)) + 16;
+    };
+    const int64_t x_kept = kept(p.tokens, p.hidden), act_kept = kept(routes, p.inter);
+    const int stage = kWarps * code_bytes(NT);
+    p.keep_x = up + x_kept + 2 * kWarps * kUpSlot <= kSmem;
+    up += p.keep_x ? (int)x_kept : stage;
+    p.keep_act = down + stage + act_kept + 2 * kWarps * kDownSlot <= kSmem;
+    down += stage + (p.keep_act ? (int)act_kept : 0);
+  }
+  const int up_slots = ring_slots(up, kUpSlot, kWarps), down_slots = ring_slots(down, kDownSlot, kWarps);
   if (up_slots < 1 || down_slots < 1) {
     set_error("moe_decode: %d tokens of hidden size %d do not fit in shared memory", p.tokens, p.hidden);
     return BOLT_ERR_UNSUPPORTED;
@@ -1230,7 +1243,6 @@ int launch(const bolt_decode_args* a, Params p, cudaStream_t st) {
   if (rc != BOLT_OK) return rc;
 
   const int sms = a->sm_count > 0 ? a->sm_count : sm_count_of_current_device();
-  const int64_t routes = (int64_t)p.tokens * p.topk;
   const int columns = is4(K) ? 8 * up_tiles(K)
                              : unit_size(p.inter, 8 * up_tiles(K), routes < p.experts ? routes : p.experts, sms,
                                          is_block(K) ? 8 : 1);

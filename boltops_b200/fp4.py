@@ -13,17 +13,18 @@ from typing import Optional, Tuple
 import torch
 
 from . import _cabi
-from ._cabi import check, dtype_code, ptr, stream_of
+from ._cabi import ptr, stream_of
 
 FORMATS = {"nvfp4": (_cabi.FP4_NV, 16, torch.float8_e4m3fn), "mxfp4": (_cabi.FP4_MX, 32, torch.uint8)}
-_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_FORMAT_OF = {dtype: name for name, (_, _, dtype) in FORMATS.items()}
+_FLOATS = {torch.bfloat16: _cabi.BF16, torch.float16: _cabi.F16, torch.float32: _cabi.F32}
 
 
 def format_of(scales: torch.Tensor) -> str:
     """The format that scales of this dtype belong to."""
-    for name, (_, _, dtype) in FORMATS.items():
-        if scales.dtype == dtype:
-            return name
+    name = _FORMAT_OF.get(scales.dtype)
+    if name is not None:
+        return name
     raise TypeError(f"4-bit scales are float8_e4m3fn (nvfp4) or uint8 (mxfp4), not {scales.dtype}")
 
 
@@ -49,29 +50,28 @@ def fp4_quant(x: torch.Tensor, format: str = "nvfp4", global_scale: Optional[tor
     power of two that is at least ``amax / 6`` (byte 0 for a block of zeros).  A code is the nearest of
     ``value / scale``, ties to even.  A block that holds a NaN or an infinity gets the NaN scale and
     reads back as NaNs."""
-    if format not in FORMATS:
+    spec = FORMATS.get(format)
+    if spec is None:
         raise ValueError(f"unknown 4-bit format {format!r}: nvfp4 or mxfp4")
-    code, block, scale_dtype = FORMATS[format]
+    code, block, scale_dtype = spec
     if not x.is_cuda:
         raise ValueError("boltops_b200 kernels need CUDA tensors (there is no CPU path)")
     if x.dtype not in _FLOATS:
         raise TypeError(f"fp4_quant takes bf16, fp16 or fp32, not {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] % block:
+    shape, dev = x.shape, x.device
+    if len(shape) < 1 or shape[-1] % block:
         raise ValueError(f"the last dimension must be whole blocks of {block} values ({format})")
-    g = check_global_scale("global_scale", global_scale, format, 1, x.device)
-    x = x.contiguous()
-    if x.data_ptr() % 16:
-        x = x.clone()
-    cols = x.shape[-1]
-    codes = torch.empty((*x.shape[:-1], cols // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*x.shape[:-1], cols // block), dtype=scale_dtype, device=x.device)
-    if x.numel() == 0:
-        return codes, scales
-    with _cabi.on_device(x.device):
-        check(_cabi.load().bolt_fp4_quant(ptr(x), dtype_code(x.dtype), x.numel() // cols, cols, code,
-                                          ptr(g), ptr(codes), ptr(scales), stream_of(x)))
-    from .fused_moe import ops
-    ops._count()
+    g = check_global_scale("global_scale", global_scale, format, 1, dev)
+    cols = shape[-1]
+    lead = shape[:-1]
+    codes = torch.empty((*lead, cols // 2), dtype=torch.uint8, device=dev)
+    scales = torch.empty((*lead, cols // block), dtype=scale_dtype, device=dev)
+    n = x.numel()
+    if n:
+        x = ops.aligned(x)
+        _cabi.call(dev, _cabi.load().bolt_fp4_quant, x.data_ptr(), _FLOATS[x.dtype], n // cols, cols, code,
+                   ptr(g), codes.data_ptr(), scales.data_ptr(), stream_of(x))
+        ops._count()
     return codes, scales
 
 
@@ -91,19 +91,18 @@ def fp4_dequant(codes: torch.Tensor, scales: torch.Tensor, global_scale: Optiona
     if scales.device != codes.device:
         raise ValueError(f"scales are on {scales.device}, codes on {codes.device}")
     g = check_global_scale("global_scale", global_scale, format, 1, codes.device)
-    codes, scales = codes.contiguous(), scales.contiguous()
-    if codes.data_ptr() % 4:
-        codes = codes.clone()
     cols = 2 * codes.shape[-1]
     out = torch.empty((*codes.shape[:-1], cols), dtype=dtype, device=codes.device)
-    if out.numel() == 0:
-        return out
-    with _cabi.on_device(codes.device):
-        check(_cabi.load().bolt_fp4_dequant(ptr(codes), ptr(scales), out.numel() // cols, cols, code,
-                                            ptr(g), ptr(out), dtype_code(dtype), stream_of(codes)))
-    from .fused_moe import ops
-    ops._count()
+    n = out.numel()
+    if n:
+        codes, scales = ops.aligned(codes, 4), ops.aligned(scales, 1)
+        _cabi.call(out.device, _cabi.load().bolt_fp4_dequant, codes.data_ptr(), scales.data_ptr(), n // cols, cols,
+                   code, ptr(g), out.data_ptr(), _FLOATS[dtype], stream_of(out))
+        ops._count()
     return out
 
 
 __all__ = ["fp4_quant", "fp4_dequant"]
+
+# (last: the package imports this module's definitions)
+from .fused_moe import ops  # noqa: E402

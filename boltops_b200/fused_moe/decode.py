@@ -15,6 +15,7 @@ and with them the codes of values that lie on the border of two.
 """
 from __future__ import annotations
 
+import functools
 from typing import List, Optional
 
 import torch
@@ -27,6 +28,15 @@ from .activation import normalize_moe_activation, resolve_kernel
 MAX_TOKENS = 32
 _FLOAT_OUT = (torch.float16, torch.bfloat16, torch.float32)
 _16BIT = (torch.bfloat16, torch.float16)
+
+
+@functools.lru_cache(maxsize=64)
+def gated_activation(activation, gemm1_alpha, gemm1_limit, situ_beta, situ_linear_beta):
+    """(kernel activation, alpha, limit) of a gated activation on [gate | up] rows."""
+    activation, is_gated = normalize_moe_activation("silu" if activation is None else activation)
+    if not is_gated or activation == "swigluoai":
+        raise NotImplementedError("gated activations on [gate | up] rows only")
+    return resolve_kernel(activation, True, gemm1_alpha, gemm1_limit, situ_beta, situ_linear_beta)
 
 
 def _kind(w1, w1_scale, use_fp8_w8a8, use_int8_w8a8, use_fp4_w4a4, per_channel_quant, block_shape) -> int:
@@ -150,11 +160,8 @@ def _decode(hidden_states, w1, w2, topk_weights, topk_ids, gating, topk, renorma
         expert_map = expert_map.to(torch.int32).contiguous()
     elif global_num_experts == -1:
         global_num_experts = e
-    activation, is_gated = normalize_moe_activation("silu" if activation is None else activation)
-    if not is_gated or activation == "swigluoai":
-        raise NotImplementedError("gated activations on [gate | up] rows only")
-    act, alpha, limit = resolve_kernel(activation, True, gemm1_alpha, gemm1_limit, activation_situ_beta,
-                                       activation_situ_linear_beta)
+    act, alpha, limit = gated_activation(activation, gemm1_alpha, gemm1_limit, activation_situ_beta,
+                                         activation_situ_linear_beta)
     out_dtype = hidden_states.dtype if output_dtype is None else output_dtype
     if out_dtype not in _FLOAT_OUT:
         raise ValueError("output_dtype must be bf16, fp16 or fp32")
@@ -164,7 +171,6 @@ def _decode(hidden_states, w1, w2, topk_weights, topk_ids, gating, topk, renorma
             or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {out_dtype} [{m}, {model_dim}] on {dev}")
 
-    args = _cabi.DecodeArgs()
     keep = []
     if gating is not None:
         if gating.dim() != 2 or tuple(gating.shape) != (m, global_num_experts) or gating.device != dev:
@@ -176,8 +182,8 @@ def _decode(hidden_states, w1, w2, topk_weights, topk_ids, gating, topk, renorma
         if not 1 <= topk <= min(32, global_num_experts):
             raise ValueError(f"topk {topk} out of range")
         gating = gating.contiguous()
-        args.gating, args.gating_dtype = gating.data_ptr(), _cabi.dtype_code(gating.dtype)
-        args.renormalize, args.is_softmax = int(renormalize), int(is_softmax)
+        routing = (None, None, gating.data_ptr(), _cabi.dtype_code(gating.dtype), int(renormalize),
+                   int(is_softmax))
     else:
         if topk_ids.dim() != 2 or topk_weights.shape != topk_ids.shape or topk_ids.shape[0] != m:
             raise ValueError("topk_weights and topk_ids must both be [tokens, topk]")
@@ -189,40 +195,35 @@ def _decode(hidden_states, w1, w2, topk_weights, topk_ids, gating, topk, renorma
             raise ValueError(f"topk {topk} out of range")
         ids = topk_ids.to(torch.int32).contiguous()
         wts = topk_weights.to(torch.float32).contiguous()
-        keep += [ids, wts]
-        args.topk_ids, args.topk_weights = ids.data_ptr(), wts.data_ptr()
+        routing = (wts.data_ptr(), ids.data_ptr(), None, 0, 0, 0)
     if m == 0:
         return out
 
     x = ops.aligned(hidden_states)
     w1, w2 = ops.aligned(w1), ops.aligned(w2)
-    args.kind, args.x_dtype, args.out_dtype = kind, _cabi.dtype_code(x.dtype), _cabi.dtype_code(out_dtype)
-    args.num_tokens, args.topk = m, topk
-    args.hidden, args.inter, args.model_dim = hidden, inter, model_dim
-    args.num_experts, args.global_num_experts = e, global_num_experts
-    args.hidden_states, args.w1, args.w2 = x.data_ptr(), w1.data_ptr(), w2.data_ptr()
+    s1 = s2 = None
     if w1_scale is not None:
         w1_scale, w2_scale = ops.aligned(w1_scale), ops.aligned(w2_scale)
-        args.w1_scale, args.w2_scale = w1_scale.data_ptr(), w2_scale.data_ptr()
+        s1, s2 = w1_scale.data_ptr(), w2_scale.data_ptr()
+    whole = (None, None, None, None)
     if fp4:
-        for name, t, n in (("w1_global_scale", w1_global_scale, e), ("w2_global_scale", w2_global_scale, e),
-                           ("a1_global_scale", a1_global_scale, 1), ("a2_global_scale", a2_global_scale, 1)):
-            t = check_global_scale(name, t, fmt, n, dev)
-            keep.append(t)
-            setattr(args, name, _cabi.ptr(t))
-    args.expert_map = _cabi.ptr(expert_map)
-    args.activation, args.act_alpha, args.act_limit = act, alpha, limit
-    args.routed_scaling_factor = 1.0 if routed_scaling_factor is None else float(routed_scaling_factor)
-    args.out = out.data_ptr()
-    args.status = ops.device_status(dev).data_ptr()
+        keep = [check_global_scale(name, t, fmt, n, dev) for name, t, n in (
+            ("w1_global_scale", w1_global_scale, e), ("w2_global_scale", w2_global_scale, e),
+            ("a1_global_scale", a1_global_scale, 1), ("a2_global_scale", a2_global_scale, 1))]
+        whole = tuple(_cabi.ptr(t) for t in keep)
     lib = _cabi.load()
+    args = _cabi.DecodeArgs(
+        kind, _cabi.dtype_code(x.dtype), _cabi.dtype_code(out_dtype), m, topk, hidden, inter, model_dim, e,
+        global_num_experts, x.data_ptr(), w1.data_ptr(), w2.data_ptr(), s1, s2, *whole, *routing,
+        _cabi.ptr(expert_map), act, alpha, limit,
+        1.0 if routed_scaling_factor is None else float(routed_scaling_factor), out.data_ptr(), None, 0,
+        ops.device_status(dev).data_ptr(), 0)
     need = lib.bolt_moe_decode_workspace_bytes(args)
     if need == 0:
         _cabi.check(1)
     workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     args.workspace, args.workspace_bytes = workspace.data_ptr(), need
-    with _cabi.on_device(dev):
-        _cabi.check(lib.bolt_moe_decode(args, _cabi.stream_of(x)))
+    _cabi.call(dev, lib.bolt_moe_decode, args, _cabi.stream_of(x))
     ops._count(2)
     return out
 

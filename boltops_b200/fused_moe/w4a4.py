@@ -17,8 +17,7 @@ import torch
 from .. import _cabi
 from ..fp4 import FORMATS, check_global_scale, format_of, fp4_quant
 from . import ops
-from .activation import normalize_moe_activation, resolve_kernel
-from .decode import check_weights
+from .decode import check_weights, gated_activation
 
 _FLOAT_OUT = (torch.float16, torch.bfloat16, torch.float32)
 
@@ -75,11 +74,8 @@ def fused_experts_fp4(
     for name, t in (("topk_weights", topk_weights), ("topk_ids", topk_ids), ("expert_map", expert_map)):
         if t is not None and t.device != dev:
             raise ValueError(f"{name} is on {t.device}, hidden_states on {dev}")
-    activation, is_gated = normalize_moe_activation("silu" if activation is None else activation)
-    if not is_gated or activation == "swigluoai":
-        raise NotImplementedError("gated activations on [gate | up] rows only")
-    act, alpha, limit = resolve_kernel(activation, True, gemm1_alpha, gemm1_limit, activation_situ_beta,
-                                       activation_situ_linear_beta)
+    act, alpha, limit = gated_activation(activation, gemm1_alpha, gemm1_limit, activation_situ_beta,
+                                         activation_situ_linear_beta)
     out_dtype = hidden_states.dtype if output_dtype is None else output_dtype
     if out_dtype not in _FLOAT_OUT:
         raise ValueError("output_dtype must be bf16, fp16 or fp32")

@@ -103,7 +103,15 @@ w8a8_triton_block_scaled_mm = w8a8_block_scaled_mm
 w8a8_block_int8_matmul = w8a8_block_scaled_mm
 
 
+# The few-row form reads the weights once at up to half of HBM's rate and computes on small matrix
+# instructions, one column tile per eight rows; the tiled form has a launch more and whole 128-row tiles.
+# Both measured in us, few / tiled: nvfp4 4096 x 7168, 1 row 8.0 / 21.7, 16 11.0 / 22.5, 32 16.7 / 22.6;
+# 7168 x 2048, 32 rows 12.1 / 12.8; 28672 x 8192, 1 row 43.0 / 41.8, 12 58.8 / 39.5; mxfp4 4096 x 7168, 1 row
+# 10.8 / 20.5, 16 14.3 / 20.5, 32 22.6 / 20.7; 7168 x 2048, 16 rows 10.3 / 11.6, 24 13.2 / 11.7; 28672 x
+# 8192, 1 row 59.0 / 37.7.  (Where they are close, the launch saved is worth more to a caller whose
+# kernels wait for its host.)
 _FEW_ROWS = 32
+_FEW_WEIGHTS = 128 << 20
 
 
 def gemm_a4w4(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor, w_scale: torch.Tensor,
@@ -136,9 +144,11 @@ def gemm_a4w4(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor, w_scale: 
     if k == 0 or k % (4 * block):
         raise NotImplementedError(f"K {k} must be a multiple of {4 * block} ({fmt})")
     dev = x.device
-    for name, t in (("w", w), ("x_scale", x_scale), ("w_scale", w_scale), ("alpha", alpha), ("out", out)):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, x on {dev}")
+    if w.device != dev or x_scale.device != dev or w_scale.device != dev or \
+            (alpha is not None and alpha.device != dev) or (out is not None and out.device != dev):
+        for name, t in (("w", w), ("x_scale", x_scale), ("w_scale", w_scale), ("alpha", alpha), ("out", out)):
+            if t is not None and t.device != dev:
+                raise ValueError(f"{name} is on {t.device}, x on {dev}")
     if alpha is not None and (alpha.numel() != 1 or alpha.dtype != torch.float32):
         raise ValueError("alpha must be one float32 value")
     if out is None:
@@ -148,19 +158,16 @@ def gemm_a4w4(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor, w_scale: 
         raise ValueError(f"out must be [{m}, {n}] in {dtype} with a dense last dimension")
     if m == 0 or n == 0:
         return out
-    x, w, x_scale, w_scale = (ops.aligned(t) for t in (x, w, x_scale, w_scale))
+    x, w = ops.aligned(x), ops.aligned(w)
+    x_scale, w_scale = ops.aligned(x_scale), ops.aligned(w_scale)
     lib = _cabi.load()
     stream = _cabi.stream_of(x)
-    if m <= _FEW_ROWS:
-        few = _cabi.Fp4FewArgs()
-        few.format, few.rows, few.n, few.k = code, m, n, k
-        few.x, few.x_scale, few.w, few.w_scale = (t.data_ptr() for t in (x, x_scale, w, w_scale))
-        few.alpha, few.out, few.out_dtype = _cabi.ptr(alpha), out.data_ptr(), _cabi.dtype_code(dtype)
-        few.out_ld = out.stride(0) if m > 1 else n
-        few.status = ops.device_status(dev).data_ptr()
-        few.sm_count = ops.gemm_sm_count(dev)
-        with _cabi.on_device(dev):
-            _cabi.check(lib.bolt_fp4_gemm_few(few, stream))
+    out_ld = out.stride(0) if m > 1 else n
+    if m <= _FEW_ROWS and n * k <= _FEW_WEIGHTS:
+        few = _cabi.Fp4FewArgs(code, m, n, k, x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
+                               _cabi.ptr(alpha), out.data_ptr(), _cabi.dtype_code(dtype), out_ld,
+                               ops.device_status(dev).data_ptr(), ops.gemm_sm_count(dev))
+        _cabi.call(dev, lib.bolt_fp4_gemm_few, few, stream)
         ops._count()
         return out
     args = _cabi.Fp4GemmArgs()
@@ -177,11 +184,10 @@ def gemm_a4w4(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor, w_scale: 
     args.a, args.b = x.data_ptr(), w.data_ptr()
     args.a_tiles, args.b_tiles = lay.job[0].dst, lay.job[1].dst
     args.alpha = _cabi.ptr(alpha)
-    args.c, args.c_dtype, args.c_ld = out.data_ptr(), _cabi.dtype_code(dtype), out.stride(0) if m > 1 else n
+    args.c, args.c_dtype, args.c_ld = out.data_ptr(), _cabi.dtype_code(dtype), out_ld
     args.status = ops.device_status(dev).data_ptr()
     args.sm_count = ops.gemm_sm_count(dev)
-    with _cabi.on_device(dev):
-        _cabi.check(lib.bolt_fp4_tile_scales(lay, stream))
-        _cabi.check(lib.bolt_fp4_gemm(args, stream))
+    _cabi.call(dev, lib.bolt_fp4_tile_scales, lay, stream)
+    _cabi.call(dev, lib.bolt_fp4_gemm, args, stream)
     ops._count(2)
     return out
