@@ -21,6 +21,7 @@
 // quantised experts keep fp32 up to their quantiser.  All sums are fp32, rounded once at the end.
 #include <cuda.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "act_pair.cuh"
@@ -360,7 +361,9 @@ constexpr int kDownBoxBytes = kMaxRows * 128;
 constexpr int up_scale_bytes(int k) {      // of a slot
   return k == K_NV4 ? 512 : k == K_MX4 ? 512 : is_block(k) ? 64 : 0;
 }
-constexpr int warps_of(int k, int nt) { return nt == 4 || k == K_MX4 ? 8 : 16; }
+constexpr int warps_of(int k, int nt) { return nt == 4 || (k == K_MX4 && nt == 2) ? 8 : 16; }
+// blocks an SM holds as far as registers go: the second kernel's beside the first's
+constexpr int blocks_of(int nt, int warps) { return nt == 1 && warps == 8 ? 2 : 1; }
 constexpr int red_bytes(int warps, int mt, int nt) { return warps * mt * nt * 128 * 4; }
 // bytes of a kept row of codes: 16 more than it has, so that eight rows lie in different banks
 __host__ __device__ constexpr int code_pitch(int k, int n) { return (int)row_bytes(k, n) + 16; }
@@ -402,10 +405,10 @@ __device__ __forceinline__ void keep_codes(int w0, int wn, int lane, int rows, i
 // ---------------------------------------------------------------------------
 // gate and up projections, activation
 // ---------------------------------------------------------------------------
-template <int K, int NT>
-__global__ void __launch_bounds__(32 * warps_of(K, NT), 1)
+template <int K, int NT, int W>
+__global__ void __launch_bounds__(32 * W, blocks_of(NT, W))
 k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
-  constexpr int MT = up_tiles(K), kBox = up_box_bytes(K), kWarps = warps_of(K, NT), kThreads = 32 * kWarps;
+  constexpr int MT = up_tiles(K), kBox = up_box_bytes(K), kWarps = W;
   constexpr int kCols = 8 * MT;       // columns a unit may have
   // rows of scales: of every gate and up row of a thread (4-bit), of the unit's gate and up block
   using Scales = ScaleRing<is_channel(K) ? (int)K_BF16 : K, is4(K) ? 2 * MT : 2>;
@@ -752,10 +755,10 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
 // ---------------------------------------------------------------------------
 // down projection, sum over a token's experts
 // ---------------------------------------------------------------------------
-template <int K, int NT>
-__global__ void __launch_bounds__(32 * warps_of(K, NT), 1)
+template <int K, int NT, int W>
+__global__ void __launch_bounds__(32 * W, blocks_of(NT, W))
 k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
-  constexpr int MT = kDownTiles, kBox = kDownBoxBytes, kWarps = warps_of(K, NT), kThreads = 32 * kWarps;
+  constexpr int MT = kDownTiles, kBox = kDownBoxBytes, kWarps = W, kThreads = 32 * kWarps;
   const int UR = p.unit;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = carve(raw);
@@ -1187,8 +1190,8 @@ int unit_size(int total, int most, int64_t copies, int blocks, int step = 1) {
   return best;
 }
 
-// Warps to a unit: as many as have four boxes of its reduction each.  With fewer boxes a warp, the end of
-// a unit (sums over the warps, activation) is not covered by other units' copies.
+// Warps that share a unit: as many as have four boxes of its reduction each.  With fewer boxes a warp, the
+// end of a unit (sums over the warps, activation) is not covered by other groups' boxes.
 int group_warps(int warps, int boxes) {
   while (warps > 1 && boxes < 4 * warps) warps /= 2;
   return warps;
@@ -1203,14 +1206,14 @@ void workspace_parts(const bolt_decode_args* a, size_t (&part)[3]) {
   part[2] = is_channel(k) ? a256(slots * ((a->inter + kMinUnit - 1) / kMinUnit) * 4) : 0;
 }
 
-constexpr int kSmem = 226 * 1024;   // of a block
-int ring_slots(int fixed, int slot_bytes, int warps) {
-  int slots = (kSmem - fixed) / (warps * slot_bytes);
+constexpr int kSmem = 226 * 1024, kHalfSmem = 113 * 1024;   // of a block, of one of two on an SM
+int ring_slots(int smem, int fixed, int slot_bytes, int warps) {
+  int slots = (smem - fixed) / (warps * slot_bytes);
   return slots * warps > kMaxBarriers ? kMaxBarriers / warps : slots;
 }
-template <int K, int NT>
-int launch(const bolt_decode_args* a, Params p, cudaStream_t st) {
-  constexpr int kWarps = warps_of(K, NT);
+template <int K, int NT, int kWarps>
+int launch(const bolt_decode_args* a, Params p, int blocks, cudaStream_t st) {
+  constexpr int kSmem = blocks_of(NT, kWarps) == 2 ? kHalfSmem : bolt::few::kSmem;
   constexpr int kUpSlot = up_box_bytes(K) + up_scale_bytes(K), kDownSlot = kDownBoxBytes + ScaleRing<K, 2 * kDownTiles>::kBytes;
   const int routes = p.tokens * p.topk;
   int up = 1024 + kCtrlBytes + red_bytes(kWarps, up_tiles(K), NT) + a16(route_bytes(p.experts, routes));
@@ -1232,21 +1235,21 @@ int launch(const bolt_decode_args* a, Params p, cudaStream_t st) {
     p.keep_act = down + stage + act_kept + 2 * kWarps * kDownSlot <= kSmem;
     down += stage + (p.keep_act ? (int)act_kept : 0);
   }
-  const int up_slots = ring_slots(up, kUpSlot, kWarps), down_slots = ring_slots(down, kDownSlot, kWarps);
+  const int up_slots = ring_slots(kSmem, up, kUpSlot, kWarps),
+            down_slots = ring_slots(kSmem, down, kDownSlot, kWarps);
   if (up_slots < 1 || down_slots < 1) {
     set_error("moe_decode: %d tokens of hidden size %d do not fit in shared memory", p.tokens, p.hidden);
     return BOLT_ERR_UNSUPPORTED;
   }
   static std::atomic<bool> ready[2][kMaxDevices];
-  int rc = configure_kernel(k_few_up<K, NT>, kSmem, ready[0], 0, 0, 0, 0);
-  if (rc == BOLT_OK) rc = configure_kernel(k_few_down<K, NT>, kSmem, ready[1], 0, 0, 0, 0);
+  int rc = configure_kernel(k_few_up<K, NT, kWarps>, kSmem, ready[0], 0, 0, 0, 0);
+  if (rc == BOLT_OK) rc = configure_kernel(k_few_down<K, NT, kWarps>, kSmem, ready[1], 0, 0, 0, 0);
   if (rc != BOLT_OK) return rc;
 
-  const int sms = a->sm_count > 0 ? a->sm_count : sm_count_of_current_device();
   const int columns = is4(K) ? 8 * up_tiles(K)
-                             : unit_size(p.inter, 8 * up_tiles(K), routes < p.experts ? routes : p.experts, sms,
+                             : unit_size(p.inter, 8 * up_tiles(K), routes < p.experts ? routes : p.experts, blocks,
                                          is_block(K) ? 8 : 1);
-  const int rows = unit_size(p.model_dim, kMaxRows, 1, sms);
+  const int rows = unit_size(p.model_dim, kMaxRows, 1, blocks);
   CUtensorMap m1, m2;
   {
     const cuuint64_t kb = (cuuint64_t)row_bytes(K, p.hidden), i = p.inter;
@@ -1266,12 +1269,12 @@ int launch(const bolt_decode_args* a, Params p, cudaStream_t st) {
   p.slots_per_warp = up_slots;
   p.unit = columns;
   p.group_warps = group_warps(kWarps, (int)((row_bytes(K, p.hidden) + 127) / 128));
-  k_few_up<K, NT><<<sms, 32 * kWarps, up + up_slots * kWarps * kUpSlot, st>>>(m1, p);
+  k_few_up<K, NT, kWarps><<<blocks, 32 * kWarps, up + up_slots * kWarps * kUpSlot, st>>>(m1, p);
   BOLT_LAUNCH_CHECK();
   p.slots_per_warp = down_slots;
   p.unit = rows;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(sms);
+  cfg.gridDim = dim3(blocks);
   cfg.blockDim = dim3(32 * kWarps);
   cfg.dynamicSmemBytes = down + down_slots * kWarps * kDownSlot;
   cfg.stream = st;
@@ -1280,15 +1283,27 @@ int launch(const bolt_decode_args* a, Params p, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  BOLT_CUDA(cudaLaunchKernelEx(&cfg, k_few_down<K, NT>, m2, p));
+  BOLT_CUDA(cudaLaunchKernelEx(&cfg, k_few_down<K, NT, kWarps>, m2, p));
   return BOLT_OK;
 }
 
+// Blocks of eight warps and half an SM's shared memory where a block's share of the weights is small: the
+// second kernel then starts beside the first, and its routing and first copies cost nothing.  SMALLNOTE
+constexpr int64_t kSmallShare = 256 << 10;
 template <int K>
 int launch_kind(const bolt_decode_args* a, const Params& p, cudaStream_t st) {
-  if (p.tokens <= 8) return launch<K, 1>(a, p, st);
-  if (p.tokens <= 16) return launch<K, 2>(a, p, st);
-  return launch<K, 4>(a, p, st);
+  const int sms = a->sm_count > 0 ? a->sm_count : sm_count_of_current_device();
+  const int64_t touched = std::min<int64_t>((int64_t)p.tokens * p.topk, p.experts);
+  const int64_t share = touched * (2 * p.inter * row_bytes(K, p.hidden) + p.model_dim * row_bytes(K, p.inter)) / sms;
+  if (p.tokens <= 8) {
+    if (share <= kSmallShare) {
+      const int rc = launch<K, 1, 8>(a, p, sms, st);
+      if (rc != BOLT_ERR_UNSUPPORTED) return rc;      // (too many or too long rows for half an SM)
+    }
+    return launch<K, 1, warps_of(K, 1)>(a, p, sms, st);
+  }
+  if (p.tokens <= 16) return launch<K, 2, warps_of(K, 2)>(a, p, sms, st);
+  return launch<K, 4, 8>(a, p, sms, st);
 }
 
 template <int K, int NT>
@@ -1299,7 +1314,7 @@ int launch_dense(const bolt_fp4_few_args* a, DenseParams p, int sms, cudaStream_
   if (rc != BOLT_OK) return rc;
   const int fixed = 1024 + kCtrlBytes + red_bytes(kWarps, kDownTiles, NT);
   constexpr int kSlot = kDownBoxBytes + ScaleRing<K, 2 * kDownTiles>::kBytes;
-  p.slots_per_warp = ring_slots(fixed, kSlot, kWarps);
+  p.slots_per_warp = ring_slots(kSmem, fixed, kSlot, kWarps);
   p.unit = unit_size(p.n, kMaxRows, 1, sms);
   const cuuint64_t kb = (cuuint64_t)p.k / 2;
   const cuuint64_t size[3] = {kb, (cuuint64_t)p.n, 1}, strides[2] = {kb, kb * p.n};
