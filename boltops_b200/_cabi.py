@@ -14,7 +14,7 @@ import torch
 _PKG = Path(__file__).resolve().parent
 _LIB_PATH = Path(os.environ.get("BOLTOPS_B200_LIB", _PKG / "lib" / "libboltops_b200.so"))
 
-BOLT_OK = 0
+BOLT_OK, BOLT_ERR_UNSUPPORTED = 0, 3
 # enum bolt_dtype
 BF16, F16, F32, FP8_E4M3, INT8 = 0, 1, 2, 3, 4
 # enum bolt_activation

@@ -1367,9 +1367,10 @@ extern "C" size_t bolt_moe_decode_workspace_bytes(const bolt_decode_args* a) {
   return part[0] + part[1] + part[2] + 256;
 }
 
-extern "C" int bolt_moe_decode(const bolt_decode_args* a, void* stream) {
-  using namespace bolt;
-  using namespace bolt::few;
+namespace bolt {
+namespace few {
+namespace {
+int decode_once(const bolt_decode_args* a, cudaStream_t st) {
   int rc = check_args(a);
   if (rc != BOLT_OK) return rc;
   if (a->num_tokens == 0) return BOLT_OK;
@@ -1428,7 +1429,6 @@ extern "C" int bolt_moe_decode(const bolt_decode_args* a, void* stream) {
   p.act_amax = reinterpret_cast<float*>(p.act_sf + part[1]);
   p.status = a->status;
 
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (k) {
     case K_BF16: return launch_kind<K_BF16>(a, p, st);
     case K_F16: return launch_kind<K_F16>(a, p, st);
@@ -1439,6 +1439,34 @@ extern "C" int bolt_moe_decode(const bolt_decode_args* a, void* stream) {
     case K_NV4: return launch_kind<K_NV4>(a, p, st);
     default: return launch_kind<K_MX4>(a, p, st);
   }
+}
+}  // namespace
+}  // namespace few
+}  // namespace bolt
+
+extern "C" int bolt_moe_decode(const bolt_decode_args* a, void* stream) {
+  using namespace bolt;
+  using namespace bolt::few;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int rc = decode_once(a, st);
+  if (rc != BOLT_ERR_UNSUPPORTED || a->num_tokens < 2) return rc;
+  // the 4-bit codes of all rows do not fit in shared memory: half of the tokens after the other (they read
+  // the experts that both touch twice)
+  bolt_decode_args part = *a;
+  part.num_tokens = a->num_tokens / 2;
+  const int first = bolt_moe_decode(&part, stream);
+  if (first != BOLT_OK) return first;
+  const int64_t done = part.num_tokens;
+  part.num_tokens = a->num_tokens - part.num_tokens;
+  part.hidden_states = static_cast<const uint8_t*>(a->hidden_states) + done * a->hidden * 2;
+  if (a->gating != nullptr) {
+    part.gating = static_cast<const uint8_t*>(a->gating) + done * a->global_num_experts * dtype_bytes(a->gating_dtype);
+  } else {
+    part.topk_ids = a->topk_ids + done * a->topk;
+    part.topk_weights = a->topk_weights + done * a->topk;
+  }
+  part.out = static_cast<uint8_t*>(a->out) + done * a->model_dim * dtype_bytes(a->out_dtype);
+  return bolt_moe_decode(&part, stream);
 }
 
 extern "C" int bolt_fp4_gemm_few(const bolt_fp4_few_args* a, void* stream) {

@@ -223,7 +223,11 @@ def _decode(hidden_states, w1, w2, topk_weights, topk_ids, gating, topk, renorma
         _cabi.check(1)
     workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     args.workspace, args.workspace_bytes = workspace.data_ptr(), need
-    _cabi.call(dev, lib.bolt_moe_decode, args, _cabi.stream_of(x))
+    with _cabi.on_device(dev):
+        status = lib.bolt_moe_decode(args, _cabi.stream_of(x))
+    if status == _cabi.BOLT_ERR_UNSUPPORTED:
+        raise NotImplementedError(lib.bolt_last_error().decode(errors="replace"))
+    _cabi.check(status)
     ops._count(2)
     return out
 
@@ -262,8 +266,10 @@ def fused_experts_decode(
     ``use_fp4_w4a4``: weights and scales as ``fused_experts_fp4`` takes them.  Routes whose id is out of
     range or not local under ``expert_map`` add nothing; a token with none gives zeros; an expert
     that a token names twice counts with the sum of its weights.  ``out``: a contiguous buffer for
-    the result.  Raises ``NotImplementedError`` above 32 tokens and for sizes that are not multiples of
-    8 (16-bit), 16 (per-channel), 64 (nvfp4) or 128 (block-scaled, mxfp4)."""
+    the result.  Raises ``NotImplementedError`` above 32 tokens, for sizes that are not multiples of 8
+    (16-bit), 16 (per-channel), 64 (nvfp4) or 128 (block-scaled, mxfp4).  (Four-bit rows whose codes do not
+    all fit in shared memory, 32 tokens above about 5000 hidden columns, go in two or more pairs of
+    kernels.)"""
     return _decode(hidden_states, w1, w2, topk_weights, topk_ids, None, 0, False, True,
                    use_fp8_w8a8=use_fp8_w8a8, use_int8_w8a8=use_int8_w8a8, use_fp4_w4a4=use_fp4_w4a4,
                    per_channel_quant=per_channel_quant, block_shape=block_shape, w1_scale=w1_scale,

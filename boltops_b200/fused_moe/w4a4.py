@@ -87,6 +87,8 @@ def fused_experts_fp4(
         ("a1_global_scale", a1_global_scale, 1), ("a2_global_scale", a2_global_scale, 1)))
     if global_num_experts == -1:
         global_num_experts = expert_map.numel() if expert_map is not None else e
+    if expert_map is None and global_num_experts != e:
+        raise ValueError(f"{global_num_experts} experts, weights of {e}: an expert_map has to say which are local")
     if expert_map is not None and expert_map.numel() != global_num_experts:
         raise ValueError("expert_map must have one entry per expert")
     topk = topk_ids.shape[1]
@@ -95,7 +97,10 @@ def fused_experts_fp4(
         return out.zero_()
     scale = 1.0 if routed_scaling_factor is None else float(routed_scaling_factor)
     w1, w2, w1_scale, w2_scale = (ops.aligned(t) for t in (w1, w2, w1_scale, w2_scale))
-    mask = (expert_map >= 0).to(torch.int32) if expert_map is not None else None
+    mask = None
+    if expert_map is not None:
+        local = (expert_map >= 0) & (expert_map < e)
+        expert_map, mask = torch.where(local, expert_map, -1), local.to(torch.int32)
     ids_all, wts_all = topk_ids.to(torch.int32), topk_weights.to(torch.float32)
     lib = _cabi.load()
     from .layer import _chunk_size

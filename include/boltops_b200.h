@@ -729,7 +729,8 @@ typedef struct bolt_decode_args {
   int sm_count;                /* SMs to use; 0: all                                          */
 } bolt_decode_args;
 
-/* Two kernels on the stream (no sort, no copies of rows).  Sizes: hidden and inter multiples of 8
+/* Two kernels on the stream (no sort, no copies of rows; 4-bit rows of more tokens than fit in shared memory
+ * go half by half).  Sizes: hidden and inter multiples of 8
  * (16-bit), 16 (per-channel), 128 (block-scaled, MX) or 64 (NV); block-scaled model_dim a multiple of 128. */
 size_t bolt_moe_decode_workspace_bytes(const bolt_decode_args* args);
 int bolt_moe_decode(const bolt_decode_args* args, void* stream);

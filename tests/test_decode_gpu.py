@@ -244,3 +244,37 @@ def test_strided_rows_weights_off_the_grid_and_no_tokens():
     assert torch.equal(fused_experts_decode(view, d1, d2.transpose(1, 2).contiguous().transpose(1, 2), weights, ids),
                        want)
     assert fused_experts_decode(view[:0], d1, d2, weights[:0], ids[:0]).shape == (0, 256)
+
+
+def test_long_rows_many_tokens():
+    """Where kept codes do not fit: 8-bit rows are quantised box by box, 4-bit ones go half by half."""
+    for m, h in ((8, 32768), (24, 9216)):
+        x = rows("fp8_block", m, h, 2) * 0.05
+        run("fp8_block", 2, h, 128, m, 1, hout=128, x=x)
+        run("int8_channel", 2, h, 128, m, 1, hout=128, x=x)
+    for kind, m, h in (("nvfp4", 32, 16384), ("mxfp4", 27, 8192)):
+        run(kind, 2, h, 128, m, 1, hout=64, x=rows(kind, m, h, 1) * 0.05)
+    w1, w2 = experts("mxfp4", 2, 8192, 128, 64)
+    d1, d2, kw = arguments("mxfp4", w1, w2)
+    x, logits = rows("mxfp4", 27, 8192, 1).cuda(), torch.randn(27, 2, device="cuda")
+    weights, ids = fused_topk(x, logits, 1, True)
+    assert torch.equal(fused_moe_decode(x, logits, d1, d2, 1, True, **kw),
+                       fused_experts_decode(x, d1, d2, weights, ids, **kw))
+
+
+def test_many_routes_and_experts():
+    """More routes than a warp has lanes, more experts than a block has threads."""
+    weights, ids = routing(32, 700, 8, 3)
+    for kind in ("bf16", "int8_channel"):
+        run(kind, 700, 64, 16, 32, 8, ids=ids, weights=weights)
+        run(kind, 700, 64, 16, 5, 7, ids=ids[:5, :7], weights=weights[:5, :7])
+
+
+def test_situ_and_step_activations():
+    def situ(g, u):
+        return 2.0 * torch.tanh(g / 2.0) * torch.sigmoid(g) * u
+
+    def step(g, u):
+        return (g * torch.sigmoid(g)).clamp(max=0.7) * u.clamp(-0.7, 0.7)
+    run("bf16", 4, 256, 128, 5, 2, activation="situ", activation_situ_beta=2.0, act=situ)
+    run("f16", 4, 256, 128, 5, 2, activation="swiglustep", gemm1_limit=0.7, act=step)

@@ -148,6 +148,10 @@ def test_layer_routing_maps_types_activations_and_chunks(fmt, monkeypatch):
     weights, ids = routing(40, 8, 3, 11)
     emap = torch.tensor([-1, 2, -1, 0, 1, -1, 3, -1], dtype=torch.int32)
     layer(fmt, 4, 256, 128, 40, 3, ids=ids, weights=weights, expert_map=emap.cuda())
+    # (an entry past the local experts is as good as none)
+    wild = torch.tensor([9, 2, -1, 0, 1, -7, 3, 4], dtype=torch.int32)
+    same = layer(fmt, 4, 256, 128, 40, 3, ids=ids, weights=weights, expert_map=emap.cuda())
+    assert torch.equal(layer(fmt, 4, 256, 128, 40, 3, ids=ids, weights=weights, expert_map=wild.cuda()), same)
     one = torch.full((200, 1), 2, dtype=torch.int32)
     layer(fmt, 4, 256, 128, 200, 1, ids=one, weights=torch.rand(200, 1))
     ids = torch.tensor([[1, 1, 3], [-1, 99, 2], [-1, -1, -5]], dtype=torch.int32)
