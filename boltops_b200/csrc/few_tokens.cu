@@ -56,7 +56,11 @@ struct Params {
   int amax_cols;            // units of an expert in the first kernel
   int unit;                 // columns (first kernel) or rows (second) of a unit
   int group_warps;          // warps that share a unit (first kernel)
-  int keep_x, keep_act;     // 8-bit codes of the rows, of the activations are made once and kept
+  // 8-bit codes of the rows, of the activations: made by every block in its shared memory, or read from
+  // k_few_codes' output: codes [rows][columns], scales [rows][groups] (block-scaled) or [rows]
+  int keep_x, keep_act;
+  uint8_t *xq, *aq;
+  float *xs, *as;
 };
 
 // ---------------------------------------------------------------------------
@@ -402,6 +406,46 @@ __device__ __forceinline__ void keep_codes(int w0, int wn, int lane, int rows, i
   }
 }
 
+// Rows to 8-bit codes in memory, a block a row: where the codes of all rows, or of all activations, do not fit
+// beside a block's rings.
+template <int K>
+__global__ void __launch_bounds__(256) k_few_codes(const void* src, int dt, int cols, uint8_t* codes, float* scales) {
+  __shared__ float top[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  let_next_start();
+  wait_for_previous();
+  const int64_t row = blockIdx.x;
+  const uint8_t* from = static_cast<const uint8_t*>(src) + row * cols * (dt == BOLT_F32 ? 4 : 2);
+  float scale = 1.f, inv = 1.f;
+  if constexpr (is_channel(K)) {
+    float amax = 0.f;
+    for (int c = 4 * threadIdx.x; c < cols; c += 1024) {
+      const float4 v = load_values4(from, dt, c);
+      amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+    }
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (lane == 0) top[warp] = amax;
+    __syncthreads();
+    amax = top[0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) amax = fmaxf(amax, top[w]);
+    scale8<K>(amax, scale, inv);
+    if (threadIdx.x == 0) scales[row] = scale;
+  }
+  const int groups = (cols + 127) / 128;
+  for (int kb = warp; kb < groups; kb += 8) {
+    const int c = kb * 128 + 4 * lane;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c < cols) v = load_values4(from, dt, c);
+    if constexpr (is_block(K)) {
+      const float most = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+      scale8<K>(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most))), scale, inv);
+      if (lane == 0) scales[row * groups + kb] = scale;
+    }
+    if (c < cols) *reinterpret_cast<uint32_t*>(codes + row * cols + c) = codes4<K>(v, inv);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // gate and up projections, activation
 // ---------------------------------------------------------------------------
@@ -423,8 +467,6 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
   uint8_t* rest = smem + kWarps * p.slots_per_warp * kBox + kCtrlBytes;
   float* red = reinterpret_cast<float*>(rest);
   rest += red_bytes(kWarps, MT, NT);
-  uint8_t* stage = rest + warp * code_bytes(NT);
-  if (is8(K) && !p.keep_x) rest += kWarps * code_bytes(NT);
   let_next_start();
 
   uint8_t* const route_mem = rest;
@@ -436,14 +478,14 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
   uint8_t* x_codes = rest;                                 // [tokens][pitch], scales behind them
   const int pitch = code_pitch(K, p.hidden);
   uint8_t* x_sf = x_codes + p.tokens * pitch;              // 4-bit: bytes
-  float* x_scale = reinterpret_cast<float*>(x_sf);         // block-scaled: [hidden / 128][tokens]
+  float* x_scale = reinterpret_cast<float*>(x_sf);         // block-scaled: [tokens][hidden / 128]
   constexpr int kBlk = K == K_NV4 ? 16 : 32;
   const int sf_row = p.hidden / kBlk;
 
   // Q1 that needs whole rows, once per block.  In front of the first weights' copies: behind them a load
   // waits until they have all come.
   auto quantise = [&](int w0, int wn) {
-    if constexpr (is_channel(K)) {
+    if (is_channel(K) && p.keep_x) {
       for (int m = w0; m < p.tokens; m += wn) {
         const uint16_t* row = static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden;
         float amax = 0.f;
@@ -465,12 +507,12 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
         for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         if (lane == 0) scale8<K>(amax, row_scale[2 * m], row_scale[2 * m + 1]);
       }
-      if (p.keep_x) asm volatile("bar.sync 15, %0;" ::"r"(32 * wn) : "memory");
+      asm volatile("bar.sync 15, %0;" ::"r"(32 * wn) : "memory");
     }
     if (is8(K) && p.keep_x) {
       keep_codes<K>(w0, wn, lane, p.tokens, p.hidden, x_codes, pitch, [&](int m) {
         return static_cast<const void*>(static_cast<const uint16_t*>(p.x) + (int64_t)m * p.hidden); }, p.x_dtype,
-        [&](int m) { return row_scale[2 * m + 1]; }, [&](int m, int kb, float scale) { x_scale[kb * p.tokens + m] = scale; });
+        [&](int m) { return row_scale[2 * m + 1]; }, [&](int m, int kb, float scale) { x_scale[m * (p.hidden / 128) + kb] = scale; });
     }
     if constexpr (is4(K)) {
       const bool nv = K == K_NV4;
@@ -576,6 +618,10 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
   };
   for (int i = 0; i < p.slots_per_warp; ++i) bring();
 
+  if (is8(K) && !p.keep_x) wait_for_previous();      // k_few_codes
+  const uint8_t* xq = p.keep_x ? x_codes : p.xq;
+  const int xq_pitch = p.keep_x ? pitch : p.hidden;
+  const float* xs = p.keep_x ? x_scale : p.xs;
   int it = 0;
   Place unit = {first_u, first_u / per_expert, first_u % per_expert, 0};
   // (the group's own barrier, named 1 to 8; a warp by itself needs none)
@@ -612,17 +658,11 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
       const int kb = cur.kb;
 
       TokenBox<K> x[NT];
-      float xs = 1.f;
-      if (is8(K) && p.keep_x) {
+      if constexpr (is8(K)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           if ((live >> nt) & 1u)
-            load_token<K>(x[nt], tok[nt] < 0 ? nullptr : x_codes + tok[nt] * pitch, p.hidden, kb, t);
-      } else if constexpr (is8(K)) {
-        xs = quant_box<K, NT>(
-            x, stage, live_cols, p.x_dtype, p.hidden, kb * 128, lane,
-            [&](int c) { return static_cast<const uint16_t*>(p.x) + (int64_t)r.token[off + c] * p.hidden; },
-            [&](int c) { return row_scale[2 * r.token[off + c] + 1]; });
+            load_token<K>(x[nt], tok[nt] < 0 ? nullptr : xq + (int64_t)tok[nt] * xq_pitch, p.hidden, kb, t);
       } else {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -666,14 +706,7 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           if (!((live >> nt) & 1u)) continue;
-          float x0, x1;
-          if (p.keep_x) {
-            x0 = x_scale[kb * p.tokens + tok_of[nt][0]];
-            x1 = x_scale[kb * p.tokens + tok_of[nt][1]];
-          } else {
-            x0 = __shfl_sync(0xffffffffu, xs, 8 * nt + 2 * t);
-            x1 = __shfl_sync(0xffffffffu, xs, 8 * nt + 2 * t + 1);
-          }
+          const float x0 = xs[tok_of[nt][0] * nb + kb], x1 = xs[tok_of[nt][1] * nb + kb];
           const float sg = __uint_as_float(ws[0].sf[0][0]), su = __uint_as_float(ws[0].sf[1][0]);
           const float s0g = x0 * sg, s1g = x1 * sg, s0u = x0 * su, s1u = x1 * su;
 #pragma unroll
@@ -708,7 +741,7 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
         float up = get_sum<MT, NT>(mine_red, per_group, c >> 3, 1, c & 7, n);
         if constexpr (is_channel(K)) {
           const float* s1 = static_cast<const float*>(p.s1) + (int64_t)e * 2 * p.inter;
-          const float xsc = row_scale[2 * r.token[slot]];
+          const float xsc = p.keep_x ? row_scale[2 * r.token[slot]] : p.xs[r.token[slot]];
           gate *= xsc * s1[col];
           up *= xsc * s1[p.inter + col];
         } else if constexpr (is4(K)) {
@@ -769,9 +802,6 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
   uint8_t* rest = smem + kWarps * p.slots_per_warp * kBox + kCtrlBytes;
   float* red = reinterpret_cast<float*>(rest);
   rest += red_bytes(kWarps, MT, NT);
-  uint8_t* stage = rest + warp * code_bytes(NT);
-  if (is8(K)) rest += kWarps * code_bytes(NT);
-
   Routes r;
   build_routes<kWarps>(p, r, rest, [](int, int) {});
   rest += (route_bytes(p.experts, p.tokens * p.topk) + 15) & ~15;
@@ -857,29 +887,27 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
 
   wait_for_previous();     // the activations
   float* row_scale = reinterpret_cast<float*>(rest);       // [slots][2]
-  if constexpr (is_channel(K)) {
-    const int per_expert = p.amax_cols;
-    for (int s = warp; s < r.slots; s += kWarps) {
-      float amax = 0.f;
-      for (int i = lane; i < per_expert; i += 32) amax = fmaxf(amax, p.act_amax[(int64_t)s * per_expert + i]);
-      for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      if (lane == 0) scale8<K>(amax, row_scale[2 * s], row_scale[2 * s + 1]);
-    }
-    __syncthreads();
-  }
-
-  // 8-bit codes of all slots, made once where they fit beside the rings
-  uint8_t* a_codes = rest + (is_channel(K) ? (8 * p.tokens * p.topk + 15) & ~15 : 0);
+  uint8_t* a_codes = rest + ((8 * p.tokens * p.topk + 15) & ~15);
   const int a_pitch = code_pitch(K, p.inter);
   float* a_scale = reinterpret_cast<float*>(a_codes + p.tokens * p.topk * a_pitch);     // [slots][boxes]
-  if constexpr (is8(K)) {
-    if (p.keep_act) {
-      keep_codes<K>(warp, kWarps, lane, r.slots, p.inter, a_codes, a_pitch, [&](int m) {
-        return static_cast<const void*>(reinterpret_cast<const float*>(p.act_rows) + (int64_t)m * p.inter); }, BOLT_F32,
-        [&](int m) { return row_scale[2 * m + 1]; }, [&](int m, int kb, float scale) { a_scale[m * nb + kb] = scale; });
+  if (is8(K) && p.keep_act) {
+    if constexpr (is_channel(K)) {
+      for (int s = warp; s < r.slots; s += kWarps) {
+        float amax = 0.f;
+        for (int i = lane; i < p.amax_cols; i += 32) amax = fmaxf(amax, p.act_amax[(int64_t)s * p.amax_cols + i]);
+        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if (lane == 0) scale8<K>(amax, row_scale[2 * s], row_scale[2 * s + 1]);
+      }
       __syncthreads();
     }
+    keep_codes<K>(warp, kWarps, lane, r.slots, p.inter, a_codes, a_pitch, [&](int m) {
+      return static_cast<const void*>(reinterpret_cast<const float*>(p.act_rows) + (int64_t)m * p.inter); }, BOLT_F32,
+      [&](int m) { return row_scale[2 * m + 1]; }, [&](int m, int kb, float scale) { a_scale[m * nb + kb] = scale; });
+    __syncthreads();
   }
+  const uint8_t* aq = p.keep_act ? a_codes : p.aq;
+  const int aq_pitch = p.keep_act ? a_pitch : p.inter;
+  const float* as = p.keep_act ? a_scale : p.as;
 
   for (int u = u0; u < u1; ++u) {
     float acc[MT][NT][4];
@@ -899,22 +927,13 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
       for (int nt = 0; nt < NT; ++nt) live |= ((mask >> (8 * nt)) & 0xFFu) != 0u ? 1u << nt : 0u;
 
       TokenBox<K> x[NT];
-      float xs = 1.f;
-      const bool kept = is8(K) && p.keep_act;
-      if (kept) {
+      if constexpr (is8(K)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           if (!((live >> nt) & 1u)) continue;
           const int slot = slot_of(mask, off, 8 * nt + g);
-          load_token<K>(x[nt], slot < 0 ? nullptr : a_codes + slot * a_pitch, p.inter, kb, t);
+          load_token<K>(x[nt], slot < 0 ? nullptr : aq + (int64_t)slot * aq_pitch, p.inter, kb, t);
         }
-      } else if constexpr (is8(K)) {
-        xs = quant_box<K, NT>(
-            x, stage, mask, BOLT_F32, p.inter, kb * 128, lane,
-            [&](int c) {
-              return reinterpret_cast<const float*>(p.act_rows) + (int64_t)slot_of(mask, off, c) * p.inter;
-            },
-            [&](int c) { return row_scale[2 * slot_of(mask, off, c) + 1]; });
       } else {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -953,19 +972,14 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         if (!((live >> nt) & 1u)) continue;
-        float s01[2] = {1.f, 1.f};
-        if (is_block(K) && !kept) {
-          s01[0] = __shfl_sync(0xffffffffu, xs, 8 * nt + 2 * t);
-          s01[1] = __shfl_sync(0xffffffffu, xs, 8 * nt + 2 * t + 1);
-        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           // tokens that did not choose the expert get nothing (not even a NaN of its weights)
           const int slot = slot_of(mask, off, 8 * nt + 2 * t + i);
           if (slot < 0) continue;
-          float f = r.coef[slot] * s01[i] * whole;
-          if (is_block(K) && kept) f *= a_scale[slot * nb + kb];
-          if constexpr (is_channel(K)) f *= row_scale[2 * slot];
+          float f = r.coef[slot] * whole;
+          if constexpr (is_block(K)) f *= as[slot * nb + kb];
+          if constexpr (is_channel(K)) f *= p.keep_act ? row_scale[2 * slot] : p.as[slot];
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
             const float f0 = is8(K) ? f * __uint_as_float(ws[mt].sf[0][0]) : f;
@@ -1197,13 +1211,42 @@ int group_warps(int warps, int boxes) {
   return warps;
 }
 
-// bytes of the three parts of the workspace
-void workspace_parts(const bolt_decode_args* a, size_t (&part)[3]) {
+// Bytes of the workspace's parts: activations, their 4-bit scales, their largest magnitudes, 8-bit codes and
+// scales of the rows, of the activations.
+constexpr int kParts = 7;
+void workspace_parts(const bolt_decode_args* a, size_t (&part)[kParts]) {
   const size_t slots = (size_t)a->num_tokens * a->topk;
   const int k = a->kind;
   part[0] = a256(slots * (is8(k) ? 4 * (size_t)a->inter : (size_t)row_bytes(k, a->inter)));
   part[1] = is4(k) ? a256(slots * (a->inter / (k == K_NV4 ? 16 : 32))) : 0;
   part[2] = is_channel(k) ? a256(slots * ((a->inter + kMinUnit - 1) / kMinUnit) * 4) : 0;
+  part[3] = is8(k) ? a256((size_t)a->num_tokens * a->hidden) : 0;
+  part[4] = is8(k) ? a256((size_t)a->num_tokens * ((a->hidden + 127) / 128) * 4) : 0;
+  part[5] = is8(k) ? a256(slots * a->inter) : 0;
+  part[6] = is8(k) ? a256(slots * ((a->inter + 127) / 128) * 4) : 0;
+}
+size_t workspace_bytes(const bolt_decode_args* a) {
+  size_t part[kParts], all = 0;
+  workspace_parts(a, part);
+  for (size_t n : part) all += n;
+  return all;
+}
+
+// A kernel that may start while the one in front of it on the stream finishes.
+template <typename... Params, typename... Args>
+int launch_early(void (*kernel)(Params...), int blocks, int threads, int smem, cudaStream_t st, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  BOLT_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return BOLT_OK;
 }
 
 constexpr int kSmem = 226 * 1024, kHalfSmem = 113 * 1024;   // of a block, of one of two on an SM
@@ -1218,22 +1261,21 @@ int launch(const bolt_decode_args* a, Params p, int blocks, cudaStream_t st) {
   const int routes = p.tokens * p.topk;
   int up = 1024 + kCtrlBytes + red_bytes(kWarps, up_tiles(K), NT) + a16(route_bytes(p.experts, routes));
   int down = 1024 + kCtrlBytes + red_bytes(kWarps, kDownTiles, NT) + a16(route_bytes(p.experts, routes));
-  if (is_channel(K)) {
-    up += a16(8 * p.tokens);
-    down += a16(8 * routes);
-  }
+  if (is_channel(K)) up += a16(8 * p.tokens);
+  down += a16(8 * routes);
   if (is4(K)) up += p.tokens * (code_pitch(K, p.hidden) + p.hidden / (K == K_NV4 ? 16 : 32));
   if (is8(K)) {
-    // codes are kept where they leave the rings two boxes a warp, else made again for every box
+    // codes are kept by every block for up to eight tokens, where they leave the rings two boxes a warp (a
+    // launch less); making more of them 148 times over takes longer than a kernel that makes them once
+    // (Qwen3-30B int8, 32 tokens: 30 us of the first kernel alone)
     const auto kept = [&](int rows, int cols) {
       return (int64_t)rows * (code_pitch(K, cols) + (is_block(K) ? cols / 128 * 4 : 0)) + 16;
     };
     const int64_t x_kept = kept(p.tokens, p.hidden), act_kept = kept(routes, p.inter);
-    const int stage = kWarps * code_bytes(NT);
-    p.keep_x = up + x_kept + 2 * kWarps * kUpSlot <= kSmem;
-    up += p.keep_x ? (int)x_kept : stage;
-    p.keep_act = down + stage + act_kept + 2 * kWarps * kDownSlot <= kSmem;
-    down += stage + (p.keep_act ? (int)act_kept : 0);
+    p.keep_x = NT == 1 && up + x_kept + 2 * kWarps * kUpSlot <= kSmem;
+    if (p.keep_x) up += (int)x_kept;
+    p.keep_act = NT == 1 && down + act_kept + 2 * kWarps * kDownSlot <= kSmem;
+    if (p.keep_act) down += (int)act_kept;
   }
   const int up_slots = ring_slots(kSmem, up, kUpSlot, kWarps),
             down_slots = ring_slots(kSmem, down, kDownSlot, kWarps);
@@ -1269,22 +1311,28 @@ int launch(const bolt_decode_args* a, Params p, int blocks, cudaStream_t st) {
   p.slots_per_warp = up_slots;
   p.unit = columns;
   p.group_warps = group_warps(kWarps, (int)((row_bytes(K, p.hidden) + 127) / 128));
-  k_few_up<K, NT, kWarps><<<blocks, 32 * kWarps, up + up_slots * kWarps * kUpSlot, st>>>(m1, p);
-  BOLT_LAUNCH_CHECK();
+  const int up_bytes = up + up_slots * kWarps * kUpSlot, down_bytes = down + down_slots * kWarps * kDownSlot;
+  if constexpr (is8(K)) {
+    if (!p.keep_x) {
+      k_few_codes<K><<<p.tokens, 256, 0, st>>>(p.x, p.x_dtype, p.hidden, p.xq, p.xs);
+      BOLT_LAUNCH_CHECK();
+      if ((rc = launch_early(k_few_up<K, NT, kWarps>, blocks, 32 * kWarps, up_bytes, st, m1, p)) != BOLT_OK) return rc;
+    }
+  }
+  if (!is8(K) || p.keep_x) {
+    k_few_up<K, NT, kWarps><<<blocks, 32 * kWarps, up_bytes, st>>>(m1, p);
+    BOLT_LAUNCH_CHECK();
+  }
   p.slots_per_warp = down_slots;
   p.unit = rows;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(32 * kWarps);
-  cfg.dynamicSmemBytes = down + down_slots * kWarps * kDownSlot;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  BOLT_CUDA(cudaLaunchKernelEx(&cfg, k_few_down<K, NT, kWarps>, m2, p));
-  return BOLT_OK;
+  if constexpr (is8(K)) {
+    if (!p.keep_act) {
+      const void* act = p.act_rows;
+      const int f32 = BOLT_F32;
+      if ((rc = launch_early(k_few_codes<K>, routes, 256, 0, st, act, f32, p.inter, p.aq, p.as)) != BOLT_OK) return rc;
+    }
+  }
+  return launch_early(k_few_down<K, NT, kWarps>, blocks, 32 * kWarps, down_bytes, st, m2, p);
 }
 
 // Blocks of eight warps and half an SM's shared memory where a block's share of the weights is small: the
@@ -1362,9 +1410,7 @@ int check_args(const bolt_decode_args* a) {
 extern "C" size_t bolt_moe_decode_workspace_bytes(const bolt_decode_args* a) {
   using namespace bolt::few;
   if (check_args(a) != BOLT_OK) return 0;
-  size_t part[3];
-  workspace_parts(a, part);
-  return part[0] + part[1] + part[2] + 256;
+  return workspace_bytes(a) + 256;
 }
 
 namespace bolt {
@@ -1393,9 +1439,9 @@ int decode_once(const bolt_decode_args* a, cudaStream_t st) {
                "moe_decode: operands must be 16-byte aligned");
   BOLT_REQUIRE(!is4(k) || ((reinterpret_cast<uintptr_t>(a->w1_scale) | reinterpret_cast<uintptr_t>(a->w2_scale)) & 3) == 0,
                "moe_decode: scale bytes must be 4-byte aligned");
-  size_t part[3];
+  BOLT_REQUIRE(a->workspace_bytes >= workspace_bytes(a), "moe_decode: workspace too small");
+  size_t part[kParts];
   workspace_parts(a, part);
-  BOLT_REQUIRE(a->workspace_bytes >= part[0] + part[1] + part[2], "moe_decode: workspace too small");
 
   Params p = {};
   p.x = a->hidden_states;
@@ -1427,6 +1473,10 @@ int decode_once(const bolt_decode_args* a, cudaStream_t st) {
   p.act_rows = static_cast<uint8_t*>(a->workspace);
   p.act_sf = p.act_rows + part[0];
   p.act_amax = reinterpret_cast<float*>(p.act_sf + part[1]);
+  p.xq = p.act_sf + part[1] + part[2];
+  p.xs = reinterpret_cast<float*>(p.xq + part[3]);
+  p.aq = p.xq + part[3] + part[4];
+  p.as = reinterpret_cast<float*>(p.aq + part[5]);
   p.status = a->status;
 
   switch (k) {

@@ -368,10 +368,7 @@ __device__ __forceinline__ void load_block_scales(uint32_t* sf, const uint8_t* r
   }
 }
 
-// A box's 128 values of every live token, quantised by the whole warp: a lane takes four consecutive
-// values of a token, one warp-wide maximum gives its scale, and the codes go through shared memory
-// to the lanes that multiply them.  (A lane that quantised its own 32 bytes of its own column would
-// spend eight times the instructions where one column of eight is live, the usual case.)
+// four values -> four 8-bit codes, the arithmetic of the row quantisers (quant.cu)
 template <int K>
 __device__ __forceinline__ uint32_t codes4(const float4& v, float inv) {
   if (is_i8(K))
@@ -399,55 +396,6 @@ __device__ __forceinline__ float4 load_values4(const void* row, int dt, int at) 
   const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
   const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
   return make_float4(a.x, a.y, b.x, b.y);
-}
-
-constexpr int kCodePitch = 144;     // bytes between columns: 16-byte reads without bank conflicts
-constexpr int code_bytes(int nt) { return 8 * nt * kCodePitch; }
-
-// `stage`: code_bytes(NT) of the warp's own shared memory.  `row_of(column)`: a live column's values;
-// `live_cols`: bit per column; `inv_of(column)`: per-channel kinds, the reciprocal scale of its row.
-// Returns in lane c the scale of column c's group (block-scaled kinds).
-template <int K, int NT, typename RowOf, typename InvOf>
-__device__ __forceinline__ float quant_box(TokenBox<K> (&x)[NT], uint8_t* stage, uint32_t live_cols, int dt,
-                                           int cols, int at, int lane, RowOf row_of, InvOf inv_of) {
-  const int g = lane >> 2, t = lane & 3, c0 = at + 4 * lane;
-  const bool in = c0 < cols;          // (cols is a multiple of 16)
-  float my_scale = 1.f, my_inv = 1.f;
-  float4 kept = make_float4(0.f, 0.f, 0.f, 0.f);      // the first token's values (often the only one)
-  if constexpr (is_block(K)) {
-    uint32_t my_amax = 0;
-    for (uint32_t left = live_cols; left != 0; left &= left - 1) {
-      const int c = __ffs(left) - 1;
-      const float4 v = load_values4(row_of(c), dt, c0);
-      if (left == live_cols) kept = v;
-      // (non-negative floats order like their bits; fmaxf passes NaNs over)
-      const float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-      if (lane == c) my_amax = top;
-    }
-    scale8<K>(__uint_as_float(my_amax), my_scale, my_inv);
-  }
-  __syncwarp();                       // the box before has been read
-  for (uint32_t left = live_cols; left != 0; left &= left - 1) {
-    const int c = __ffs(left) - 1;
-    float4 v = kept;
-    if (in && !(is_block(K) && left == live_cols)) v = load_values4(row_of(c), dt, c0);
-    const float inv = is_block(K) ? __shfl_sync(0xffffffffu, my_inv, c) : inv_of(c);
-    *reinterpret_cast<uint32_t*>(stage + c * kCodePitch + 4 * lane) = codes4<K>(v, inv);
-  }
-  __syncwarp();
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int c = 8 * nt + g;
-    uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
-    if ((live_cols >> c) & 1u) {
-      a = *reinterpret_cast<const uint4*>(stage + c * kCodePitch + 32 * t);
-      b = *reinterpret_cast<const uint4*>(stage + c * kCodePitch + 32 * t + 16);
-    }
-    x[nt].w[0] = a.x; x[nt].w[1] = a.y; x[nt].w[2] = a.z; x[nt].w[3] = a.w;
-    x[nt].w[4] = b.x; x[nt].w[5] = b.y; x[nt].w[6] = b.z; x[nt].w[7] = b.w;
-  }
-  return my_scale;
 }
 
 // 32 consecutive values of a 16-bit row as floats (the block quantiser of 4-bit rows)
