@@ -5,17 +5,24 @@
 // k_few_up: routing (and, from logits, the router's top-k), Q1, the gate and up projections and the
 // activation; k_few_down: routing again, Q2, the down projection and the weighted sum over a token's
 // experts.  Nothing is sorted or copied: with so few tokens the routing is a bit mask of tokens per
-// expert, which every block builds for itself in shared memory in about a microsecond.
+// touched expert, which every block builds for itself in shared memory.  (8-bit rows or activations whose
+// codes do not fit beside a block's rings are quantised by k_few_codes in between.)
 //
 // What bounds it: the weights of the touched experts, read once each from HBM.  Split: k_few_up's unit
-// is 16 (MX: 32) intermediate columns of one expert, gate and up rows together over the whole hidden
+// is up to 16 (MX: 32) intermediate columns of one expert, gate and up rows together over the whole hidden
 // size, so that activation and (4-bit experts) the block quantiser run on finished sums; k_few_down's
-// unit is 16 output columns over ALL touched experts, so that the sum over a token's experts stays in
-// registers.  Units go to the blocks in contiguous runs, the 128-byte boxes of a unit to the warps
-// (token_mma.cuh).  The second kernel is launched with programmatic serialisation: its blocks start
-// as soon as there is room, build the routing and fill their rings with weights while the first
-// kernel finishes, and wait for it before they read its activations.  No block waits for another,
-// nothing is counted in memory, and results do not depend on timing.
+// unit is up to 32 output columns over ALL touched experts, so that the sum over a token's experts stays in
+// registers.  Units go to the blocks in contiguous runs of equal length (their size is chosen for that), the
+// 128-byte boxes of a unit to the warps (token_mma.cuh).  The second kernel is launched with programmatic
+// serialisation: its blocks start as soon as there is room, build the routing and fill their rings with
+// weights while the first kernel finishes, and wait for it before they read its activations.  No block
+// waits for another, nothing is counted in memory, and results do not depend on timing.
+//
+// Measured (graph replays, weights apart from call to call): Mixtral bf16, one token 114 us, 6.2 TB/s of
+// weights; DeepSeek-V3 fp8, one token 85 us, 4.1 TB/s, eight 468 us, 5.4 TB/s; nvfp4, one token 64 us, eight
+// 372 us, 3.8 TB/s.  Beside HBM they wait for: two prologues of 3 us each (instructions that are not in the
+// cache yet, routing, the first loads), and with 4-bit codes the ALU: widening a code and scaling it costs
+// about 2.3 instructions a weight pair, as long as HBM takes to bring it.
 //
 // Rounding: 16-bit experts round the activation to the weights' type (the tensor cores' operand);
 // quantised experts keep fp32 up to their quantiser.  All sums are fp32, rounded once at the end.
@@ -332,8 +339,8 @@ __device__ __forceinline__ void finish(volatile int* abort_flag) {
     for (int i = 0; i < 200; ++i) __nanosleep(1000);
 }
 
-template <int MT, int NT>
-__device__ __forceinline__ void put_sums(float* red, const float (&acc)[MT][NT][4], int warp, int lane,
+template <int MT, int NT, int TG>
+__device__ __forceinline__ void put_sums(float* red, const float (&acc)[NT / TG][MT][TG][4], int warp, int lane,
                                          unsigned live) {
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
@@ -341,8 +348,17 @@ __device__ __forceinline__ void put_sums(float* red, const float (&acc)[MT][NT][
     for (int nt = 0; nt < NT; ++nt) {
       if (!((live >> nt) & 1u)) continue;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) red[(((warp * MT + mt) * NT + nt) * 4 + i) * 32 + lane] = acc[mt][nt][i];
+      for (int i = 0; i < 4; ++i) red[(((warp * MT + mt) * NT + nt) * 4 + i) * 32 + lane] = acc[nt / TG][mt][nt % TG][i];
     }
+}
+template <int MT, int TG>
+__device__ __forceinline__ void zero_sums(float (&v)[MT][TG][4]) {
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < TG; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[mt][nt][i] = 0.f;
 }
 // Sum over the warps of element (row half r, row g of tile mt, token n).
 template <int MT, int NT>
@@ -365,7 +381,11 @@ constexpr int kDownBoxBytes = kMaxRows * 128;
 constexpr int up_scale_bytes(int k) {      // of a slot
   return k == K_NV4 ? 512 : k == K_MX4 ? 512 : is_block(k) ? 64 : 0;
 }
-constexpr int warps_of(int k, int nt) { return nt == 4 || (k == K_MX4 && nt == 2) ? 8 : 16; }
+constexpr int warps_of(int k, int nt) { return k == K_MX4 && nt > 1 ? 8 : 16; }
+// Token tiles computed together; the four tiles of more than 16 tokens go one by one (few of them are live,
+// and eight warps with the registers for four at once took 411 us where sixteen take 278:
+// Qwen3-30B bf16, 32 tokens).
+constexpr int tiles_at_once(int k, int nt) { return nt == 4 && k != K_MX4 ? 1 : nt; }
 // blocks an SM holds as far as registers go: the second kernel's beside the first's
 constexpr int blocks_of(int nt, int warps) { return nt == 1 && warps == 8 ? 2 : 1; }
 constexpr int red_bytes(int warps, int mt, int nt) { return warps * mt * nt * 128 * 4; }
@@ -452,7 +472,7 @@ __global__ void __launch_bounds__(256) k_few_codes(const void* src, int dt, int 
 template <int K, int NT, int W>
 __global__ void __launch_bounds__(32 * W, blocks_of(NT, W))
 k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
-  constexpr int MT = up_tiles(K), kBox = up_box_bytes(K), kWarps = W;
+  constexpr int MT = up_tiles(K), kBox = up_box_bytes(K), kWarps = W, TG = tiles_at_once(K, NT);
   constexpr int kCols = 8 * MT;       // columns a unit may have
   // rows of scales: of every gate and up row of a thread (4-bit), of the unit's gate and up block
   using Scales = ScaleRing<is_channel(K) ? (int)K_BF16 : K, is4(K) ? 2 * MT : 2>;
@@ -635,13 +655,9 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
     const int off = r.off[unit.a], cnt = __popc(r.mask[unit.a]);
     const unsigned live = (1u << ((cnt + 7) / 8)) - 1u;
     const uint32_t live_cols = cnt == 32 ? ~0u : (1u << cnt) - 1u;
-    float acc[MT][NT][4];
+    float acc[NT / TG][MT][TG][4];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[mt][nt][i] = 0.f;
+    for (int n = 0; n < NT / TG; ++n) zero_sums(acc[n]);
     int tok[NT];     // token of column g of every tile
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) tok[nt] = 8 * nt + g < cnt ? r.token[off + 8 * nt + g] : -1;
@@ -657,36 +673,31 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
     while (it < n_it && cur.u == unit.u) {
       const int kb = cur.kb;
 
-      TokenBox<K> x[NT];
-      if constexpr (is8(K)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          if ((live >> nt) & 1u)
-            load_token<K>(x[nt], tok[nt] < 0 ? nullptr : xq + (int64_t)tok[nt] * xq_pitch, p.hidden, kb, t);
-      } else {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (!((live >> nt) & 1u)) continue;
-          const int m = tok[nt];
-          if constexpr (is16(K)) {
-            load_token<K>(x[nt], m < 0 ? nullptr : static_cast<const uint8_t*>(p.x) + (int64_t)m * p.hidden * 2,
-                          p.hidden * 2, kb, t);
+      // what the columns of token tile nt are multiplied with
+      auto load_x = [&](TokenBox<K>& x, int nt, int m) {
+        if constexpr (is8(K)) {
+          load_token<K>(x, m < 0 ? nullptr : xq + (int64_t)m * xq_pitch, p.hidden, kb, t);
+        } else if constexpr (is16(K)) {
+          load_token<K>(x, m < 0 ? nullptr : static_cast<const uint8_t*>(p.x) + (int64_t)m * p.hidden * 2,
+                        p.hidden * 2, kb, t);
+        } else {
+          load_token<K>(x, m < 0 ? nullptr : x_codes + m * pitch, p.hidden / 2, kb, t);
+          if constexpr (K == K_NV4) {
+            load_block_scales<K>(x.sf, m < 0 ? nullptr : x_sf + (int64_t)m * sf_row, sf_row, kb, t);
           } else {
-            load_token<K>(x[nt], m < 0 ? nullptr : x_codes + m * pitch, p.hidden / 2, kb, t);
-            if constexpr (K == K_NV4) {
-              load_block_scales<K>(x[nt].sf, m < 0 ? nullptr : x_sf + (int64_t)m * sf_row, sf_row, kb, t);
-            } else {
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const int col = 8 * nt + 2 * t + i;
-                load_block_scales<K>(x[nt].sf + 2 * i,
-                                     col < cnt ? x_sf + (int64_t)r.token[off + col] * sf_row : nullptr,
-                                     sf_row, kb, t);
-              }
+            for (int i = 0; i < 2; ++i) {
+              const int col = 8 * nt + 2 * t + i;
+              load_block_scales<K>(x.sf + 2 * i,
+                                   col < cnt ? x_sf + (int64_t)r.token[off + col] * sf_row : nullptr, sf_row, kb, t);
             }
           }
         }
-      }
+      };
+      TokenBox<K> x[TG];
+#pragma unroll
+      for (int j = 0; j < TG; ++j)
+        if ((live >> j) & 1u) load_x(x[j], j, tok[j]);
       RowScales<K> ws[MT];
       if constexpr (is4(K) || is_block(K)) {
         cp_async_wait(p.slots_per_warp - 1);
@@ -694,31 +705,36 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
         scales.read(ws, ring.s_out, lane);
       }
       const uint32_t box = ring.wait(abort_flag, p.status);
-      if constexpr (is_block(K)) {
-        float part[MT][NT][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+      for (int n = 0; n < NT / TG; ++n) {
+        const unsigned here = live >> (n * TG);
+        if (here == 0) break;
+        if (n > 0) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) part[mt][nt][i] = 0.f;
-        box_mma<K, MT, NT, true>(box, UC, lane, x, ws, live, part);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (!((live >> nt) & 1u)) continue;
-          const float x0 = xs[tok_of[nt][0] * nb + kb], x1 = xs[tok_of[nt][1] * nb + kb];
-          const float sg = __uint_as_float(ws[0].sf[0][0]), su = __uint_as_float(ws[0].sf[1][0]);
-          const float s0g = x0 * sg, s1g = x1 * sg, s0u = x0 * su, s1u = x1 * su;
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            acc[mt][nt][0] = fmaf(part[mt][nt][0], s0g, acc[mt][nt][0]);
-            acc[mt][nt][1] = fmaf(part[mt][nt][1], s1g, acc[mt][nt][1]);
-            acc[mt][nt][2] = fmaf(part[mt][nt][2], s0u, acc[mt][nt][2]);
-            acc[mt][nt][3] = fmaf(part[mt][nt][3], s1u, acc[mt][nt][3]);
-          }
+          for (int j = 0; j < TG; ++j) load_x(x[j], n * TG + j, tok[n * TG + j]);
         }
-      } else {
-        box_mma<K, MT, NT, true>(box, UC, lane, x, ws, live, acc);
+        if constexpr (is_block(K)) {
+          float part[MT][TG][4];
+          zero_sums(part);
+          box_mma<K, MT, TG, true>(box, UC, lane, x, ws, here, part);
+#pragma unroll
+          for (int j = 0; j < TG; ++j) {
+            if (!((here >> j) & 1u)) continue;
+            const float x0 = xs[tok_of[n * TG + j][0] * nb + kb], x1 = xs[tok_of[n * TG + j][1] * nb + kb];
+            const float sg = __uint_as_float(ws[0].sf[0][0]), su = __uint_as_float(ws[0].sf[1][0]);
+            const float s0g = x0 * sg, s1g = x1 * sg, s0u = x0 * su, s1u = x1 * su;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              float(&sum)[4] = acc[n][mt][j];
+              sum[0] = fmaf(part[mt][j][0], s0g, sum[0]);
+              sum[1] = fmaf(part[mt][j][1], s1g, sum[1]);
+              sum[2] = fmaf(part[mt][j][2], s0u, sum[2]);
+              sum[3] = fmaf(part[mt][j][3], s1u, sum[3]);
+            }
+          }
+        } else {
+          box_mma<K, MT, TG, true>(box, UC, lane, x, ws, here, acc[n]);
+        }
       }
       ring.release();
       bring();
@@ -727,7 +743,7 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
     }
 
     // ---- sums over the warps, activation, Q2 of the 4-bit kinds ----
-    put_sums<MT, NT>(red, acc, warp, lane, live);
+    put_sums<MT, NT, TG>(red, acc, warp, lane, live);
     group_sync();
     const float* mine_red = red + group * per_group * MT * NT * 128;
     const int all = ((cnt * kCols + 31) / 32) * 32;      // whole warps take part in the exchanges
@@ -791,7 +807,8 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
 template <int K, int NT, int W>
 __global__ void __launch_bounds__(32 * W, blocks_of(NT, W))
 k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
-  constexpr int MT = kDownTiles, kBox = kDownBoxBytes, kWarps = W, kThreads = 32 * kWarps;
+  constexpr int MT = kDownTiles, kBox = kDownBoxBytes, kWarps = W, kThreads = 32 * kWarps,
+                TG = tiles_at_once(K, NT);
   const int UR = p.unit;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = carve(raw);
@@ -910,13 +927,9 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
   const float* as = p.keep_act ? a_scale : p.as;
 
   for (int u = u0; u < u1; ++u) {
-    float acc[MT][NT][4];
+    float acc[NT / TG][MT][TG][4];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[mt][nt][i] = 0.f;
+    for (int n = 0; n < NT / TG; ++n) zero_sums(acc[n]);
 
     while (it < n_it && cur.u == u) {
       const int e = r.list[cur.a], kb = cur.kb;
@@ -926,34 +939,30 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) live |= ((mask >> (8 * nt)) & 0xFFu) != 0u ? 1u << nt : 0u;
 
-      TokenBox<K> x[NT];
-      if constexpr (is8(K)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (!((live >> nt) & 1u)) continue;
-          const int slot = slot_of(mask, off, 8 * nt + g);
-          load_token<K>(x[nt], slot < 0 ? nullptr : aq + (int64_t)slot * aq_pitch, p.inter, kb, t);
-        }
-      } else {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (!((live >> nt) & 1u)) continue;
-          const int slot = slot_of(mask, off, 8 * nt + g);
-          if constexpr (is16(K)) {
-            load_token<K>(x[nt], slot < 0 ? nullptr : p.act_rows + (int64_t)slot * p.inter * 2, p.inter * 2, kb, t);
+      auto load_x = [&](TokenBox<K>& x, int nt) {
+        const int slot = slot_of(mask, off, 8 * nt + g);
+        if constexpr (is8(K)) {
+          load_token<K>(x, slot < 0 ? nullptr : aq + (int64_t)slot * aq_pitch, p.inter, kb, t);
+        } else if constexpr (is16(K)) {
+          load_token<K>(x, slot < 0 ? nullptr : p.act_rows + (int64_t)slot * p.inter * 2, p.inter * 2, kb, t);
+        } else {
+          load_token<K>(x, slot < 0 ? nullptr : p.act_rows + (int64_t)slot * (p.inter / 2), p.inter / 2, kb, t);
+          if constexpr (K == K_NV4) {
+            load_block_scales<K>(x.sf, slot < 0 ? nullptr : p.act_sf + (int64_t)slot * sf_row, sf_row, kb, t);
           } else {
-            load_token<K>(x[nt], slot < 0 ? nullptr : p.act_rows + (int64_t)slot * (p.inter / 2), p.inter / 2, kb, t);
-            if constexpr (K == K_NV4) {
-              load_block_scales<K>(x[nt].sf, slot < 0 ? nullptr : p.act_sf + (int64_t)slot * sf_row, sf_row, kb, t);
-            } else {
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const int s = slot_of(mask, off, 8 * nt + 2 * t + i);
-                load_block_scales<K>(x[nt].sf + 2 * i, s < 0 ? nullptr : p.act_sf + (int64_t)s * sf_row, sf_row, kb, t);
-              }
+            for (int i = 0; i < 2; ++i) {
+              const int s = slot_of(mask, off, 8 * nt + 2 * t + i);
+              load_block_scales<K>(x.sf + 2 * i, s < 0 ? nullptr : p.act_sf + (int64_t)s * sf_row, sf_row, kb, t);
             }
           }
         }
+      };
+      TokenBox<K> x[TG];
+      if constexpr (TG == NT) {
+#pragma unroll
+        for (int j = 0; j < TG; ++j)
+          if ((live >> j) & 1u) load_x(x[j], j);
       }
       const float whole = is4(K) ? (p.g2 != nullptr ? p.g2[e] : 1.f) * (p.a2 != nullptr ? *p.a2 : 1.f) : 1.f;
       RowScales<K> ws[MT];
@@ -961,31 +970,32 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
       if (K != K_NV4) __syncwarp();
       scales.read(ws, ring.s_out, lane);
       const uint32_t box = ring.wait(abort_flag, p.status);
-      float part[MT][NT][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int n = 0; n < NT / TG; ++n) {
+        const unsigned here = (live >> (n * TG)) & ((1u << TG) - 1u);
+        if (here == 0) continue;
+        if constexpr (TG != NT) load_x(x[0], n);
+        float part[MT][TG][4];
+        zero_sums(part);
+        box_mma<K, MT, TG, false>(box, 0, lane, x, ws, here, part);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int j = 0; j < TG; ++j) {
+          if (!((here >> j) & 1u)) continue;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) part[mt][nt][i] = 0.f;
-      box_mma<K, MT, NT, false>(box, 0, lane, x, ws, live, part);
+          for (int i = 0; i < 2; ++i) {
+            // tokens that did not choose the expert get nothing (not even a NaN of its weights)
+            const int slot = slot_of(mask, off, 8 * (n * TG + j) + 2 * t + i);
+            if (slot < 0) continue;
+            float f = r.coef[slot] * whole;
+            if constexpr (is_block(K)) f *= as[slot * nb + kb];
+            if constexpr (is_channel(K)) f *= p.keep_act ? row_scale[2 * slot] : p.as[slot];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (!((live >> nt) & 1u)) continue;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          // tokens that did not choose the expert get nothing (not even a NaN of its weights)
-          const int slot = slot_of(mask, off, 8 * nt + 2 * t + i);
-          if (slot < 0) continue;
-          float f = r.coef[slot] * whole;
-          if constexpr (is_block(K)) f *= as[slot * nb + kb];
-          if constexpr (is_channel(K)) f *= p.keep_act ? row_scale[2 * slot] : p.as[slot];
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            const float f0 = is8(K) ? f * __uint_as_float(ws[mt].sf[0][0]) : f;
-            const float f1 = is8(K) ? f * __uint_as_float(ws[mt].sf[1][0]) : f;
-            acc[mt][nt][i] = fmaf(part[mt][nt][i], f0, acc[mt][nt][i]);
-            acc[mt][nt][2 + i] = fmaf(part[mt][nt][2 + i], f1, acc[mt][nt][2 + i]);
+            for (int mt = 0; mt < MT; ++mt) {
+              const float f0 = is8(K) ? f * __uint_as_float(ws[mt].sf[0][0]) : f;
+              const float f1 = is8(K) ? f * __uint_as_float(ws[mt].sf[1][0]) : f;
+              acc[n][mt][j][i] = fmaf(part[mt][j][i], f0, acc[n][mt][j][i]);
+              acc[n][mt][j][2 + i] = fmaf(part[mt][j][2 + i], f1, acc[n][mt][j][2 + i]);
+            }
           }
         }
       }
@@ -995,7 +1005,7 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
       if (++it < n_it) settle(cur);
     }
 
-    put_sums<MT, NT>(red, acc, warp, lane, ~0u);
+    put_sums<MT, NT, TG>(red, acc, warp, lane, ~0u);
     __syncthreads();
     for (int i = tid; i < p.tokens * kMaxRows; i += kThreads) {
       const int n = i / kMaxRows, c = i % kMaxRows, col = u * UR + c;
@@ -1024,10 +1034,12 @@ struct DenseParams {
   int32_t* status;
 };
 
+constexpr int dense_warps(int k, int nt) { return nt == 4 || k == K_MX4 ? 8 : 16; }
 template <int K, int NT>
-__global__ void __launch_bounds__(32 * warps_of(K, NT), 1)
+__global__ void __launch_bounds__(32 * dense_warps(K, NT), 1)
 k_few_dense(const __grid_constant__ CUtensorMap map, const DenseParams p) {
-  constexpr int MT = kDownTiles, kBox = kDownBoxBytes, kWarps = warps_of(K, NT), kThreads = 32 * kWarps;
+  constexpr int MT = kDownTiles, kBox = kDownBoxBytes, kWarps = dense_warps(K, NT), kThreads = 32 * kWarps,
+                TG = NT;
   const int UR = p.unit;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = carve(raw);
@@ -1094,43 +1106,45 @@ k_few_dense(const __grid_constant__ CUtensorMap map, const DenseParams p) {
   const float alpha = p.alpha != nullptr ? *p.alpha : 1.f;
 
   for (int u = u0; u < u1; ++u) {
-    float acc[MT][NT][4];
+    float acc[NT / TG][MT][TG][4];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[mt][nt][i] = 0.f;
+    for (int n = 0; n < NT / TG; ++n) zero_sums(acc[n]);
     while (it < n_it && cur.u == u) {
-      TokenBox<K> x[NT];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (!((live >> nt) & 1u)) continue;
+      auto load_x = [&](TokenBox<K>& x, int nt) {
         const int m = 8 * nt + g;
-        load_token<K>(x[nt], m < p.rows ? p.x + (int64_t)m * row_len : nullptr, row_len, cur.kb, t);
+        load_token<K>(x, m < p.rows ? p.x + (int64_t)m * row_len : nullptr, row_len, cur.kb, t);
         if constexpr (K == K_NV4) {
-          load_block_scales<K>(x[nt].sf, m < p.rows ? p.x_sf + (int64_t)m * sf_row : nullptr, sf_row, cur.kb, t);
+          load_block_scales<K>(x.sf, m < p.rows ? p.x_sf + (int64_t)m * sf_row : nullptr, sf_row, cur.kb, t);
         } else {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int c = 8 * nt + 2 * t + i;
-            load_block_scales<K>(x[nt].sf + 2 * i, c < p.rows ? p.x_sf + (int64_t)c * sf_row : nullptr, sf_row,
-                                 cur.kb, t);
+            load_block_scales<K>(x.sf + 2 * i, c < p.rows ? p.x_sf + (int64_t)c * sf_row : nullptr, sf_row, cur.kb, t);
           }
         }
-      }
+      };
       RowScales<K> ws[MT];
       cp_async_wait(p.slots_per_warp - 1);
       if (K != K_NV4) __syncwarp();
       scales.read(ws, ring.s_out, lane);
+      TokenBox<K> x[TG];
+#pragma unroll
+      for (int j = 0; j < TG; ++j) load_x(x[j], j);
       const uint32_t box = ring.wait(abort_flag, p.status);
-      box_mma<K, MT, NT, false>(box, 0, lane, x, ws, live, acc);
+#pragma unroll
+      for (int n = 0; n < NT / TG; ++n) {
+        if (n > 0) {
+#pragma unroll
+          for (int j = 0; j < TG; ++j) load_x(x[j], n * TG + j);
+        }
+        box_mma<K, MT, TG, false>(box, 0, lane, x, ws, live >> (n * TG), acc[n]);
+      }
       ring.release();
       bring();
       cur.kb += kWarps;
       if (++it < n_it) settle(cur);
     }
-    put_sums<MT, NT>(red, acc, warp, lane, live);
+    put_sums<MT, NT, TG>(red, acc, warp, lane, live);
     __syncthreads();
     for (int i = tid; i < p.rows * kMaxRows; i += kThreads) {
       const int n = i / kMaxRows, c = i % kMaxRows, col = u * UR + c;
@@ -1353,12 +1367,12 @@ int launch_kind(const bolt_decode_args* a, const Params& p, cudaStream_t st) {
     return launch<K, 1, warps_of(K, 1)>(a, p, sms, st);
   }
   if (p.tokens <= 16) return launch<K, 2, warps_of(K, 2)>(a, p, sms, st);
-  return launch<K, 4, 8>(a, p, sms, st);
+  return launch<K, 4, warps_of(K, 4)>(a, p, sms, st);
 }
 
 template <int K, int NT>
 int launch_dense(const bolt_fp4_few_args* a, DenseParams p, int sms, cudaStream_t st) {
-  constexpr int kWarps = warps_of(K, NT);
+  constexpr int kWarps = dense_warps(K, NT);
   static std::atomic<bool> ready[kMaxDevices];
   int rc = configure_kernel(k_few_dense<K, NT>, kSmem, ready, 0, 0, 0, 0);
   if (rc != BOLT_OK) return rc;
