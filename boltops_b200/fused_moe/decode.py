@@ -5,7 +5,8 @@ combines in five to seven launches.  With one or a few tokens these launches and
 a large part of the time.  The forms here take 1 to 32 tokens and leave out everything but
 the weights: routing is a bit mask per expert that every block of the kernel builds for itself, the
 first kernel does gate, up and activation, the second the down projection and the sum over a token's
-experts, and it fills its weight rings while the first one finishes.
+experts, and it fills its weight rings while the first one finishes.  (8-bit codes that a block cannot keep
+beside its rings, as a rule above eight tokens, are made by a small kernel in front of either.)
 
 Same recipes as ``fused_experts`` (16-bit, fp8 and int8 w8a8 block-scaled and per-channel) and
 ``fused_experts_fp4`` (w4a4), with fewer roundings: GEMM 1 and the routes' results stay in fp32, quantised
