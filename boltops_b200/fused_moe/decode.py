@@ -92,18 +92,16 @@ def check_weights(kind_name, w1, w2, w1_scale, w2_scale, hidden, w_dtype, scale_
                                ("w2_scale", w2_scale, scale2(e, model_dim, inter))):
             if s is None:
                 raise ValueError(f"{name} is required ({kind_name})")
-            if s.numel() != _numel(shape):
+            # (dimensions of one value apart: per-channel scales come as [E, N] or [E, N, 1])
+            if _long_dims(s.shape) != _long_dims(shape):
                 raise ValueError(f"{name} {tuple(s.shape)}: expected {shape} ({kind_name})")
             if scale_dtype != torch.float32 and s.dtype != scale_dtype:
                 raise TypeError(f"{name} must be {scale_dtype} ({kind_name})")
     return e, inter, model_dim
 
 
-def _numel(shape):
-    n = 1
-    for s in shape:
-        n *= s
-    return n
+def _long_dims(shape):
+    return [n for n in shape if n != 1]
 
 
 def _decode(hidden_states, w1, w2, topk_weights, topk_ids, gating, topk, renormalize, is_softmax, *,

@@ -225,6 +225,21 @@ def test_fused_experts_decode_refuses():
             fused_moe_decode(**{**route, "gating_output": torch.zeros(2, 2), "topk": 1, "renormalize": True, **bad})
 
 
+@pytest.mark.parametrize("kind", ["fp8_block", "int8_block", "nvfp4", "mxfp4"])
+def test_scales_in_another_order_are_refused(kind):
+    from boltops_b200.fused_moe import fused_experts_decode, fused_experts_fp4
+    good = _layer(kind, h=256, i=384)
+    flags = dict(use_fp4_w4a4=True) if kind.endswith("fp4") else \
+        {f"use_{kind[:-6]}_w8a8": True, "block_shape": [128, 128]}
+    for name in ("w1_scale", "w2_scale"):
+        turned = {**good, name: good[name].transpose(1, 2)}
+        with pytest.raises(ValueError, match=name):
+            fused_experts_decode(**turned, **flags)
+        if kind.endswith("fp4"):
+            with pytest.raises(ValueError, match=name):
+                fused_experts_fp4(**turned)
+
+
 def test_fused_experts_fp4_refuses():
     from boltops_b200.fused_moe import fused_experts_fp4
     good = _layer("nvfp4")
