@@ -74,6 +74,8 @@ def fused_experts_fp4(
     for name, t in (("topk_weights", topk_weights), ("topk_ids", topk_ids), ("expert_map", expert_map)):
         if t is not None and t.device != dev:
             raise ValueError(f"{name} is on {t.device}, hidden_states on {dev}")
+    if expert_map is not None and expert_map.dim() != 1:
+        raise ValueError("expert_map must be one row of entries")
     act, alpha, limit = gated_activation(activation, gemm1_alpha, gemm1_limit, activation_situ_beta,
                                          activation_situ_linear_beta)
     out_dtype = hidden_states.dtype if output_dtype is None else output_dtype

@@ -275,3 +275,13 @@ def test_reference_quantiser_is_the_nearest_code(fmt):
     assert torch.allclose(off, best, rtol=0, atol=1e-12)
     if fmt == "mxfp4":      # nothing saturates: the largest magnitude is at most 6 scales
         assert (x.double().abs().unflatten(-1, (-1, 32)) <= 6 * s).all()
+
+
+@pytest.mark.parametrize("shape", [(2, 4), (1, 2), ()])
+def test_an_expert_map_of_several_rows_is_refused(shape):
+    """The tiles' experts are looked up in it by one index: a map of two rows would be read past its end."""
+    from boltops_b200.fused_moe import fused_experts_decode, fused_experts_fp4
+    good = {**_layer("nvfp4"), "expert_map": torch.zeros(shape, dtype=torch.int32)}
+    for call, more in ((fused_experts_fp4, {}), (fused_experts_decode, dict(use_fp4_w4a4=True))):
+        with pytest.raises(ValueError, match="one row"):
+            call(**good, **more)
