@@ -1246,9 +1246,11 @@ size_t workspace_bytes(const bolt_decode_args* a) {
   return all;
 }
 
-// A kernel that may start while the one in front of it on the stream finishes.
+// A kernel that may start while the one in front of it on the stream finishes (`early` false: it waits for that one,
+// as a caller who leaves SMs to other kernels wants: blocks that start early would take those SMs and wait there).
 template <typename... Params, typename... Args>
-int launch_early(void (*kernel)(Params...), int blocks, int threads, int smem, cudaStream_t st, const Args&... args) {
+int launch_early(bool early, void (*kernel)(Params...), int blocks, int threads, int smem, cudaStream_t st,
+                 const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks);
   cfg.blockDim = dim3(threads);
@@ -1258,7 +1260,7 @@ int launch_early(void (*kernel)(Params...), int blocks, int threads, int smem, c
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = early ? 1 : 0;
   BOLT_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
   return BOLT_OK;
 }
@@ -1306,6 +1308,7 @@ int launch(const bolt_decode_args* a, Params p, int blocks, cudaStream_t st) {
                              : unit_size(p.inter, 8 * up_tiles(K), routes < p.experts ? routes : p.experts, blocks,
                                          is_block(K) ? 8 : 1);
   const int rows = unit_size(p.model_dim, kMaxRows, 1, blocks);
+  const bool early = a->sm_count <= 0;
   CUtensorMap m1, m2;
   {
     const cuuint64_t kb = (cuuint64_t)row_bytes(K, p.hidden), i = p.inter;
@@ -1330,7 +1333,7 @@ int launch(const bolt_decode_args* a, Params p, int blocks, cudaStream_t st) {
     if (!p.keep_x) {
       k_few_codes<K><<<p.tokens, 256, 0, st>>>(p.x, p.x_dtype, p.hidden, p.xq, p.xs);
       BOLT_LAUNCH_CHECK();
-      if ((rc = launch_early(k_few_up<K, NT, kWarps>, blocks, 32 * kWarps, up_bytes, st, m1, p)) != BOLT_OK) return rc;
+      if ((rc = launch_early(early, k_few_up<K, NT, kWarps>, blocks, 32 * kWarps, up_bytes, st, m1, p)) != BOLT_OK) return rc;
     }
   }
   if (!is8(K) || p.keep_x) {
@@ -1343,10 +1346,10 @@ int launch(const bolt_decode_args* a, Params p, int blocks, cudaStream_t st) {
     if (!p.keep_act) {
       const void* act = p.act_rows;
       const int f32 = BOLT_F32;
-      if ((rc = launch_early(k_few_codes<K>, routes, 256, 0, st, act, f32, p.inter, p.aq, p.as)) != BOLT_OK) return rc;
+      if ((rc = launch_early(early, k_few_codes<K>, routes, 256, 0, st, act, f32, p.inter, p.aq, p.as)) != BOLT_OK) return rc;
     }
   }
-  return launch_early(k_few_down<K, NT, kWarps>, blocks, 32 * kWarps, down_bytes, st, m2, p);
+  return launch_early(early, k_few_down<K, NT, kWarps>, blocks, 32 * kWarps, down_bytes, st, m2, p);
 }
 
 // Blocks of eight warps and half an SM's shared memory where a block's share of the weights is small: the

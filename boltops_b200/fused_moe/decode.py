@@ -222,7 +222,7 @@ def _decode(hidden_states, w1, w2, topk_weights, topk_ids, gating, topk, renorma
         global_num_experts, x.data_ptr(), w1.data_ptr(), w2.data_ptr(), s1, s2, *whole, *routing,
         _cabi.ptr(expert_map), act, alpha, limit,
         1.0 if routed_scaling_factor is None else float(routed_scaling_factor), out.data_ptr(), None, 0,
-        ops.device_status(dev).data_ptr(), 0)
+        ops.device_status(dev).data_ptr(), ops.gemm_sm_count(dev))
     need = lib.bolt_moe_decode_workspace_bytes(args)
     if need == 0:
         _cabi.check(1)

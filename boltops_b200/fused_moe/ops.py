@@ -503,9 +503,9 @@ _gemm_sm_reserve = 0
 
 
 def set_gemm_sm_reserve(sms: int) -> None:
-    """Number of SMs the grouped GEMMs leave free (0 = none).  The expert-parallel layer sets it
-    while exchange kernels run next to the GEMMs: a persistent GEMM with one CTA on every SM would
-    make a concurrently launched collective wait for it."""
+    """Number of SMs that the products and the few-token layer leave free (0 = none).  The
+    expert-parallel layer sets it while exchange kernels run next to the GEMMs: a persistent GEMM with
+    one CTA on every SM would make a concurrently launched collective wait for it."""
     global _gemm_sm_reserve
     _gemm_sm_reserve = max(int(sms), 0)
 
@@ -530,7 +530,7 @@ def check_device_status(device: torch.device) -> None:
 
 
 def gemm_sm_count(device) -> int:
-    """SMs a grouped GEMM may use on ``device`` (0: all of them)."""
+    """SMs a product or the few-token layer may use on ``device`` (0: all of them)."""
     if _gemm_sm_reserve <= 0:
         return 0
     total = torch.cuda.get_device_properties(device).multi_processor_count

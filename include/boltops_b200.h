@@ -726,7 +726,7 @@ typedef struct bolt_decode_args {
   void* workspace;             /* contents do not matter; one call at a time                  */
   size_t workspace_bytes;
   int32_t* status;             /* optional, as in bolt_gemm_args; 30: a weight copy did not land */
-  int sm_count;                /* SMs to use; 0: all                                          */
+  int sm_count;                /* SMs to use; 0: all (the second kernel then starts beside the first) */
 } bolt_decode_args;
 
 /* Two kernels on the stream (no sort, no copies of rows; 4-bit rows of more tokens than fit in shared memory

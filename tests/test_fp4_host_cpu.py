@@ -285,3 +285,37 @@ def test_an_expert_map_of_several_rows_is_refused(shape):
     for call, more in ((fused_experts_fp4, {}), (fused_experts_decode, dict(use_fp4_w4a4=True))):
         with pytest.raises(ValueError, match="one row"):
             call(**good, **more)
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The C entries that a call reaches, with their argument structures: nothing is launched."""
+    from boltops_b200 import _cabi
+    from boltops_b200.fused_moe import ops
+    made = []
+
+    class Lib:
+        def __getattr__(self, name):
+            def entry(*args):
+                made.append((name, args))
+                return 64 if name.endswith("_bytes") else 0
+            return entry
+
+    monkeypatch.setattr(_cabi, "load", lambda: Lib())
+    monkeypatch.setattr(_cabi, "stream_of", lambda t: 0)
+    monkeypatch.setattr(_cabi, "call", lambda device, fn, *args: fn(*args))
+    monkeypatch.setattr(ops, "device_status", lambda d: torch.zeros(1, dtype=torch.int32))
+    return made
+
+
+@pytest.mark.parametrize("kind", ["bf16", "nvfp4"])
+def test_few_token_layer_leaves_the_reserved_sms_free(calls, monkeypatch, kind):
+    from types import SimpleNamespace
+    from boltops_b200.fused_moe import fused_experts_decode, ops
+    monkeypatch.setattr(torch.cuda, "get_device_properties", lambda d: SimpleNamespace(multi_processor_count=148))
+    flags = dict(use_fp4_w4a4=True) if kind == "nvfp4" else {}
+    for reserve, used in ((0, 0), (20, 128)):
+        monkeypatch.setattr(ops, "_gemm_sm_reserve", reserve)
+        calls.clear()
+        fused_experts_decode(**_layer(kind), **flags)
+        assert [args[0].sm_count for name, args in calls if name == "bolt_moe_decode"] == [used]
