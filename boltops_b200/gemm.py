@@ -103,15 +103,30 @@ w8a8_triton_block_scaled_mm = w8a8_block_scaled_mm
 w8a8_block_int8_matmul = w8a8_block_scaled_mm
 
 
-# The few-row form reads the weights once at up to half of HBM's rate and computes on small matrix
-# instructions, one column tile per eight rows; the tiled form has a launch more and whole 128-row tiles.
-# Both measured in us, few / tiled: nvfp4 4096 x 7168, 1 row 8.0 / 21.7, 16 11.0 / 22.5, 32 16.7 / 22.6;
-# 7168 x 2048, 32 rows 12.1 / 12.8; 28672 x 8192, 1 row 43.0 / 41.8, 12 58.8 / 39.5; mxfp4 4096 x 7168, 1 row
-# 10.8 / 20.5, 16 14.3 / 20.5, 32 22.6 / 20.7; 7168 x 2048, 16 rows 10.3 / 11.6, 24 13.2 / 11.7; 28672 x
-# 8192, 1 row 59.0 / 37.7.  (Where they are close, the launch saved is worth more to a caller whose
-# kernels wait for its host.)
+# Which form a product of up to 32 rows takes.  The few-row form reads the weights once and computes on small
+# matrix instructions, a column tile per eight rows, so its time grows with weights times row tiles; the tiled
+# form has a launch more and whole 128-row tiles, whatever the rows.  Up to a product of weights and row tiles the
+# former is ahead.  Kernels alone, us, few / tiled:
+#   nvfp4   rows     1          8          16         24         32
+#   4096 x 7168   8.2/22.8   8.5/22.8  10.5/22.8  14.2/22.8  16.0/22.9
+#   7168 x 7168  13.4/23.3  13.9/23.5  17.6/23.5  25.9/23.6  29.7/23.6
+#   8192 x 8192  14.8/25.7  15.5/25.7  19.7/25.9  28.7/25.9  33.2/25.9
+#  16384 x 8192  24.2/34.0  26.6/32.4  35.4/33.0  54.1/33.2  62.1/29.1
+#  28672 x 8192  38.9/43.6  43.1/41.7  58.7/41.2  91.0/39.7 105.6/39.7
+#   mxfp4
+#   4096 x 4096   7.4/15.6   7.8/15.6   9.8/15.7  13.2/15.8  15.0/15.8
+#   4096 x 7168  10.8/20.8  11.1/20.9  14.1/21.0  19.8/21.0  22.5/21.0
+#   7168 x 7168  17.8/21.3  19.0/21.3  25.1/21.5  36.5/21.4  41.6/21.5
+#   8192 x 8192  19.8/23.5  21.6/23.4  28.7/23.5  39.6/23.7  44.9/23.7
+#  16384 x 8192  35.9/31.3  40.6/29.7  54.6/29.9  76.3/29.1  87.7/24.6
+# (a short reduction is best for the tiled form: mxfp4 7168 x 2048, 24 rows 14.2/11.9, where the few-row one
+# still saves a caller that waits for its host a launch)
 _FEW_ROWS = 32
-_FEW_WEIGHTS = 128 << 20
+_FEW_WORK = {"nvfp4": 128 << 20, "mxfp4": 64 << 20}
+
+
+def _takes_few_rows(fmt: str, m: int, n: int, k: int) -> bool:
+    return m <= _FEW_ROWS and n * k * ((m + 7) // 8) <= _FEW_WORK[fmt]
 
 
 def gemm_a4w4(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor, w_scale: torch.Tensor,
@@ -163,7 +178,7 @@ def gemm_a4w4(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor, w_scale: 
     lib = _cabi.load()
     stream = _cabi.stream_of(x)
     out_ld = out.stride(0) if m > 1 else n
-    if m <= _FEW_ROWS and n * k <= _FEW_WEIGHTS:
+    if _takes_few_rows(fmt, m, n, k):
         few = _cabi.Fp4FewArgs(code, m, n, k, x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
                                _cabi.ptr(alpha), out.data_ptr(), _cabi.dtype_code(dtype), out_ld,
                                ops.device_status(dev).data_ptr(), ops.gemm_sm_count(dev))

@@ -319,3 +319,19 @@ def test_few_token_layer_leaves_the_reserved_sms_free(calls, monkeypatch, kind):
         calls.clear()
         fused_experts_decode(**_layer(kind), **flags)
         assert [args[0].sm_count for name, args in calls if name == "bolt_moe_decode"] == [used]
+
+
+@pytest.mark.parametrize("fmt,m,n,k,few", [
+    ("nvfp4", 32, 4096, 7168, True), ("nvfp4", 16, 8192, 8192, True), ("nvfp4", 8, 16384, 8192, True),
+    ("nvfp4", 17, 8192, 8192, False), ("nvfp4", 32, 16384, 8192, False), ("nvfp4", 33, 128, 128, False),
+    ("mxfp4", 32, 4096, 4096, True), ("mxfp4", 16, 4096, 7168, True), ("mxfp4", 8, 8192, 8192, True),
+    ("mxfp4", 32, 4096, 7168, False), ("mxfp4", 9, 8192, 8192, False), ("mxfp4", 1, 16384, 8192, False)])
+def test_the_form_of_a_4bit_product_goes_by_rows_and_weights(calls, fmt, m, n, k, few):
+    """On which side the measured times of the two forms lie, per format."""
+    from boltops_b200.fp4 import FORMATS
+    from boltops_b200.gemm import gemm_a4w4
+    _, block, scale_dtype = FORMATS[fmt]
+    rows = lambda r: (torch.empty(r, k // 2, dtype=torch.uint8), torch.empty(r, k // block, dtype=scale_dtype))  # noqa: E731
+    (x, xs), (w, ws) = rows(m), rows(n)
+    gemm_a4w4(gpu(x), w, xs, ws)
+    assert [name for name, _ in calls] == (["bolt_fp4_gemm_few"] if few else ["bolt_fp4_tile_scales", "bolt_fp4_gemm"])
