@@ -238,6 +238,7 @@ _SIGNATURES = {
     "bolt_fp4_gemm": (C.c_int, [C.POINTER(Fp4GemmArgs), C.c_void_p]),
     "bolt_fp4_gemm_few": (C.c_int, [C.POINTER(Fp4FewArgs), C.c_void_p]),
     "bolt_moe_decode_workspace_bytes": (C.c_size_t, [C.POINTER(DecodeArgs)]),
+    "bolt_moe_decode_kernel_count": (C.c_int, [C.POINTER(DecodeArgs)]),
     "bolt_moe_decode": (C.c_int, [C.POINTER(DecodeArgs), C.c_void_p]),
 }
 

@@ -1270,8 +1270,9 @@ int ring_slots(int smem, int fixed, int slot_bytes, int warps) {
   int slots = (smem - fixed) / (warps * slot_bytes);
   return slots * warps > kMaxBarriers ? kMaxBarriers / warps : slots;
 }
+// `kernels` not null: it becomes the number of kernels, and none is launched.
 template <int K, int NT, int kWarps>
-int launch(const bolt_decode_args* a, Params p, int blocks, cudaStream_t st) {
+int launch(const bolt_decode_args* a, Params p, int blocks, cudaStream_t st, int* kernels) {
   constexpr int kSmem = blocks_of(NT, kWarps) == 2 ? kHalfSmem : bolt::few::kSmem;
   constexpr int kUpSlot = up_box_bytes(K) + up_scale_bytes(K), kDownSlot = kDownBoxBytes + ScaleRing<K, 2 * kDownTiles>::kBytes;
   const int routes = p.tokens * p.topk;
@@ -1298,6 +1299,10 @@ int launch(const bolt_decode_args* a, Params p, int blocks, cudaStream_t st) {
   if (up_slots < 1 || down_slots < 1) {
     set_error("moe_decode: %d tokens of hidden size %d do not fit in shared memory", p.tokens, p.hidden);
     return BOLT_ERR_UNSUPPORTED;
+  }
+  if (kernels != nullptr) {
+    *kernels = 2 + (is8(K) ? !p.keep_x + !p.keep_act : 0);
+    return BOLT_OK;
   }
   static std::atomic<bool> ready[2][kMaxDevices];
   int rc = configure_kernel(k_few_up<K, NT, kWarps>, kSmem, ready[0], 0, 0, 0, 0);
@@ -1358,19 +1363,19 @@ int launch(const bolt_decode_args* a, Params p, int blocks, cudaStream_t st) {
 // nvfp4, one token (140 KB) 18.6 / 19.5, bf16, one token (510 KB) 28.3 / 26.0, two 48 / 41.
 constexpr int64_t kSmallShare = 256 << 10;
 template <int K>
-int launch_kind(const bolt_decode_args* a, const Params& p, cudaStream_t st) {
+int launch_kind(const bolt_decode_args* a, const Params& p, cudaStream_t st, int* kernels) {
   const int sms = a->sm_count > 0 ? a->sm_count : sm_count_of_current_device();
   const int64_t touched = std::min<int64_t>((int64_t)p.tokens * p.topk, p.experts);
   const int64_t share = touched * (2 * p.inter * row_bytes(K, p.hidden) + p.model_dim * row_bytes(K, p.inter)) / sms;
   if (p.tokens <= 8) {
     if (share <= kSmallShare) {
-      const int rc = launch<K, 1, 8>(a, p, sms, st);
+      const int rc = launch<K, 1, 8>(a, p, sms, st, kernels);
       if (rc != BOLT_ERR_UNSUPPORTED) return rc;      // (too many or too long rows for half an SM)
     }
-    return launch<K, 1, warps_of(K, 1)>(a, p, sms, st);
+    return launch<K, 1, warps_of(K, 1)>(a, p, sms, st, kernels);
   }
-  if (p.tokens <= 16) return launch<K, 2, warps_of(K, 2)>(a, p, sms, st);
-  return launch<K, 4, warps_of(K, 4)>(a, p, sms, st);
+  if (p.tokens <= 16) return launch<K, 2, warps_of(K, 2)>(a, p, sms, st, kernels);
+  return launch<K, 4, warps_of(K, 4)>(a, p, sms, st, kernels);
 }
 
 template <int K, int NT>
@@ -1433,10 +1438,7 @@ extern "C" size_t bolt_moe_decode_workspace_bytes(const bolt_decode_args* a) {
 namespace bolt {
 namespace few {
 namespace {
-int decode_once(const bolt_decode_args* a, cudaStream_t st) {
-  int rc = check_args(a);
-  if (rc != BOLT_OK) return rc;
-  if (a->num_tokens == 0) return BOLT_OK;
+int check_operands(const bolt_decode_args* a) {
   const int k = a->kind;
   BOLT_REQUIRE(a->hidden_states && a->w1 && a->w2 && a->out && a->workspace, "moe_decode: null pointer");
   BOLT_REQUIRE(is16(k) || (a->w1_scale && a->w2_scale), "moe_decode: scales required");
@@ -1457,6 +1459,15 @@ int decode_once(const bolt_decode_args* a, cudaStream_t st) {
   BOLT_REQUIRE(!is4(k) || ((reinterpret_cast<uintptr_t>(a->w1_scale) | reinterpret_cast<uintptr_t>(a->w2_scale)) & 3) == 0,
                "moe_decode: scale bytes must be 4-byte aligned");
   BOLT_REQUIRE(a->workspace_bytes >= workspace_bytes(a), "moe_decode: workspace too small");
+  return BOLT_OK;
+}
+
+int decode_once(const bolt_decode_args* a, cudaStream_t st, int* kernels) {
+  int rc = check_args(a);
+  if (rc != BOLT_OK) return rc;
+  if (kernels != nullptr) *kernels = 0;
+  if (a->num_tokens == 0) return BOLT_OK;
+  if (kernels == nullptr && (rc = check_operands(a)) != BOLT_OK) return rc;
   size_t part[kParts];
   workspace_parts(a, part);
 
@@ -1496,32 +1507,26 @@ int decode_once(const bolt_decode_args* a, cudaStream_t st) {
   p.as = reinterpret_cast<float*>(p.aq + part[5]);
   p.status = a->status;
 
-  switch (k) {
-    case K_BF16: return launch_kind<K_BF16>(a, p, st);
-    case K_F16: return launch_kind<K_F16>(a, p, st);
-    case K_F8_BLOCK: return launch_kind<K_F8_BLOCK>(a, p, st);
-    case K_I8_CHANNEL: return launch_kind<K_I8_CHANNEL>(a, p, st);
-    case K_F8_CHANNEL: return launch_kind<K_F8_CHANNEL>(a, p, st);
-    case K_I8_BLOCK: return launch_kind<K_I8_BLOCK>(a, p, st);
-    case K_NV4: return launch_kind<K_NV4>(a, p, st);
-    default: return launch_kind<K_MX4>(a, p, st);
+  switch (a->kind) {
+    case K_BF16: return launch_kind<K_BF16>(a, p, st, kernels);
+    case K_F16: return launch_kind<K_F16>(a, p, st, kernels);
+    case K_F8_BLOCK: return launch_kind<K_F8_BLOCK>(a, p, st, kernels);
+    case K_I8_CHANNEL: return launch_kind<K_I8_CHANNEL>(a, p, st, kernels);
+    case K_F8_CHANNEL: return launch_kind<K_F8_CHANNEL>(a, p, st, kernels);
+    case K_I8_BLOCK: return launch_kind<K_I8_BLOCK>(a, p, st, kernels);
+    case K_NV4: return launch_kind<K_NV4>(a, p, st, kernels);
+    default: return launch_kind<K_MX4>(a, p, st, kernels);
   }
 }
-}  // namespace
-}  // namespace few
-}  // namespace bolt
-
-extern "C" int bolt_moe_decode(const bolt_decode_args* a, void* stream) {
-  using namespace bolt;
-  using namespace bolt::few;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int rc = decode_once(a, st);
+// (`kernels` as in launch)
+int decode(const bolt_decode_args* a, cudaStream_t st, int* kernels) {
+  const int rc = decode_once(a, st, kernels);
   if (rc != BOLT_ERR_UNSUPPORTED || a->num_tokens < 2) return rc;
   // the 4-bit codes of all rows do not fit in shared memory: half of the tokens after the other (they read
   // the experts that both touch twice)
   bolt_decode_args part = *a;
   part.num_tokens = a->num_tokens / 2;
-  const int first = bolt_moe_decode(&part, stream);
+  const int first = decode(&part, st, kernels);
   if (first != BOLT_OK) return first;
   const int64_t done = part.num_tokens;
   part.num_tokens = a->num_tokens - part.num_tokens;
@@ -1533,7 +1538,22 @@ extern "C" int bolt_moe_decode(const bolt_decode_args* a, void* stream) {
     part.topk_weights = a->topk_weights + done * a->topk;
   }
   part.out = static_cast<uint8_t*>(a->out) + done * a->model_dim * dtype_bytes(a->out_dtype);
-  return bolt_moe_decode(&part, stream);
+  int more = 0;
+  const int second = decode(&part, st, kernels != nullptr ? &more : nullptr);
+  if (kernels != nullptr) *kernels += more;
+  return second;
+}
+}  // namespace
+}  // namespace few
+}  // namespace bolt
+
+extern "C" int bolt_moe_decode(const bolt_decode_args* a, void* stream) {
+  return bolt::few::decode(a, static_cast<cudaStream_t>(stream), nullptr);
+}
+
+extern "C" int bolt_moe_decode_kernel_count(const bolt_decode_args* a) {
+  int kernels = 0;
+  return bolt::few::decode(a, nullptr, &kernels) == BOLT_OK ? kernels : -1;
 }
 
 extern "C" int bolt_fp4_gemm_few(const bolt_fp4_few_args* a, void* stream) {

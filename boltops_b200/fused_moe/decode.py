@@ -230,10 +230,11 @@ def _decode(hidden_states, w1, w2, topk_weights, topk_ids, gating, topk, renorma
     args.workspace, args.workspace_bytes = workspace.data_ptr(), need
     with _cabi.on_device(dev):
         status = lib.bolt_moe_decode(args, _cabi.stream_of(x))
+        kernels = lib.bolt_moe_decode_kernel_count(args)
     if status == _cabi.BOLT_ERR_UNSUPPORTED:
         raise NotImplementedError(lib.bolt_last_error().decode(errors="replace"))
     _cabi.check(status)
-    ops._count(2)
+    ops._count(kernels)
     return out
 
 

@@ -733,6 +733,9 @@ typedef struct bolt_decode_args {
  * go half by half).  Sizes: hidden and inter multiples of 8
  * (16-bit), 16 (per-channel), 128 (block-scaled, MX) or 64 (NV); block-scaled model_dim a multiple of 128. */
 size_t bolt_moe_decode_workspace_bytes(const bolt_decode_args* args);
+/* Kernels that bolt_moe_decode launches for these sizes on the current device (pointers are not looked at);
+ * -1: invalid. */
+int bolt_moe_decode_kernel_count(const bolt_decode_args* args);
 int bolt_moe_decode(const bolt_decode_args* args, void* stream);
 
 #ifdef __cplusplus

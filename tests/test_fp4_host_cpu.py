@@ -335,3 +335,35 @@ def test_the_form_of_a_4bit_product_goes_by_rows_and_weights(calls, fmt, m, n, k
     (x, xs), (w, ws) = rows(m), rows(n)
     gemm_a4w4(gpu(x), w, xs, ws)
     assert [name for name, _ in calls] == (["bolt_fp4_gemm_few"] if few else ["bolt_fp4_tile_scales", "bolt_fp4_gemm"])
+
+
+def test_few_token_layer_says_how_many_kernels_it_launches(lib):
+    """Two; one more where 8-bit rows, or activations, are quantised by a kernel of their own; as many again for
+    every part of a batch whose 4-bit rows do not fit together."""
+    from boltops_b200 import _cabi
+
+    def count(kind, m, h, i, k=8):
+        a = _cabi.DecodeArgs(kind=getattr(_cabi, "DECODE_" + kind), num_tokens=m, topk=k, hidden=h, inter=i, model_dim=1024,
+                             num_experts=8, global_num_experts=8, sm_count=148)
+        return lib.bolt_moe_decode_kernel_count(a)
+    assert count("BF16", 0, 1024, 512) == 0 and count("BF16", 32, 1024, 512) == 2
+    for kind in ("FP8_BLOCK", "INT8_BLOCK", "FP8_CHANNEL", "INT8_CHANNEL"):
+        assert count(kind, 8, 1024, 512) == 2
+        assert count(kind, 8, 16384, 256) == 3      # the rows
+        assert count(kind, 8, 1024, 2176) == 3      # the activations
+        assert count(kind, 9, 1024, 512) == 4       # both
+    assert count("NVFP4", 32, 1024, 512) == 2 and count("NVFP4", 32, 16384, 512) == 8       # four times eight tokens
+    assert count("BF16", 33, 1024, 512) == -1 and count("BF16", 1, 1020, 512) == -1
+    assert lib.bolt_moe_decode_kernel_count(None) == -1
+
+
+@pytest.mark.parametrize("kernels", [2, 4])
+def test_few_token_layer_counts_its_launches(calls, monkeypatch, kernels):
+    from boltops_b200 import _cabi
+    from boltops_b200.fused_moe import fused_experts_decode, ops
+    lib = _cabi.load()
+    type(lib).bolt_moe_decode_kernel_count = lambda self, args: kernels
+    monkeypatch.setattr(_cabi, "load", lambda: lib)
+    before = ops.launch_count()
+    fused_experts_decode(**_layer())
+    assert ops.launch_count() - before == kernels
