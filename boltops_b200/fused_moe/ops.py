@@ -121,7 +121,7 @@ def moe_sorting_ck(topk_ids: torch.Tensor, topk_weights: torch.Tensor, num_exper
             ptr(num_valid), ptr(route_pos), ptr(segments), ptr(num_segments), segment_rows,
             ptr(moe_buf), 0 if moe_buf is None else moe_buf.numel() * moe_buf.element_size(),
             ptr(ws), ws_bytes, stream_of(topk_ids)))
-    _count(1 if ws_bytes <= 16 else 3)
+    _count(1 if ws_bytes <= 16 else 2)
     if segment_rows > 0:
         return (sorted_ids, sorted_weights, sorted_expert_ids, num_valid, positions, moe_buf,
                 segments, num_segments)
@@ -164,7 +164,7 @@ def moe_align_block_size(topk_ids: torch.Tensor, block_size: int, num_experts: i
         check(lib.bolt_moe_align_block_size(
             ptr(ids), numel, num_experts, block_size, ptr(expert_map), ptr(sorted_ids),
             ptr(expert_ids), ptr(num_post), ptr(ws), ws_bytes, stream_of(ids)))
-    _count(1 if ws_bytes <= 16 else 3)
+    _count(1 if ws_bytes <= 16 else 2)
     return sorted_ids, expert_ids, num_post
 
 
