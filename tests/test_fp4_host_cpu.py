@@ -372,7 +372,8 @@ def test_few_token_layer_counts_its_launches(calls, monkeypatch, kernels):
 def test_a_sort_counts_one_kernel_or_two(calls):
     from boltops_b200.fused_moe import ops
     ids = gpu(torch.zeros(4, 2, dtype=torch.int32))
-    for sort in (lambda: ops.moe_sorting_ck(ids, torch.ones(4, 2), 4), lambda: ops.moe_align_block_size(ids, 32, 4)):
+    weights = gpu(torch.ones(4, 2))
+    for sort in (lambda: ops.moe_sorting_ck(ids, weights, 4), lambda: ops.moe_align_block_size(ids, 32, 4)):
         before = ops.launch_count()
         sort()      # (a workspace of 64 bytes: the form for many routes, which has no scan kernel)
         assert ops.launch_count() - before == 2
