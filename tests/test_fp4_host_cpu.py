@@ -304,6 +304,7 @@ def calls(monkeypatch):
     monkeypatch.setattr(_cabi, "load", lambda: Lib())
     monkeypatch.setattr(_cabi, "stream_of", lambda t: 0)
     monkeypatch.setattr(_cabi, "call", lambda device, fn, *args: fn(*args))
+    monkeypatch.setattr(ops, "stream_of", lambda t: 0)
     monkeypatch.setattr(ops, "device_status", lambda d: torch.zeros(1, dtype=torch.int32))
     return made
 
