@@ -212,7 +212,7 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
         tc_fence_after();
         for (int kb = 0; kb < p.num_kb; ++kb) {
           ok = mbar_wait(bar_full + 8 * s, ph, abort_flag, p.status, 42) &&
-               mbar_wait(bar_sf + 8 * set, sph, abort_flag, p.status, 44);
+               mbar_wait(bar_sf + 8 * set, sph, abort_flag, p.status, 43);
           if (!ok) break;
           tc_fence_after();
           const uint32_t sa = smem_base + s * S::kOperandBytes;
@@ -250,7 +250,7 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CU
         if (t.expert < 0) continue;
         for (int kb = 0; kb < p.num_kb; ++kb) {
           ok = mbar_wait(bar_full + 8 * s, ph, abort_flag, p.status, 42) &&
-               mbar_wait(bar_sf_free + 8 * set, sph ^ 1, abort_flag, p.status, 44);
+               mbar_wait(bar_sf_free + 8 * set, sph ^ 1, abort_flag, p.status, 43);
           if (!ok) break;
           tc_fence_after();
           const uint32_t sf = sf_base + s * S::kSfBytes;

@@ -512,8 +512,8 @@ def set_gemm_sm_reserve(sms: int) -> None:
 
 
 def device_status(device: torch.device) -> torch.Tensor:
-    """Per-device int32 word that the grouped GEMM and the expert-parallel exchange kernels set
-    when a bounded device-side wait expired (0 = healthy).  Reading it synchronises; kernels
+    """Per-device int32 word that the products, the few-token layer and the expert-parallel exchange
+    kernels set when a bounded device-side wait expired (0 = healthy).  Reading it synchronises; kernels
     never do."""
     key = torch.device(device).index or 0
     if key not in _status_words:
@@ -526,7 +526,8 @@ def check_device_status(device: torch.device) -> None:
     if code != 0:
         device_status(device).zero_()
         raise _cabi.BoltError(f"a kernel reported an expired device-side wait (code {code}: 1-6 grouped "
-                              f"GEMM, 20 exchange barrier, 21 exchange segment overflow)")
+                              f"GEMM, 20 exchange barrier, 21 exchange segment overflow, 30 few-token layer or "
+                              f"few-row 4-bit product, 40-43 tiled 4-bit product)")
 
 
 def gemm_sm_count(device) -> int:

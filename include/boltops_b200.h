@@ -658,7 +658,8 @@ typedef struct bolt_fp4_gemm_args {
   const int32_t* num_valid_ids;
   int activation;              /* enum bolt_activation, gated                                 */
   float act_alpha, act_limit;
-  int32_t* status;             /* optional, set to 40 to 43 by a wait that ran out            */
+  int32_t* status;             /* optional, set by a wait that ran out: 40 for a free stage, 41 for the */
+                               /*   accumulator, 42 for operands, 43 for scales in TMEM       */
   int sm_count;                /* blocks to launch; 0: one per SM                             */
 } bolt_fp4_gemm_args;
 
@@ -676,7 +677,7 @@ typedef struct bolt_fp4_few_args {
   void* out;                   /* [rows, n], rows out_ld elements apart                       */
   int out_dtype;
   int64_t out_ld;
-  int32_t* status;             /* optional, set to 30 by a wait that ran out                  */
+  int32_t* status;             /* optional, set to 30 by a wait for weights that ran out      */
   int sm_count;                /* blocks to launch; 0: one per SM                             */
 } bolt_fp4_few_args;
 int bolt_fp4_gemm_few(const bolt_fp4_few_args* args, void* stream);
@@ -725,7 +726,7 @@ typedef struct bolt_decode_args {
                                /*   without a local expert                                    */
   void* workspace;             /* contents do not matter; one call at a time                  */
   size_t workspace_bytes;
-  int32_t* status;             /* optional, as in bolt_gemm_args; 30: a weight copy did not land */
+  int32_t* status;             /* optional, set to 30 by a wait for weights that ran out      */
   int sm_count;                /* SMs to use; 0: all (the second kernel then starts beside the first) */
 } bolt_decode_args;
 

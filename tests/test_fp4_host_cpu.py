@@ -378,3 +378,22 @@ def test_a_sort_counts_one_kernel_or_two(calls):
         before = ops.launch_count()
         sort()      # (a workspace of 64 bytes: the form for many routes, which has no scan kernel)
         assert ops.launch_count() - before == 2
+
+
+def test_expired_waits_are_named(monkeypatch):
+    """Every code that the 4-bit kernels can leave has a meaning in the header and in the error."""
+    from boltops_b200 import _cabi
+    from boltops_b200.fused_moe import ops
+    header = (ROOT / "include" / "boltops_b200.h").read_text()
+    codes = set()
+    for source in ("few_tokens.cu", "fp4_gemm.cu"):
+        text = (ROOT / "boltops_b200" / "csrc" / source).read_text()
+        codes |= {int(c) for c in re.findall(r"\bstatus, (\d+)\)", text)}
+    assert codes == {30, 40, 41, 42, 43}
+    for code in codes:
+        assert f"set to {code} by a wait" in header or f"{code} for " in header
+        word = torch.tensor([code], dtype=torch.int32)
+        monkeypatch.setattr(ops, "device_status", lambda d: word)
+        with pytest.raises(_cabi.BoltError, match="30 few-token layer" if code == 30 else "40-43 tiled 4-bit product"):
+            ops.check_device_status(torch.device("cuda"))
+        assert not word.any()
