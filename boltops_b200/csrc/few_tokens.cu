@@ -33,6 +33,7 @@
 
 #include "act_pair.cuh"
 #include "routing_row.cuh"
+#include "tensor_map.cuh"
 #include "token_mma.cuh"
 
 namespace bolt {
@@ -654,7 +655,6 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
     const int e = r.list[unit.a], c0 = unit.c * UC;
     const int off = r.off[unit.a], cnt = __popc(r.mask[unit.a]);
     const unsigned live = (1u << ((cnt + 7) / 8)) - 1u;
-    const uint32_t live_cols = cnt == 32 ? ~0u : (1u << cnt) - 1u;
     float acc[NT / TG][MT][TG][4];
 #pragma unroll
     for (int n = 0; n < NT / TG; ++n) zero_sums(acc[n]);
@@ -833,7 +833,7 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
   const int64_t boxes = (int64_t)(u1 - u0) * r.touched * nb;
   const int n_it = boxes > warp ? (int)((boxes - warp + kWarps - 1) / kWarps) : 0;
 
-  // boxes in the order (unit, expert, place in the reduction), every eighth this warp's
+  // boxes in the order (unit, expert, place in the reduction), to the warps in turn
   struct Place {
     int u, a, kb;
   };
@@ -1038,8 +1038,7 @@ constexpr int dense_warps(int k, int nt) { return nt == 4 || k == K_MX4 ? 8 : 16
 template <int K, int NT>
 __global__ void __launch_bounds__(32 * dense_warps(K, NT), 1)
 k_few_dense(const __grid_constant__ CUtensorMap map, const DenseParams p) {
-  constexpr int MT = kDownTiles, kBox = kDownBoxBytes, kWarps = dense_warps(K, NT), kThreads = 32 * kWarps,
-                TG = NT;
+  constexpr int MT = kDownTiles, kBox = kDownBoxBytes, kWarps = dense_warps(K, NT), kThreads = 32 * kWarps;
   const int UR = p.unit;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = carve(raw);
@@ -1106,9 +1105,8 @@ k_few_dense(const __grid_constant__ CUtensorMap map, const DenseParams p) {
   const float alpha = p.alpha != nullptr ? *p.alpha : 1.f;
 
   for (int u = u0; u < u1; ++u) {
-    float acc[NT / TG][MT][TG][4];
-#pragma unroll
-    for (int n = 0; n < NT / TG; ++n) zero_sums(acc[n]);
+    float acc[1][MT][NT][4];
+    zero_sums(acc[0]);
     while (it < n_it && cur.u == u) {
       auto load_x = [&](TokenBox<K>& x, int nt) {
         const int m = 8 * nt + g;
@@ -1127,24 +1125,17 @@ k_few_dense(const __grid_constant__ CUtensorMap map, const DenseParams p) {
       cp_async_wait(p.slots_per_warp - 1);
       if (K != K_NV4) __syncwarp();
       scales.read(ws, ring.s_out, lane);
-      TokenBox<K> x[TG];
+      TokenBox<K> x[NT];
 #pragma unroll
-      for (int j = 0; j < TG; ++j) load_x(x[j], j);
+      for (int j = 0; j < NT; ++j) load_x(x[j], j);
       const uint32_t box = ring.wait(abort_flag, p.status);
-#pragma unroll
-      for (int n = 0; n < NT / TG; ++n) {
-        if (n > 0) {
-#pragma unroll
-          for (int j = 0; j < TG; ++j) load_x(x[j], n * TG + j);
-        }
-        box_mma<K, MT, TG, false>(box, 0, lane, x, ws, live >> (n * TG), acc[n]);
-      }
+      box_mma<K, MT, NT, false>(box, 0, lane, x, ws, live, acc[0]);
       ring.release();
       bring();
       cur.kb += kWarps;
       if (++it < n_it) settle(cur);
     }
-    put_sums<MT, NT, TG>(red, acc, warp, lane, live);
+    put_sums<MT, NT, NT>(red, acc, warp, lane, live);
     __syncthreads();
     for (int i = tid; i < p.rows * kMaxRows; i += kThreads) {
       const int n = i / kMaxRows, c = i % kMaxRows, col = u * UR + c;
@@ -1163,23 +1154,6 @@ k_few_dense(const __grid_constant__ CUtensorMap map, const DenseParams p) {
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static const EncodeTiledFn fn = [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess)
-      return reinterpret_cast<EncodeTiledFn>(ptr);
-    return EncodeTiledFn(nullptr);
-  }();
-  return fn;
-}
-
 int encode(CUtensorMap* map, const void* base, int dims, const cuuint64_t* size, const cuuint64_t* strides,
            const cuuint32_t* box) {
   const EncodeTiledFn fn = encode_fn();

@@ -16,9 +16,6 @@
 namespace bolt {
 namespace fp4 {
 
-template <bool NV>
-constexpr int kBlock = NV ? 16 : 32;
-
 __device__ __forceinline__ bool finite_amax(float amax) {
   return __float_as_uint(amax) < 0x7F800000u;      // amax is not negative
 }
@@ -87,7 +84,7 @@ __device__ __forceinline__ float quotient(float v, const Scaler& k) {
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(lo, hi), __NV_E2M1, cudaRoundNearest);
 }
-// eight values -> eight codes; `ok` false (a block without finite values): codes 0
+// eight values -> eight codes; k.r of 0 (a block of zeros or without finite values): codes 0
 template <bool NV>
 __device__ __forceinline__ uint32_t codes8(const float* v, const Scaler& k) {
   // (0 * infinity would be a NaN, and a NaN has no code: blocks with either have k.r = 0)

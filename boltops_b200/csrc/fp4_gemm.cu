@@ -24,6 +24,7 @@
 #include "fp4.cuh"
 #include "row_store.cuh"
 #include "tc_ptx.cuh"
+#include "tensor_map.cuh"
 
 namespace bolt {
 namespace fp4gemm {
@@ -463,23 +464,6 @@ __global__ void __launch_bounds__(256) k_tile_scales(const TileParams p) {
         if (piece * 16 + 4 * k < job.row_bytes) *reinterpret_cast<uint4*>(dst + 512 * k) = out[k];
     }
   }
-}
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static const EncodeTiledFn fn = [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess)
-      return reinterpret_cast<EncodeTiledFn>(ptr);
-    return EncodeTiledFn(nullptr);
-  }();
-  return fn;
 }
 
 template <bool NV, int BN, bool GATED>

@@ -34,6 +34,7 @@
 #include "row_store.cuh"
 #include "stream_gemm.cuh"
 #include "tc_ptx.cuh"
+#include "tensor_map.cuh"
 
 namespace bolt {
 namespace {
@@ -1433,24 +1434,6 @@ k_mx_gemm(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUt
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn get_encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (fn == nullptr) {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) ==
-            cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-  }
-  return fn;
-}
-
 template <int OPK, bool BS, int EPI, bool PAIR, bool slots>
 int launch_form(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mc,
                 const GemmParams& p, int grid, cudaStream_t st) {
@@ -1619,7 +1602,7 @@ extern "C" int bolt_grouped_gemm(const bolt_gemm_args* a, void* stream) {
                  "grouped_gemm: a_row_bytes must be a multiple of 16 and cover a row");
   }
 
-  EncodeTiledFn encode = get_encode_fn();
+  const EncodeTiledFn encode = encode_fn();
   if (encode == nullptr) {
     set_error("grouped_gemm: cuTensorMapEncodeTiled is unavailable");
     return BOLT_ERR_CUDA;
