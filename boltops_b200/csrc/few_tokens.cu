@@ -389,6 +389,9 @@ constexpr int warps_of(int k, int nt) { return k == K_MX4 && nt > 1 ? 8 : 16; }
 constexpr int tiles_at_once(int k, int nt) { return nt == 4 && k != K_MX4 ? 1 : nt; }
 // blocks an SM holds as far as registers go: the second kernel's beside the first's
 constexpr int blocks_of(int nt, int warps) { return nt == 1 && warps == 8 ? 2 : 1; }
+// boxes that a warp's ring brings ahead, at most: six slots for one of eight warps with an SM's shared memory to
+// themselves, three for the others
+constexpr int most_pending(int warps, bool half_sm) { return warps == 8 && !half_sm ? 5 : 2; }
 constexpr int red_bytes(int warps, int mt, int nt) { return warps * mt * nt * 128 * 4; }
 // bytes of a kept row of codes: 16 more than it has, so that eight rows lie in different banks
 __host__ __device__ constexpr int code_pitch(int k, int n) { return (int)row_bytes(k, n) + 16; }
@@ -700,7 +703,7 @@ k_few_up(const __grid_constant__ CUtensorMap map, const Params p) {
         if ((live >> j) & 1u) load_x(x[j], j, tok[j]);
       RowScales<K> ws[MT];
       if constexpr (is4(K) || is_block(K)) {
-        cp_async_wait(p.slots_per_warp - 1);
+        cp_async_wait<most_pending(kWarps, NT == 1)>(p.slots_per_warp - 1);
         if (K != K_NV4) __syncwarp();
         scales.read(ws, ring.s_out, lane);
       }
@@ -966,7 +969,7 @@ k_few_down(const __grid_constant__ CUtensorMap map, const Params p) {
       }
       const float whole = is4(K) ? (p.g2 != nullptr ? p.g2[e] : 1.f) * (p.a2 != nullptr ? *p.a2 : 1.f) : 1.f;
       RowScales<K> ws[MT];
-      cp_async_wait(p.slots_per_warp - 1);
+      cp_async_wait<most_pending(kWarps, NT == 1)>(p.slots_per_warp - 1);
       if (K != K_NV4) __syncwarp();
       scales.read(ws, ring.s_out, lane);
       const uint32_t box = ring.wait(abort_flag, p.status);
@@ -1122,7 +1125,7 @@ k_few_dense(const __grid_constant__ CUtensorMap map, const DenseParams p) {
         }
       };
       RowScales<K> ws[MT];
-      cp_async_wait(p.slots_per_warp - 1);
+      cp_async_wait<most_pending(kWarps, false)>(p.slots_per_warp - 1);
       if (K != K_NV4) __syncwarp();
       scales.read(ws, ring.s_out, lane);
       TokenBox<K> x[NT];

@@ -288,12 +288,14 @@ __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool h
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(have ? 4u : 0u) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// All but the newest `pending` groups of this thread have landed.
+// All but the newest `pending` groups of this thread have landed; MOST: the deepest ring's slots less one (a
+// deeper one would wait for more than it has to).
+template <int MOST, int AT = 0>
 __device__ __forceinline__ void cp_async_wait(int pending) {
-  if (pending <= 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
-  else if (pending == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-  else if (pending == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
-  else asm volatile("cp.async.wait_group 3;" ::: "memory");
+  if constexpr (AT < MOST) {
+    if (pending > AT) return cp_async_wait<MOST, AT + 1>(pending);
+  }
+  asm volatile("cp.async.wait_group %0;" ::"n"(AT) : "memory");
 }
 
 // A warp's ring of weight scales, beside its ring of boxes and as far ahead: read when they are needed,
