@@ -278,3 +278,55 @@ def test_situ_and_step_activations():
         return (g * torch.sigmoid(g)).clamp(max=0.7) * u.clamp(-0.7, 0.7)
     run("bf16", 4, 256, 128, 5, 2, activation="situ", activation_situ_beta=2.0, act=situ)
     run("f16", 4, 256, 128, 5, 2, activation="swiglustep", gemm1_limit=0.7, act=step)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8_channel", "int8_channel", "nvfp4", "mxfp4"])
+@pytest.mark.parametrize("hout", [1, 3, 7, 33])
+def test_output_sizes_below_and_beside_a_unit(kind, hout):
+    run(kind, 4, 256, 128, 1, 2, hout=hout, output_dtype=torch.float32)
+    run(kind, 4, 256, 128, 19, 2, hout=hout)
+
+
+@pytest.mark.parametrize("m", [1, 3, 20])
+def test_router_of_all_experts_of_one_and_of_views(m):
+    """Every expert chosen; one expert; logits in a wider array; logits that are NaN or infinite."""
+    for e, topk in ((8, 8), (1, 1), (5, 4)):
+        w1, w2 = experts("bf16", e, 64, 16)
+        x = rows("bf16", m, 64, m).cuda()
+        wide = torch.randn(m, e + 3, generator=torch.Generator().manual_seed(m)).cuda()
+        view = wide[:, 2:2 + e]
+        sick = view.clone()
+        sick[0, 0], sick[-1, -1] = float("nan"), float("-inf")
+        for logits in (view, sick, torch.full_like(sick, float("nan"))):
+            weights, ids = fused_topk(x, logits.contiguous(), topk, True)
+            got = fused_moe_decode(x, logits, w1[0].cuda(), w2[0].cuda(), topk, True)
+            want = fused_experts_decode(x, w1[0].cuda(), w2[0].cuda(), weights, ids)
+            assert torch.equal(torch.nan_to_num(got, nan=7.0), torch.nan_to_num(want, nan=7.0))
+
+
+def test_calls_with_reserved_sms_and_without_alternate():
+    """The second kernel starts early in one and waits in the other; both on two streams, and in a graph."""
+    w1, w2 = experts("int8_channel", 6, 512, 256)
+    d1, d2, kw = arguments("int8_channel", w1, w2)
+    weights, ids = (t.cuda() for t in routing(12, 6, 2, 3))
+    x = rows("int8_channel", 12, 512, 4).cuda()
+
+    def call(reserve):
+        ops.set_gemm_sm_reserve(reserve)
+        try:
+            return fused_experts_decode(x, d1, d2, weights, ids, **kw)
+        finally:
+            ops.set_gemm_sm_reserve(0)
+    want = {r: call(r) for r in (0, 40)}
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 2]):
+            streams[i % 2].wait_stream(torch.cuda.default_stream())
+            got.append((call(40 * (i % 3 == 0)), want[40 * (i % 3 == 0)]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ys = [call(r) for r in (40, 0, 40)]
+    graph.replay()
+    assert torch.equal(ys[0], want[40]) and torch.equal(ys[1], want[0]) and torch.equal(ys[2], want[40])
