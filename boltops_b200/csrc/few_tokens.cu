@@ -6,9 +6,10 @@
 // activation; k_few_down: routing again, Q2, the down projection and the weighted sum over a token's
 // experts.  Nothing is sorted or copied: with so few tokens the routing is a bit mask of tokens per
 // touched expert, which every block builds for itself in shared memory.  (8-bit rows or activations whose
-// codes do not fit beside a block's rings are quantised by k_few_codes in between.)
+// codes do not fit beside a block's rings are quantised by k_few_codes in between; 4-bit rows whose codes do not
+// fit in shared memory go part by part, each by its own pair of kernels.)
 //
-// What bounds it: the weights of the touched experts, read once each from HBM.  Split: k_few_up's unit
+// What bounds it: the weights of the touched experts, read from HBM once each (once a part).  Split: k_few_up's unit
 // is up to 16 (MX: 32) intermediate columns of one expert, gate and up rows together over the whole hidden
 // size, so that activation and (4-bit experts) the block quantiser run on finished sums; k_few_down's
 // unit is up to 32 output columns over ALL touched experts, so that the sum over a token's experts stays in
@@ -19,8 +20,8 @@
 // waits for another, nothing is counted in memory, and results do not depend on timing.
 //
 // Measured (graph replays, weights apart from call to call): Mixtral bf16, one token 114 us, 6.2 TB/s of
-// weights; DeepSeek-V3 fp8, one token 85 us, 4.1 TB/s, eight 468 us, 5.4 TB/s; nvfp4, one token 64 us, eight
-// 372 us, 3.8 TB/s.  Beside HBM they wait for: two prologues of 3 us each (instructions that are not in the
+// weights; DeepSeek-V3 fp8, one token 85 us, 4.1 TB/s, eight 468 us, 5.4 TB/s (the row tiles of bolt_moe_layer
+// take 410); nvfp4, one token 64 us, eight 372 us, 3.8 TB/s.  Beside HBM they wait for: two prologues of 3 us each (instructions that are not in the
 // cache yet, routing, the first loads), and with 4-bit codes the ALU: widening a code and scaling it costs
 // about 2.3 instructions a weight pair, as long as HBM takes to bring it.
 //
@@ -372,8 +373,9 @@ __device__ __forceinline__ float get_sum(const float* red, int warps, int mt, in
 }
 
 // Boxes hold up to 32 weight rows (64 for MX's gate and up rows: a block of 32 columns is quantised
-// at once).  Sixteen warps an SM hide the latencies of a box that eight do not, as far as registers
-// allow: the sums of 32 tokens, and MX with its scales apart, need more than 128.
+// at once).  Sixteen warps an SM hide the latencies of a box that eight do not, with 128 registers a thread:
+// MX above eight tokens, with its scales apart, needs more and takes eight warps.  Of the forms for more than 16
+// tokens NV spills 312 bytes a thread in the first kernel, the block-scaled ones 116 and 124, the others up to 40.
 constexpr int kMaxRows = 32;
 constexpr int up_tiles(int k) { return k == K_MX4 ? 4 : 2; }
 constexpr int up_box_bytes(int k) { return up_tiles(k) * 2048; }

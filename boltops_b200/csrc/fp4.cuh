@@ -3,7 +3,8 @@
 // A code is e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign), two to a byte, the first in the low bits.
 //   NV: blocks of 16, the scale an E4M3 byte: s = e4m3(min(amax * (1/6), 448)), code = e2m1(v / s)
 //   MX: blocks of 32, the scale an E8M0 byte: the smallest 2^e with amax <= 6 * 2^e, 0 for a block
-//       of zeros, code = e2m1(v / 2^e)
+//       of zeros, code = e2m1(v / 2^e).  (The OCP MX specification's conversion, 2^(floor(log2 amax) - 2), is
+//       half of that for amax between 6 and 8 times a power of two, and saturates there.)
 // Codes are rounded to the nearest, ties to even, magnitudes above 6 to 6 (only NV has them: its
 // scale may have been rounded down).  A block that holds a NaN or an infinity gets the NaN byte
 // (0x7F, 0xFF) and codes 0.

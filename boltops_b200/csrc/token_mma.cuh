@@ -2,17 +2,22 @@
 // few-token layer and the few-row 4-bit projection.
 //
 // At these sizes a product reads every weight once for a handful of multiply-adds, so it is bound by
-// HBM, and what matters is that every SM always has enough bytes in flight and spends few
-// instructions per byte:
+// HBM, and what matters is that every SM has enough bytes in flight and spends few instructions per
+// byte:
 //
 // * Each warp owns a ring of shared-memory slots and fills it itself with bulk
 //   tensor copies of (rows x 128 bytes) boxes; no warp waits for another inside a reduction.  The
 //   warps share out the boxes of a unit (a few weight rows over the whole reduction) and add up
-//   their accumulators through shared memory once per unit.
+//   their accumulators through shared memory once per unit.  A ring has two or three slots beside sums and
+//   kept codes, up to six for eight warps with an SM to themselves, and one where MX boxes are 8 KB (gate and
+//   up rows of 32 columns) or 4-bit rows fill the memory: then only the other warps' boxes are in
+//   flight while a warp computes.
 // * The weights are the A operand (16 rows) of mma.sync.m16n8k16, the tokens its eight columns.
 //   tcgen05 wants 128 rows on the A side and its operands in shared memory in their final format;
 //   here the 8- and 4-bit codes are widened to halves in registers on the way (exact: e4m3, int8
-//   and e2m1 x e4m3 all fit a half), and the instruction rate is far from what bounds the kernel.
+//   and e2m1 x e4m3 all fit a half).  Products are exact and sums fp32, those of int8 codes too: they
+//   can round from 2^24 on, which a block-scaled group of 128 never reaches and 1041 of the largest codes do.  Widening
+//   is what bounds the 4-bit kinds, and all kinds once several token tiles use the same weights.
 // * The K order inside a box is free as long as both operands agree.  A lane takes 32 contiguous
 //   bytes of its row (two 16-byte chunks, which the 128-byte swizzle places without bank
 //   conflicts), and the same 32 bytes' worth of its token.  MX codes go by 4-byte words instead, so

@@ -3,7 +3,10 @@
 Two formats.  ``"nvfp4"``: blocks of 16 values, an E4M3 scale each, optionally one fp32 scale for the
 whole tensor.  ``"mxfp4"``: blocks of 32, an E8M0 scale (a power of two) each.  Codes are packed two to
 a byte along the last dimension, the first value in the low bits; a tensor's format is the dtype of
-its scales, ``torch.float8_e4m3fn`` or ``torch.uint8``, wherever the framework takes one.  The products
+its scales, ``torch.float8_e4m3fn`` or ``torch.uint8``, wherever the framework takes one.  (mxfp4 scales are chosen so
+that no value saturates.  The OCP MX specification's conversion takes ``2 ** (floor(log2(amax)) - 2)`` instead,
+half of it where amax is more than 6 and less than 8 times a power of two, and saturates there.  Both are valid
+encodings, and whatever reads codes and scales takes either.)  The products
 that read them: ``gemm.gemm_a4w4``, ``fused_moe.fused_experts_fp4`` and ``fused_moe.fused_experts_decode``.
 """
 from __future__ import annotations

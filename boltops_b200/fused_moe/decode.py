@@ -5,20 +5,38 @@ combines in five to seven launches.  With one or a few tokens these launches and
 a large part of the time.  The forms here take 1 to 32 tokens and leave out everything but
 the weights: routing is a bit mask per expert that every block of the kernel builds for itself, the
 first kernel does gate, up and activation, the second the down projection and the sum over a token's
-experts, and it fills its weight rings while the first one finishes.  (8-bit codes that a block cannot keep
-beside its rings, as a rule above eight tokens, are made by a small kernel in front of either.)
+experts, and it fills its weight rings while the first one finishes.  (8-bit rows and activations whose codes a
+block cannot keep beside its rings, as a rule above eight tokens, are quantised by a kernel of their own in front
+of either.  4-bit rows that do not fit in shared memory together, 32 tokens above about 5000 hidden columns, go
+in two parts or more, which read the experts that they share again.)
 
-With 4-bit experts the work of widening codes grows with the tokens, while ``fused_experts_fp4`` pays once for the
-scales of all experts, so which is faster turns over.  128 experts of 2048 x 768, eight a token, kernels
-alone (here / there): nvfp4 51 / 63 us at 4 tokens, 67 / 76 at 8, 116 / 93 at 16, 202 / 110 at 32; mxfp4 28 / 37 at
-one, 58 / 54 at 4, 165 / 82 at 16.  Called one by one from Python the layer there costs at least 130 us on the
-host, here 33.
+Which layer to call.  Every eight tokens cost a pass of small matrix instructions over widened weights, where
+the tensor-core tiles of ``fused_experts`` take up to 128 rows at once, so the forms here are for one to four
+tokens.  Kernels alone, us, here / there, routes at random:
+
+    tokens                           1          2          4          8         16         32
+    Mixtral, bf16                114/154    194/219    324/358    411/412    511/445    780/448
+    Mixtral, fp8 block            72/128    112/157    181/184    255/225    376/235    630/241
+    Qwen3-30B, bf16               27/40      41/46      68/69     100/98     165/140    280/179
+    Qwen3-30B, int8 channel       28/39      40/44      65/60      94/79     141/105    215/131
+    Qwen3-235B, fp8 block         55/55      68/80     113/116    181/172    340/262    539/341
+    DeepSeek-V3, fp8 block        74/84     132/140    241/239    473/410    941/703   1735/1124
+    DeepSeek-V3, fp8 channel      78/91     136/147    238/248    442/433    823/722   1518/1139
+    DeepSeek-V3, int8 block       89/85     151/140    277/237    528/405   1088/706   2048/1109
+    DeepSeek-V3, int8 channel     90/91     153/147    275/250    499/435    937/728   1745/1137
+    8 experts of 1024 x 512, bf16  9/26      11/26      13/26      17/26      26/26      26/27
+
+Called one by one from Python, a caller that waits for its host gains about 10 us more here.  4-bit experts
+against ``fused_experts_fp4``, 128 experts of 2048 x 768, eight a token: nvfp4 51/63 us at 4 tokens, 67/76 at 8,
+116/93 at 16, 202/110 at 32; mxfp4 28/37 at one, 58/54 at 4, 165/82 at 16; that layer costs at least 130 us
+on the host, this one 33.
 
 Same recipes as ``fused_experts`` (16-bit, fp8 and int8 w8a8 block-scaled and per-channel) and
 ``fused_experts_fp4`` (w4a4), with fewer roundings: GEMM 1 and the routes' results stay in fp32, quantised
 experts quantise the fp32 activation, 16-bit experts round it to the weights' type.  The w8a8 scales are
 amax times the rounded 1/448 or 1/127, where ``fused_experts`` divides: they may differ in the last bit,
-and with them the codes of values that lie on the border of two.
+and with them the codes of values that lie on the border of two.  Sums of int8 products are fp32 here and can
+round from 2^24 on; ``fused_experts`` keeps them in 32-bit integers.
 """
 from __future__ import annotations
 
@@ -267,15 +285,16 @@ def fused_experts_decode(
     output_dtype: Optional[torch.dtype] = None,
     out: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
-    """``fused_experts`` for 1 to 32 tokens in two kernels; arguments as there.
+    """``fused_experts`` for 1 to 32 tokens; meant for one to four, above which ``fused_experts`` is the faster
+    layer for most weights (the module's docstring has the times).
 
-    ``use_fp4_w4a4``: weights and scales as ``fused_experts_fp4`` takes them.  Routes whose id is out of
-    range or not local under ``expert_map`` add nothing; a token with none gives zeros; an expert
+    Arguments as there, without biases, ``is_gated`` (always), ``inplace`` (pass ``out=hidden_states``),
+    ``apply_router_weight_on_input`` and ``no_combine``.
+    ``use_fp4_w4a4``: weights and scales as ``fused_experts_fp4`` takes them.  Routes whose id (read as int32)
+    is out of range or not local under ``expert_map`` add nothing; a token with none gives zeros; an expert
     that a token names twice counts with the sum of its weights.  ``out``: a contiguous buffer for
     the result.  Raises ``NotImplementedError`` above 32 tokens, for sizes that are not multiples of 8
-    (16-bit), 16 (per-channel), 64 (nvfp4) or 128 (block-scaled, mxfp4).  (Four-bit rows whose codes do not
-    all fit in shared memory, 32 tokens above about 5000 hidden columns, go in two or more pairs of
-    kernels.)"""
+    (16-bit), 16 (per-channel), 64 (nvfp4) or 128 (block-scaled, mxfp4)."""
     return _decode(hidden_states, w1, w2, topk_weights, topk_ids, None, 0, False, True,
                    use_fp8_w8a8=use_fp8_w8a8, use_int8_w8a8=use_int8_w8a8, use_fp4_w4a4=use_fp4_w4a4,
                    per_channel_quant=per_channel_quant, block_shape=block_shape, w1_scale=w1_scale,

@@ -730,8 +730,9 @@ typedef struct bolt_decode_args {
   int sm_count;                /* SMs to use; 0: all (the second kernel then starts beside the first) */
 } bolt_decode_args;
 
-/* Two kernels on the stream (no sort, no copies of rows; 4-bit rows of more tokens than fit in shared memory
- * go half by half).  Sizes: hidden and inter multiples of 8
+/* Two kernels on the stream (no sort, no copies of rows), one more for 8-bit rows and one for 8-bit activations whose
+ * codes a block cannot keep; 4-bit rows of more tokens than fit in shared memory go half by half, each half by
+ * kernels of its own.  Sizes: hidden and inter multiples of 8
  * (16-bit), 16 (per-channel), 128 (block-scaled, MX) or 64 (NV); block-scaled model_dim a multiple of 128. */
 size_t bolt_moe_decode_workspace_bytes(const bolt_decode_args* args);
 /* Kernels that bolt_moe_decode launches for these sizes on the current device (pointers are not looked at);
